@@ -389,6 +389,77 @@ int32_t rvc_cuda_resample(int64_t ctx, const void* x, int32_t x_f32, int64_t n_i
 /* Peak-normalised int16 conversion (runtime/pipeline.py:1208-1213). */
 int32_t rvc_cuda_to_int16(int64_t ctx, const float* x, int64_t n, int16_t* y);
 
+/* ------------------------------------------------- attention operators
+ * Attention over states of another length, a learned relative position bias by
+ * buckets, the per-head norm of queries and keys with their rotation, and the
+ * gradient of each.  No counterpart in the reference (its attention is
+ * runtime/models/vits.py:993-1014 and runtime/models/hubert.py:1315-1400).
+ * All pointers but `desc` and `borders` are DEVICE pointers; the calls are
+ * asynchronous on `stream` (a cudaStream_t of the context's device, NULL = its
+ * default stream) and touch no memory of the context: scratch is the caller's
+ * `ws` (16-byte aligned, at least the bytes that the matching *_workspace call
+ * gives), so calls on several streams, and captured graphs, run side by side as
+ * long as each has its own.  Types: 0 = float32, 1 = bfloat16, 2 = float16.
+ * Strides count elements; the D values of a head are contiguous.
+ *
+ * desc of attention: {type, B, Hq, Hkv, Lq, Lk, D, q stride (batch, row, head),
+ * k stride (3), v stride (3), kv_lens bits (0 none, 32, 64), key_mask stride
+ * (batch, key) in bytes, causal, q_offset, buckets (0 = no bias),
+ * bidirectional, dout stride (3), out stride (3)}: 29 values.  1 <= D <= 128,
+ * Hq a multiple of Hkv.  Key j of batch entry b is alive when j < kv_lens[b]
+ * (clamped to [0, Lk]), key_mask[b, j] != 0 and, when causal, j <= i + q_offset;
+ * nothing of a dead key's k or v reaches a result, whatever it holds.  A query
+ * without a live key gives out = 0, lse = -inf and zero gradients.
+ * table [buckets, Hq] (in `type`) adds table[bucket(j - i - q_offset), h] to the
+ * scaled score; borders (host, int32) are the smallest distances of the buckets
+ * 1, 2, ... of one direction.  out [B, Lq, Hq, D] contiguous, lse [B, Hq, Lq]
+ * float32 (natural logarithm). */
+int32_t rvc_cuda_attention_workspace(int64_t ctx, const int64_t* desc, int32_t ndesc, int32_t backward,
+                                     int64_t* bytes);
+int32_t rvc_cuda_attention_device(int64_t ctx, void* stream, const int64_t* desc, int32_t ndesc, double scale,
+                                  const void* q, const void* k, const void* v, const void* kv_lens,
+                                  const uint8_t* key_mask, const void* table, const int32_t* borders, int32_t nborders,
+                                  void* out, float* lse, void* ws, int64_t ws_bytes);
+/* Gradients of the call above for dout: dq [B, Lq, Hq, D], dk and dv
+ * [B, Lk, Hkv, D], dtable [buckets, Hq] (NULL without a bias), all in `type`,
+ * contiguous, each element written; sums run in a fixed order. */
+int32_t rvc_cuda_attention_backward_device(int64_t ctx, void* stream, const int64_t* desc, int32_t ndesc, double scale,
+                                           const void* dout, const void* q, const void* k, const void* v,
+                                           const void* out, const float* lse, const void* kv_lens,
+                                           const uint8_t* key_mask, const void* table, const int32_t* borders,
+                                           int32_t nborders, void* dq, void* dk, void* dv, void* dtable, void* ws,
+                                           int64_t ws_bytes);
+/* desc of relative_bias: {type, B, H, Lq, Lk, q_offset, buckets, bidirectional,
+ * dbias stride (batch, head, row)}: 11 values.  out [H, Lq, Lk] contiguous:
+ * out[h, i, j] = table[bucket(j - i - q_offset), h]. */
+int32_t rvc_cuda_relative_bias_device(int64_t ctx, void* stream, const int64_t* desc, int32_t ndesc, const void* table,
+                                      const int32_t* borders, int32_t nborders, void* out);
+/* dtable[b, h] = sum of dbias [B, H, Lq, Lk] over the batch and the pairs of
+ * bucket b (keys contiguous). */
+int32_t rvc_cuda_relative_bias_workspace(int64_t ctx, const int64_t* desc, int32_t ndesc, int64_t* bytes);
+int32_t rvc_cuda_relative_bias_backward_device(int64_t ctx, void* stream, const int64_t* desc, int32_t ndesc,
+                                               const void* dbias, const int32_t* borders, int32_t nborders,
+                                               void* dtable, void* ws, int64_t ws_bytes);
+/* Per-head norm and rotation: y = x / sqrt(mean x^2 + eps) * w, then the pairs
+ * (a, b) of the first R values become (a c - b s, a s + b c) with c, s =
+ * cos / sin[position, pair] (float32 [P, R/2]).  Pairs are (x, x + R/2), or
+ * (2x, 2x + 1) when interleaved.  desc: {type, weight type (float32 or `type`),
+ * B, L, Hq, Hk, D, R, P, interleaved, positions bits (0: 0 .. L-1, 32, 64),
+ * positions stride (batch, row), q stride (batch, row, head), k stride (3), dqo
+ * stride (3), dko stride (3)}: 25 values; D <= 256 and R <= D even.  qo
+ * [B, L, Hq, D], ko [B, L, Hk, D] contiguous.  A row whose position is outside
+ * the table comes out as NaN. */
+int32_t rvc_cuda_qk_norm_rope_device(int64_t ctx, void* stream, const int64_t* desc, int32_t ndesc, double eps,
+                                     const void* q, const void* k, const void* q_weight, const void* k_weight,
+                                     const float* cos, const float* sin, const void* positions, void* qo, void* ko);
+int32_t rvc_cuda_qk_norm_rope_workspace(int64_t ctx, const int64_t* desc, int32_t ndesc, int64_t* bytes);
+/* Gradients for dqo, dko: dq, dk (contiguous) and the weights' [D] in the weight type. */
+int32_t rvc_cuda_qk_norm_rope_backward_device(int64_t ctx, void* stream, const int64_t* desc, int32_t ndesc, double eps,
+                                              const void* dqo, const void* dko, const void* q, const void* k,
+                                              const void* q_weight, const void* k_weight, const float* cos,
+                                              const float* sin, const void* positions, void* dq, void* dk,
+                                              void* dq_weight, void* dk_weight, void* ws, int64_t ws_bytes);
+
 #ifdef __cplusplus
 }
 #endif

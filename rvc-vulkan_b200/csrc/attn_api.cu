@@ -1,0 +1,189 @@
+// Attention operators: choice of kernel, workspace, the expanded bias and the
+// gradient of its table.
+#include "attn_common.cuh"
+#include "context.cuh"
+
+#include <algorithm>
+
+namespace rvc {
+
+namespace {
+
+constexpr int64_t kAlign = 256;
+int64_t up(int64_t n, int64_t g = kAlign) { return (n + g - 1) / g * g; }
+
+template <typename T>
+__global__ void expand_bias_kernel(const T* __restrict__ table, int H, long long ld, long long d0, float mul,
+                                   const __grid_constant__ BucketRule rule, float* __restrict__ diag) {
+  const long long x = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (x >= ld) return;
+  const int b = bucket_of(rule, x - d0);
+  for (int h = 0; h < H; ++h) diag[h * ld + x] = to_f(table[(long long)b * H + h]) * mul;
+}
+
+// sums[h][x] = sum over batch entries and query tiles of the diagonal
+// j - i = x - (Lq - 1); tile t of BM queries holds it at x - (Lq - 1) + BM - 1 + t BM.
+__global__ void diag_sums_kernel(const float* __restrict__ ws, int B, int H, int nq, int BM, long long ld,
+                                 long long Lq, long long Lk, double* __restrict__ sums) {
+  const long long x = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const int h = blockIdx.y;
+  if (x >= Lq + Lk - 1) return;
+  double s = 0.0;
+  for (int t = 0; t < nq; ++t) {
+    const long long e = x - (Lq - 1) + BM - 1 + (long long)t * BM;
+    if (e < 0 || e >= ld) continue;
+    for (int b = 0; b < B; ++b) s += ws[(((long long)b * H + h) * nq + t) * ld + e];
+  }
+  sums[h * (Lq + Lk - 1) + x] = s;
+}
+
+// One block per (bucket, head): its diagonals are a run, found with the borders.
+template <typename T>
+__global__ void bucket_sums_kernel(const double* __restrict__ sums, int H, long long Lq, long long Lk, long long q_off,
+                                   const __grid_constant__ BucketRule rule, T* __restrict__ dtable) {
+  __shared__ double red[128];
+  const int b = blockIdx.x, h = blockIdx.y;
+  // relative positions [lo, hi) of bucket b
+  const long long far = (long long)1 << 40;
+  const int half = rule.both ? rule.n / 2 : rule.n;
+  const bool ahead = rule.both && b >= half;
+  const int f = ahead ? b - half : b;
+  const long long a0 = f == 0 ? 0 : (f <= rule.nb ? rule.border[f - 1] : far), a1 = f < rule.nb ? rule.border[f] : far;
+  long long lo, hi;  // distances [a0, a1): behind r = -a, ahead r = a (a > 0)
+  if (ahead) {
+    lo = a0 > 1 ? a0 : 1;
+    hi = a1;
+  } else {
+    lo = 1 - a1;
+    hi = 1 - a0;
+    if (!rule.both && f == 0) hi = far;  // one direction: every key ahead has distance 0
+  }
+  // diagonal x holds r = x - (Lq - 1) - q_off
+  const long long x0 = max(0ll, lo + (Lq - 1) + q_off), x1 = min(Lq + Lk - 1, hi + (Lq - 1) + q_off);
+  double s = 0.0;
+  for (long long x = x0 + threadIdx.x; x < x1; x += 128) s += sums[h * (Lq + Lk - 1) + x];
+  red[threadIdx.x] = s;
+  __syncthreads();
+  for (int n = 64; n; n >>= 1) {
+    if (threadIdx.x < n) red[threadIdx.x] += red[threadIdx.x + n];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) dtable[(long long)b * H + h] = from_f<T>((float)red[0]);
+}
+
+struct Layout {
+  int64_t diag = -1, po = -1, pml = -1, delta = -1, dws = -1, sums = -1, bytes = 0;
+  int nsplit = 1, BM = 64;
+  int64_t diag_ld = 0, diag0 = 0, dws_ld = 0;
+  int nq = 0;
+};
+
+Layout plan(const AttnArgs& a, bool bias, bool backward, int sms) {
+  Layout l;
+  auto take = [&](int64_t n) {
+    const int64_t at = l.bytes;
+    l.bytes += up(n);
+    return at;
+  };
+  const int64_t rows = (int64_t)a.B * a.Hq * a.Lq;
+  if (rows == 0 || (backward && a.Lk == 0)) return l;  // no launch
+  if (bias) {
+    l.diag0 = up(a.Lq, kDiagTile);
+    l.diag_ld = l.diag0 + up(a.Lk, kDiagTile) + kDiagTile;
+    l.diag = take(4 * l.diag_ld * a.Hq);
+  }
+  if (!backward) {
+    l.nsplit = attn_mma_splits(a, sms);
+    if (l.nsplit > 1) {
+      l.po = take(4 * rows * a.D * l.nsplit);
+      l.pml = take(8 * rows * l.nsplit);
+    }
+  } else {
+    l.delta = take(4 * rows);
+    if (bias) {
+      l.nq = (int)((a.Lq + l.BM - 1) / l.BM);
+      l.dws_ld = up(a.Lk, l.BM) + l.BM;
+      l.dws = take(4 * l.dws_ld * l.nq * a.B * a.Hq);
+      l.sums = take(8 * ((int64_t)a.Lq + a.Lk - 1) * a.Hq);
+    }
+  }
+  return l;
+}
+
+template <typename P>
+P* at(void* ws, int64_t off) {
+  return off < 0 ? nullptr : reinterpret_cast<P*>(static_cast<char*>(ws) + off);
+}
+
+void apply(AttnArgs& a, const Layout& l, void* ws) {
+  a.diag = at<float>(ws, l.diag);
+  a.diag_ld = l.diag_ld;
+  a.diag0 = (int)l.diag0;
+  a.nsplit = l.nsplit;
+  a.po = at<float>(ws, l.po);
+  a.pml = at<float>(ws, l.pml);
+  a.delta = at<float>(ws, l.delta);
+  a.dws = at<float>(ws, l.dws);
+  a.dws_ld = l.dws_ld;
+}
+
+}  // namespace
+
+void attn_expand_bias(const AttnArgs& a, const void* table, const BucketRule& rule, float* diag, cudaStream_t st) {
+  const unsigned grid = (unsigned)((a.diag_ld + 255) / 256);
+  const long long d0 = a.diag0 + a.q_off;
+  switch (a.type) {
+    case kF32:
+      expand_bias_kernel<<<grid, 256, 0, st>>>((const float*)table, a.Hq, a.diag_ld, d0, kLog2e, rule, diag);
+      break;
+    case kBf16:
+      expand_bias_kernel<<<grid, 256, 0, st>>>((const __nv_bfloat16*)table, a.Hq, a.diag_ld, d0, kLog2e, rule, diag);
+      break;
+    default:
+      expand_bias_kernel<<<grid, 256, 0, st>>>((const __half*)table, a.Hq, a.diag_ld, d0, kLog2e, rule, diag);
+  }
+  note_launch();
+  RVC_CUDA_TRY(cudaGetLastError());
+}
+
+void relbias_bucket_sums(int type, int H, int64_t Lq, int64_t Lk, int64_t q_off, const double* sums,
+                         const BucketRule& rule, void* dtable, cudaStream_t st) {
+  const dim3 grid(rule.n, H);
+  switch (type) {
+    case kF32: bucket_sums_kernel<<<grid, 128, 0, st>>>(sums, H, Lq, Lk, q_off, rule, (float*)dtable); break;
+    case kBf16: bucket_sums_kernel<<<grid, 128, 0, st>>>(sums, H, Lq, Lk, q_off, rule, (__nv_bfloat16*)dtable); break;
+    default: bucket_sums_kernel<<<grid, 128, 0, st>>>(sums, H, Lq, Lk, q_off, rule, (__half*)dtable);
+  }
+  note_launch();
+  RVC_CUDA_TRY(cudaGetLastError());
+}
+
+int64_t attn_workspace(const AttnArgs& a, bool bias, bool backward, int sms) {
+  return plan(a, bias, backward, sms).bytes;
+}
+
+void attn_forward(AttnArgs a, const void* table, const BucketRule* rule, void* ws, int sms, cudaStream_t st) {
+  const Layout l = plan(a, rule != nullptr, false, sms);
+  apply(a, l, ws);
+  if (rule) attn_expand_bias(a, table, *rule, const_cast<float*>(a.diag), st);
+  attn_mma_forward(a, st);
+}
+
+void attn_backward(AttnArgs a, const void* table, const BucketRule* rule, void* dtable, void* ws, int sms,
+                   cudaStream_t st) {
+  const Layout l = plan(a, rule != nullptr, true, sms);
+  apply(a, l, ws);
+  if (rule) attn_expand_bias(a, table, *rule, const_cast<float*>(a.diag), st);
+  attn_mma_backward(a, st);
+  if (rule) {
+    double* sums = at<double>(ws, l.sums);
+    const int64_t n = (int64_t)a.Lq + a.Lk - 1;
+    diag_sums_kernel<<<dim3((unsigned)((n + 127) / 128), a.Hq), 128, 0, st>>>(a.dws, a.B, a.Hq, l.nq, l.BM, l.dws_ld, a.Lq,
+                                                                      a.Lk, sums);
+    note_launch();
+    RVC_CUDA_TRY(cudaGetLastError());
+    relbias_bucket_sums(a.type, a.Hq, a.Lq, a.Lk, a.q_off, sums, *rule, dtable, st);
+  }
+}
+
+}  // namespace rvc

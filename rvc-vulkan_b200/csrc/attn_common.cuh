@@ -1,0 +1,141 @@
+// Shared pieces of the attention operators (attention / attention_backward,
+// relative_bias, qk_norm_rope): arguments, the bucket rule of the learned
+// relative position bias, element types.
+//
+//   s_ij = scale q_i . k_j + T[bucket(j - i - q_offset), h]
+//   out_i = sum_j p_ij v_j,  p_ij = exp(s_ij - lse_i),  lse_i = log sum_j exp(s_ij)
+// over the keys j that are alive: j < kv_len, key_mask[j], and (causal)
+// j <= i + q_offset.  A row with no key alive gives out = 0, lse = -inf and
+// zero gradients.  Scores are kept in the base-2 domain (scale and bias times
+// log2 e) so that the exponential is one ex2.
+#pragma once
+
+#include "common.cuh"
+
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace rvc {
+
+struct Context;
+
+enum AttnType : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
+constexpr int kMaxBuckets = 1024;  // rows of a bias table (the rule travels as a kernel parameter, 4 KB)
+constexpr int kDiagTile = 128;     // granule of the expanded bias (one value per diagonal)
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// border[b - 1] is the smallest distance of bucket b; `nb` of them.  With both
+// directions the second half of the table's rows holds the keys ahead.
+struct BucketRule {
+  int n = 0, both = 0, nb = 0;
+  int32_t border[kMaxBuckets];
+};
+
+__host__ __device__ __forceinline__ int bucket_of(const BucketRule& r, long long rel) {
+  const long long a = r.both ? (rel < 0 ? -rel : rel) : (rel < 0 ? -rel : 0);
+  int lo = 0, hi = r.nb;  // number of borders <= a
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if ((long long)r.border[mid] <= a)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo + (r.both && rel > 0 ? r.n / 2 : 0);
+}
+
+struct AttnArgs {
+  int type = 0;
+  int B = 0, Hq = 0, Hkv = 0, Lq = 0, Lk = 0, D = 0;
+  const void *q = nullptr, *k = nullptr, *v = nullptr;
+  // strides in elements: batch, row, head (the head's D values are contiguous)
+  int64_t qs[3] = {0, 0, 0}, ks[3] = {0, 0, 0}, vs[3] = {0, 0, 0};
+  const void* lens = nullptr;  // [B] int32 or int64, clamped to [0, Lk]
+  int lens64 = 0;
+  const uint8_t* mask = nullptr;  // [B, Lk] bytes, non-zero = alive
+  int64_t mask_b = 0, mask_k = 0;
+  int causal = 0;
+  int64_t q_off = 0;
+  float scale = 0.f;             // of q . k
+  const float* diag = nullptr;   // [Hq][diag_ld]: log2 e T[bucket], index j - i + diag0; nullptr = no bias
+  int64_t diag_ld = 0;
+  int diag0 = 0;
+  void* out = nullptr;           // [B, Lq, Hq, D]
+  float* lse = nullptr;          // [B, Hq, Lq]
+  // keys split over nsplit blocks: unnormalised partial rows and their (max, sum)
+  int nsplit = 1;
+  float* po = nullptr;           // [nsplit][B][Hq][Lq][D]
+  float* pml = nullptr;          // [nsplit][B][Hq][Lq][2]
+  // backward
+  const void *dout = nullptr, *fout = nullptr;
+  int64_t dos[3] = {0, 0, 0}, os[3] = {0, 0, 0};
+  float* delta = nullptr;        // [B, Hq, Lq] rowsum(dout * out)
+  void *dq = nullptr, *dk = nullptr, *dv = nullptr;  // contiguous [B, L, H, D]
+  float* dws = nullptr;          // diagonal sums of dS: [B][Hq][query tiles][dws_ld]
+  int64_t dws_ld = 0;
+};
+
+__device__ __forceinline__ int kv_len(const AttnArgs& a, int b) {
+  if (!a.lens) return a.Lk;
+  const long long n = a.lens64 ? static_cast<const long long*>(a.lens)[b] : (long long)static_cast<const int*>(a.lens)[b];
+  return (int)(n < 0 ? 0 : (n > a.Lk ? a.Lk : n));
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+// Two values in one word, the first in the low half.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+
+inline int type_size(int t) { return t == kF32 ? 4 : 2; }
+inline bool aligned16(const AttnArgs& a, const void* p, const int64_t* s) {
+  const int64_t e = type_size(a.type);
+  return (reinterpret_cast<uintptr_t>(p) % 16 == 0) && (a.D * e % 16 == 0) && (s[0] * e % 16 == 0) &&
+         (s[1] * e % 16 == 0) && (s[2] * e % 16 == 0);
+}
+
+// ------------------------------------------------------------- entry points
+// Each queues its kernels on `st`; throws Error on a launch error.
+int64_t attn_workspace(const AttnArgs& a, bool bias, bool backward, int sms);
+void attn_forward(AttnArgs a, const void* table, const BucketRule* rule, void* ws, int sms, cudaStream_t st);
+void attn_backward(AttnArgs a, const void* table, const BucketRule* rule, void* dtable, void* ws, int sms,
+                   cudaStream_t st);
+// expanded bias: diag[h][x] = log2 e T[bucket(x - diag0 - q_off), h]
+void attn_expand_bias(const AttnArgs& a, const void* table, const BucketRule& rule, float* diag, cudaStream_t st);
+// kernels of attn_mma.cu (every type, stride and size)
+void attn_mma_forward(const AttnArgs& a, cudaStream_t st);
+void attn_mma_backward(const AttnArgs& a, cudaStream_t st);
+int attn_mma_splits(const AttnArgs& a, int sms);
+
+void relbias_forward(int type, int H, int64_t Lq, int64_t Lk, int64_t q_off, const void* table, const BucketRule& rule,
+                     void* out, cudaStream_t st);
+int64_t relbias_backward_workspace(int B, int H, int64_t Lq, int64_t Lk, int sms);
+void relbias_backward(int type, int B, int H, int64_t Lq, int64_t Lk, const int64_t* strides, int64_t q_off,
+                      const void* dbias, const BucketRule& rule, void* dtable, void* ws, int sms, cudaStream_t st);
+// diagonal sums [H][Lq + Lk - 1] (fp64) -> dtable [n][H] in `type`
+void relbias_bucket_sums(int type, int H, int64_t Lq, int64_t Lk, int64_t q_off, const double* sums,
+                         const BucketRule& rule, void* dtable, cudaStream_t st);
+
+}  // namespace rvc

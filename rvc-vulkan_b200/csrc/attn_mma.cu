@@ -1,0 +1,803 @@
+// Attention and its gradient on warp-level matrix instructions: the kernels
+// that take every type, stride, length and head dimension (<= 128), and the
+// fast ones where rows are few (one new token against long states) or the
+// type is fp32.
+//
+// 16-bit inputs go through m16n8k16 with fp32 accumulators; fp32 inputs
+// through m16n8k8 TF32 with each operand split as hi + lo (both rounded to
+// TF32's 11 bits) and three products hi.hi + hi.lo + lo.hi, which leaves about
+// 2^-22 of a product: the accuracy of an fp32 sum.  Weights P and dS enter
+// their second product rounded to the inputs' type (16-bit inputs: 2^-9 /
+// 2^-12, the rounding of the output itself) or split the same way (fp32).
+//
+// Layout: a block stages a tile of keys and values in shared memory (cp.async,
+// two stages) with 16 bytes of padding per row, so that both the row-wise and
+// the transposed fragment reads are free of bank conflicts.  Dead keys (past
+// the length or masked out) are staged as zeros: whatever the caller's buffer
+// holds there, NaN included, never meets a product.
+#include "attn_common.cuh"
+#include "context.cuh"
+#include "tc_ptx.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+namespace rvc {
+
+namespace {
+
+constexpr int kT = 128;   // threads of a block (4 warps)
+constexpr int kBN = 64;   // keys per tile
+constexpr int kBM = 64;   // query rows per block (4 warps x 16) where rows are many
+
+// ------------------------------------------------------------ fragment helpers
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t tf32_rn(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = tf32_rn(x);
+  lo = tf32_rn(x - __uint_as_float(hi));
+}
+struct Split4 {
+  uint32_t hi[4], lo[4];
+};
+__device__ __forceinline__ void mma8x3(float (&c)[4], const Split4& a, float b0, float b1) {
+  uint32_t h0, l0, h1, l1;
+  split_tf32(b0, h0, l0);
+  split_tf32(b1, h1, l1);
+  mma8(c, a.lo, h0, h1);
+  mma8(c, a.hi, l0, l1);
+  mma8(c, a.hi, h0, h1);
+}
+__device__ __forceinline__ float lds_f(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Bytes of a staged row: D values and 16 bytes, so rows start 4 banks apart.
+template <typename T, int DP> constexpr int pitch() { return DP * (int)sizeof(T) + 16; }
+
+// C[16][8 NT] (+)= A[16][DP] . B[8 NT][DP]^T; A at `a`, B at `b`, both staged rows.
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void mma_abt(float (&c)[NT][4], uint32_t a, uint32_t b, int lane) {
+  constexpr int P = pitch<T, DP>();
+  if constexpr (sizeof(T) == 2) {
+    const int mi = lane >> 3, r8 = lane & 7;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      uint32_t af[4];
+      ldsm4(af, a + ((mi & 1) * 8 + r8) * P + (kk * 16 + (mi >> 1) * 8) * 2);
+#pragma unroll
+      for (int n = 0; n < NT; n += 2) {
+        uint32_t bf[4];
+        ldsm4(bf, b + (n * 8 + (mi >> 1) * 8 + r8) * P + (kk * 16 + (mi & 1) * 8) * 2);
+        mma16(c[n], af, bf[0], bf[1], T());
+        mma16(c[n + 1], af, bf[2], bf[3], T());
+      }
+    }
+  } else {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll 2
+    for (int kk = 0; kk < DP / 8; ++kk) {
+      Split4 af;
+      const uint32_t ar = a + g * P + (kk * 8 + t) * 4;
+      split_tf32(lds_f(ar), af.hi[0], af.lo[0]);
+      split_tf32(lds_f(ar + 8 * P), af.hi[1], af.lo[1]);
+      split_tf32(lds_f(ar + 16), af.hi[2], af.lo[2]);
+      split_tf32(lds_f(ar + 8 * P + 16), af.hi[3], af.lo[3]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const uint32_t br = b + (n * 8 + g) * P + (kk * 8 + t) * 4;
+        mma8x3(c[n], af, lds_f(br), lds_f(br + 16));
+      }
+    }
+  }
+}
+
+// C[16][DP] += A[16][8 NT] . B[8 NT][DP]: A are accumulator fragments (weights),
+// B staged rows.  fp32: the contraction runs over the columns in the order
+// 2t, 2t + 1, which is the accumulators' own, so no value changes lanes.
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void mma_pb(float (&c)[DP / 8][4], const float (&p)[NT][4], uint32_t b, int lane) {
+  constexpr int P = pitch<T, DP>();
+  if constexpr (sizeof(T) == 2) {
+    const int mi = lane >> 3, r8 = lane & 7;
+#pragma unroll
+    for (int n = 0; n < NT; n += 2) {
+      const uint32_t af[4] = {pack2<T>(p[n][0], p[n][1]), pack2<T>(p[n][2], p[n][3]),
+                              pack2<T>(p[n + 1][0], p[n + 1][1]), pack2<T>(p[n + 1][2], p[n + 1][3])};
+#pragma unroll
+      for (int d = 0; d < DP / 8; d += 2) {
+        uint32_t bf[4];
+        ldsm4t(bf, b + (n * 8 + (mi & 1) * 8 + r8) * P + (d * 8 + (mi >> 1) * 8) * 2);
+        mma16(c[d], af, bf[0], bf[1], T());
+        mma16(c[d + 1], af, bf[2], bf[3], T());
+      }
+    }
+  } else {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      Split4 af;
+      split_tf32(p[n][0], af.hi[0], af.lo[0]);
+      split_tf32(p[n][2], af.hi[1], af.lo[1]);
+      split_tf32(p[n][1], af.hi[2], af.lo[2]);
+      split_tf32(p[n][3], af.hi[3], af.lo[3]);
+      const uint32_t br = b + (n * 8 + 2 * t) * P + g * 4;
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d) mma8x3(c[d], af, lds_f(br + d * 32), lds_f(br + P + d * 32));
+    }
+  }
+}
+
+// Stages `rows` rows into `dst`; row r comes from src(r), a null source is
+// staged as zeros.  Columns past D are zeros.
+template <typename T, int DP, typename F>
+__device__ __forceinline__ void stage_rows(uint32_t dst, int rows, int D, bool vec, int tid, F src) {
+  constexpr int P = pitch<T, DP>();
+  constexpr int E = 16 / (int)sizeof(T), CH = DP / E;
+  if (vec) {
+    for (int e = tid; e < rows * CH; e += kT) {
+      const int r = e / CH, c = e % CH;
+      const T* s = src(r);
+      const bool on = s != nullptr && c * E < D;
+      cp16(dst + r * P + c * 16, on ? s + c * E : nullptr, on ? 16u : 0u);
+    }
+  } else {
+    for (int e = tid; e < rows * DP; e += kT) {
+      const int r = e / DP, c = e % DP;
+      const T* s = src(r);
+      const T v = (s != nullptr && c < D) ? s[c] : from_f<T>(0.f);
+      if constexpr (sizeof(T) == 4)
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + r * P + c * 4), "f"(v) : "memory");
+      else
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + r * P + c * 2), "h"(*reinterpret_cast<const uint16_t*>(&v))
+                     : "memory");
+    }
+  }
+}
+
+// ---------------------------------------------------------------- forward
+// One block: one KV head of one batch entry, ROWS rows of the (query head in
+// the group, query) plane, and the key tiles of one split.  ROWS = 64: every
+// warp has 16 rows of its own and all 64 keys of a tile.  ROWS = 16 (few
+// rows): the warps share the rows and take 16 keys of each tile each; their
+// running (max, sum, row) are joined at the end through shared memory.
+template <typename T, int DP, int ROWS>
+__global__ void __launch_bounds__(kT) attn_mma_fwd_kernel(const __grid_constant__ AttnArgs a, int vec_q, int vec_kv) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int P = pitch<T, DP>();
+  constexpr bool SHARED = ROWS == 16;
+  constexpr int NT = SHARED ? 2 : 8;  // key groups of 8 per warp
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int G = a.Hq / a.Hkv;
+  const long long rows = (long long)G * a.Lq;
+  const unsigned ntile = (unsigned)((rows + ROWS - 1) / ROWS);
+  const int b = blockIdx.x / ntile / a.Hkv, kh = blockIdx.x / ntile % a.Hkv;
+  const long long r0 = (long long)(blockIdx.x % ntile) * ROWS;
+  const uint32_t sm = ptx::smem_u32(smem);
+  const uint32_t sQ = sm, sK = sQ + ROWS * P, sV = sK + 2 * kBN * P;
+  const int len = kv_len(a, b);
+
+  // the furthest key that a row of this block may meet
+  long long kend = len;
+  if (a.causal) {
+    const long long last = min(rows, r0 + ROWS) - 1;
+    const long long imax = (r0 / a.Lq != last / a.Lq) ? a.Lq - 1 : last % a.Lq;
+    kend = max(0ll, min(kend, imax + a.q_off + 1));
+  }
+  const int tiles = (int)((kend + kBN - 1) / kBN);
+  const int t0 = (int)((long long)tiles * blockIdx.y / a.nsplit), t1 = (int)((long long)tiles * (blockIdx.y + 1) / a.nsplit);
+
+  const T* qb = static_cast<const T*>(a.q) + (int64_t)b * a.qs[0];
+  const T* kb = static_cast<const T*>(a.k) + (int64_t)b * a.ks[0] + (int64_t)kh * a.ks[2];
+  const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.vs[0] + (int64_t)kh * a.vs[2];
+  const uint8_t* mb = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
+  stage_rows<T, DP>(sQ, ROWS, a.D, vec_q, tid, [&](int r) -> const T* {
+    const long long x = r0 + r;
+    return x < rows ? qb + (x % a.Lq) * a.qs[1] + (kh * G + x / a.Lq) * a.qs[2] : nullptr;
+  });
+  auto load = [&](int tile, int st) {
+    const int j0 = tile * kBN;
+    auto alive = [&](int r) { return j0 + r < len && (!mb || mb[(int64_t)(j0 + r) * a.mask_k]); };
+    stage_rows<T, DP>(sK + st * kBN * P, kBN, a.D, vec_kv, tid,
+                      [&](int r) -> const T* { return alive(r) ? kb + (int64_t)(j0 + r) * a.ks[1] : nullptr; });
+    stage_rows<T, DP>(sV + st * kBN * P, kBN, a.D, vec_kv, tid,
+                      [&](int r) -> const T* { return alive(r) ? vb + (int64_t)(j0 + r) * a.vs[1] : nullptr; });
+    cp_commit();
+  };
+  if (t0 < t1) load(t0, 0);
+
+  // the two rows of this thread
+  const int wr = SHARED ? 0 : warp * 16;
+  long long qi[2];
+  const float* bias[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const long long r = min(r0 + wr + g + 8 * x, rows - 1);
+    qi[x] = r % a.Lq;
+    bias[x] = a.diag ? a.diag + (kh * G + r / a.Lq) * a.diag_ld + a.diag0 - qi[x] : nullptr;
+  }
+  const float sc = a.scale * kLog2e;
+  float o[DP / 8][4];
+#pragma unroll
+  for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) o[d][x] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  for (int tile = t0; tile < t1; ++tile) {
+    const int st = (tile - t0) & 1;
+    if (tile + 1 < t1) {
+      load(tile + 1, st ^ 1);
+      cp_wait<1>();
+    } else {
+      cp_wait<0>();
+    }
+    __syncthreads();
+    const int key0 = SHARED ? warp * 16 : 0;
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[n][x] = 0.f;
+    mma_abt<T, DP, NT>(s, sQ + wr * P, sK + (st * kBN + key0) * P, lane);
+    const int j0 = tile * kBN + key0;
+    const bool whole = !mb && j0 + NT * 8 <= len && (!a.causal || j0 + NT * 8 <= min(qi[0], qi[1]) + a.q_off + 1);
+    float mx[2] = {m[0], m[1]};
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int j = j0 + n * 8 + 2 * t + (x & 1), y = x >> 1;
+        float v = s[n][x] * sc;
+        if (a.diag && j < a.Lk) v += __ldg(bias[y] + j);
+        if (!whole) {
+          const bool on = j < len && (!mb || mb[(int64_t)j * a.mask_k]) && (!a.causal || j <= qi[y] + a.q_off);
+          v = on ? v : -INFINITY;
+        }
+        s[n][x] = v;
+        mx[y] = fmaxf(mx[y], v);
+      }
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      mx[y] = fmaxf(mx[y], __shfl_xor_sync(0xffffffffu, mx[y], 1));
+      mx[y] = fmaxf(mx[y], __shfl_xor_sync(0xffffffffu, mx[y], 2));
+    }
+    const float base[2] = {mx[0] == -INFINITY ? 0.f : mx[0], mx[1] == -INFINITY ? 0.f : mx[1]};
+    const float f[2] = {exp2_approx(m[0] - base[0]), exp2_approx(m[1] - base[1])};
+    l[0] *= f[0];
+    l[1] *= f[1];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        s[n][x] = exp2_approx(s[n][x] - base[x >> 1]);
+        l[x >> 1] += s[n][x];
+      }
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o[d][x] *= f[x >> 1];
+    m[0] = mx[0];
+    m[1] = mx[1];
+    mma_pb<T, DP, NT>(o, s, sV + (st * kBN + key0) * P, lane);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
+    l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
+  }
+  if constexpr (SHARED) {  // join the four warps: rows of warp w at [w][16][DP + 4] floats, (m, l) behind
+    cp_wait<0>();
+    __syncthreads();
+    float* part = reinterpret_cast<float*>(smem);
+    constexpr int LD = DP + 4;
+    float* ml = part + 4 * 16 * LD;
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) part[(warp * 16 + g + 8 * (x >> 1)) * LD + d * 8 + 2 * t + (x & 1)] = o[d][x];
+    if (t == 0)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        ml[2 * (warp * 16 + g + 8 * y)] = m[y];
+        ml[2 * (warp * 16 + g + 8 * y) + 1] = l[y];
+      }
+    __syncthreads();
+    for (int e = tid; e < 16 * DP; e += kT) {
+      const int r = e / DP, d = e % DP;
+      const long long x = r0 + r;
+      if (x >= rows || d >= a.D) continue;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[2 * (w * 16 + r)]);
+      float L = 0.f, v = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = ml[2 * (w * 16 + r)] == -INFINITY ? 0.f : exp2_approx(ml[2 * (w * 16 + r)] - M);
+        L = fmaf(f, ml[2 * (w * 16 + r) + 1], L);
+        v = fmaf(f, part[(w * 16 + r) * LD + d], v);
+      }
+      const long long i = x % a.Lq, h = kh * G + x / a.Lq;
+      const long long row = ((long long)b * a.Hq + h) * a.Lq + i;
+      if (a.nsplit > 1) {
+        const long long pr = (long long)blockIdx.y * a.B * a.Hq * a.Lq + row;
+        a.po[pr * a.D + d] = v;
+        if (d == 0) {
+          a.pml[2 * pr] = M;
+          a.pml[2 * pr + 1] = L;
+        }
+      } else {
+        static_cast<T*>(a.out)[(((long long)b * a.Lq + i) * a.Hq + h) * a.D + d] = from_f<T>(L > 0.f ? v / L : 0.f);
+        if (d == 0) a.lse[row] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const long long x = r0 + wr + g + 8 * y;
+      if (x >= rows) continue;
+      const long long i = x % a.Lq, h = kh * G + x / a.Lq;
+      const long long row = ((long long)b * a.Hq + h) * a.Lq + i;
+      if (a.nsplit > 1) {
+        const long long pr = (long long)blockIdx.y * a.B * a.Hq * a.Lq + row;
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+          for (int z = 0; z < 2; ++z)
+            if (d * 8 + 2 * t + z < a.D) a.po[pr * a.D + d * 8 + 2 * t + z] = o[d][2 * y + z];
+        if (t == 0) {
+          a.pml[2 * pr] = m[y];
+          a.pml[2 * pr + 1] = l[y];
+        }
+      } else {
+        const float inv = l[y] > 0.f ? 1.f / l[y] : 0.f;
+        T* dst = static_cast<T*>(a.out) + (((long long)b * a.Lq + i) * a.Hq + h) * a.D;
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+          for (int z = 0; z < 2; ++z)
+            if (d * 8 + 2 * t + z < a.D) dst[d * 8 + 2 * t + z] = from_f<T>(o[d][2 * y + z] * inv);
+        if (t == 0) a.lse[row] = l[y] > 0.f ? (m[y] + log2f(l[y])) * kLn2 : -INFINITY;
+      }
+    }
+  }
+}
+
+// Joins the splits of a row: one warp per row, lanes over the head dimension.
+template <typename T>
+__global__ void attn_join_kernel(const __grid_constant__ AttnArgs a, long long rows) {
+  const long long row = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  float M = -INFINITY, L = 0.f;
+  for (int s = lane; s < a.nsplit; s += 32) M = fmaxf(M, a.pml[2 * (s * rows + row)]);
+#pragma unroll
+  for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.nsplit; ++s) {
+    const long long pr = s * rows + row;
+    const float ms = a.pml[2 * pr];
+    if (ms == -INFINITY) continue;
+    const float f = exp2_approx(ms - M);
+    L = fmaf(f, a.pml[2 * pr + 1], L);
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (lane + 32 * x < a.D) o[x] = fmaf(f, a.po[pr * a.D + lane + 32 * x], o[x]);
+  }
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const long long i = row % a.Lq, bh = row / a.Lq, b = bh / a.Hq, h = bh % a.Hq;
+  T* dst = static_cast<T*>(a.out) + ((b * a.Lq + i) * a.Hq + h) * a.D;
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    if (lane + 32 * x < a.D) dst[lane + 32 * x] = from_f<T>(o[x] * inv);
+  if (lane == 0) a.lse[row] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+}
+
+// --------------------------------------------------------------- backward
+// delta_i = dout_i . out_i, one warp per row.
+template <typename T>
+__global__ void attn_delta_kernel(const __grid_constant__ AttnArgs a, long long rows) {
+  const long long row = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const long long i = row % a.Lq, bh = row / a.Lq, b = bh / a.Hq, h = bh % a.Hq;
+  const T* x = static_cast<const T*>(a.dout) + b * a.dos[0] + i * a.dos[1] + h * a.dos[2];
+  const T* y = static_cast<const T*>(a.fout) + b * a.os[0] + i * a.os[1] + h * a.os[2];
+  float s = 0.f;
+  for (int d = lane; d < a.D; d += 32) s = fmaf(to_f(x[d]), to_f(y[d]), s);
+#pragma unroll
+  for (int z = 16; z; z >>= 1) s += __shfl_xor_sync(0xffffffffu, s, z);
+  if (lane == 0) a.delta[row] = s;
+}
+
+// dQ = scale dS K for 64 queries of one query head, with the sums of dS along
+// the diagonals of every tile when the table's gradient is wanted: thread u
+// adds the entries (y, x) with x - y = u - 63, in the order of the rows; the
+// upper half of a tile's diagonals goes on in the next tile.
+template <typename T, int DP, int BN>
+__global__ void __launch_bounds__(kT) attn_mma_dq_kernel(const __grid_constant__ AttnArgs a, int vec_q, int vec_kv,
+                                                         int vec_do) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int P = pitch<T, DP>();
+  constexpr int NT = BN / 8;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int G = a.Hq / a.Hkv;
+  const unsigned ntile = (unsigned)((a.Lq + kBM - 1) / kBM);
+  const int b = blockIdx.x / ntile / a.Hq, h = blockIdx.x / ntile % a.Hq, kh = h / G;
+  const long long i0 = (long long)(blockIdx.x % ntile) * kBM;
+  const uint32_t sm = ptx::smem_u32(smem);
+  const uint32_t sQ = sm, sO = sQ + kBM * P, sK = sO + kBM * P, sV = sK + 2 * BN * P;
+  constexpr int SL = BN + 1;
+  float* sD = reinterpret_cast<float*>(smem + 2 * kBM * P + 4 * BN * P);  // dS tile [64][BN + 1], carry behind
+  float* carry = sD + kBM * SL;
+  const int len = kv_len(a, b);
+  long long kend = len;
+  if (a.causal) kend = max(0ll, min(kend, min((long long)a.Lq, i0 + kBM) - 1 + a.q_off + 1));
+  const int tiles = (int)((kend + BN - 1) / BN);
+  const T* qb = static_cast<const T*>(a.q) + (int64_t)b * a.qs[0] + (int64_t)h * a.qs[2];
+  const T* ob = static_cast<const T*>(a.dout) + (int64_t)b * a.dos[0] + (int64_t)h * a.dos[2];
+  const T* kb = static_cast<const T*>(a.k) + (int64_t)b * a.ks[0] + (int64_t)kh * a.ks[2];
+  const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.vs[0] + (int64_t)kh * a.vs[2];
+  const uint8_t* mb = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
+  stage_rows<T, DP>(sQ, kBM, a.D, vec_q, tid,
+                    [&](int r) -> const T* { return i0 + r < a.Lq ? qb + (i0 + r) * a.qs[1] : nullptr; });
+  stage_rows<T, DP>(sO, kBM, a.D, vec_do, tid,
+                    [&](int r) -> const T* { return i0 + r < a.Lq ? ob + (i0 + r) * a.dos[1] : nullptr; });
+  auto load = [&](int tile, int st) {
+    const int j0 = tile * BN;
+    auto alive = [&](int r) { return j0 + r < len && (!mb || mb[(int64_t)(j0 + r) * a.mask_k]); };
+    stage_rows<T, DP>(sK + st * BN * P, BN, a.D, vec_kv, tid,
+                      [&](int r) -> const T* { return alive(r) ? kb + (int64_t)(j0 + r) * a.ks[1] : nullptr; });
+    stage_rows<T, DP>(sV + st * BN * P, BN, a.D, vec_kv, tid,
+                      [&](int r) -> const T* { return alive(r) ? vb + (int64_t)(j0 + r) * a.vs[1] : nullptr; });
+    cp_commit();
+  };
+  if (tiles > 0) load(0, 0);
+  long long qi[2];
+  float lse2[2], delta[2];
+  const float* bias[2];
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    qi[y] = min(i0 + warp * 16 + g + 8 * y, (long long)a.Lq - 1);
+    const long long row = ((long long)b * a.Hq + h) * a.Lq + qi[y];
+    const float z = a.lse[row];
+    const bool live = z != -INFINITY && i0 + warp * 16 + g + 8 * y < a.Lq;
+    lse2[y] = live ? z * kLog2e : INFINITY;  // a row that is not there or has no key: P = 0
+    delta[y] = a.delta[row];
+    bias[y] = a.diag ? a.diag + h * a.diag_ld + a.diag0 - qi[y] : nullptr;
+  }
+  const float sc = a.scale * kLog2e;
+  float acc[DP / 8][4];
+#pragma unroll
+  for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) acc[d][x] = 0.f;
+  float* dws = a.dws ? a.dws + (long long)blockIdx.x * a.dws_ld : nullptr;
+  if (dws && tid < kBM) carry[tid] = 0.f;
+  for (int tile = 0; tile < tiles; ++tile) {
+    const int st = tile & 1;
+    if (tile + 1 < tiles) {
+      load(tile + 1, st ^ 1);
+      cp_wait<1>();
+    } else {
+      cp_wait<0>();
+    }
+    __syncthreads();
+    float s[NT][4], dp[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[n][x] = dp[n][x] = 0.f;
+    mma_abt<T, DP, NT>(s, sQ + warp * 16 * P, sK + st * BN * P, lane);
+    mma_abt<T, DP, NT>(dp, sO + warp * 16 * P, sV + st * BN * P, lane);
+    const int j0 = tile * BN;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int j = j0 + n * 8 + 2 * t + (x & 1), y = x >> 1;
+        float v = s[n][x] * sc;
+        if (a.diag && j < a.Lk) v += __ldg(bias[y] + j);
+        const bool on = j < len && (!mb || mb[(int64_t)j * a.mask_k]) && (!a.causal || j <= qi[y] + a.q_off);
+        const float p = on ? exp2_approx(v - lse2[y]) : 0.f;
+        s[n][x] = p != 0.f ? p * (dp[n][x] - delta[y]) : 0.f;
+        if (dws) sD[(warp * 16 + g + 8 * y) * SL + n * 8 + 2 * t + (x & 1)] = s[n][x];
+      }
+    mma_pb<T, DP, NT>(acc, s, sK + st * BN * P, lane);
+    __syncthreads();
+    if (dws) {  // diagonals u = x - y + 63 of this tile, 0 <= u < 63 + BN
+      const int u = tid;
+      float v = u < kBM - 1 ? carry[u] : 0.f;
+      if (u < kBM - 1 + BN) {
+        const int d = u - (kBM - 1);
+        for (int y = max(0, -d); y < min(kBM, BN - d); ++y) v += sD[y * SL + y + d];
+        if (u < BN) dws[(long long)tile * BN + u] = v;
+      }
+      __syncthreads();
+      if (u >= BN && u < kBM - 1 + BN) carry[u - BN] = v;
+      __syncthreads();
+    }
+  }
+  if (dws) {  // the last diagonals, and zeros where no tile was
+    const long long at = (long long)tiles * BN;
+    for (long long x = at + tid; x < a.dws_ld; x += kT) dws[x] = x - at < kBM - 1 ? carry[x - at] : 0.f;
+  }
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    const long long i = i0 + warp * 16 + g + 8 * y;
+    if (i >= a.Lq) continue;
+    T* dst = static_cast<T*>(a.dq) + (((long long)b * a.Lq + i) * a.Hq + h) * a.D;
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+      for (int z = 0; z < 2; ++z)
+        if (d * 8 + 2 * t + z < a.D) dst[d * 8 + 2 * t + z] = from_f<T>(acc[d][2 * y + z] * a.scale);
+  }
+}
+
+// dK = scale sum dS^T Q and dV = sum P^T dO for 64 keys of one KV head, over
+// every query of every head of its group, BQ rows at a time.
+template <typename T, int DP, int BQ>
+__global__ void __launch_bounds__(kT) attn_mma_dkv_kernel(const __grid_constant__ AttnArgs a, int vec_q, int vec_kv,
+                                                          int vec_do) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int P = pitch<T, DP>();
+  constexpr int NT = BQ / 8;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int G = a.Hq / a.Hkv;
+  const unsigned ntile = (unsigned)((a.Lk + kBN - 1) / kBN);
+  const int b = blockIdx.x / ntile / a.Hkv, kh = blockIdx.x / ntile % a.Hkv;
+  const int j0 = (int)(blockIdx.x % ntile) * kBN;
+  const uint32_t sm = ptx::smem_u32(smem);
+  const uint32_t sK = sm, sV = sK + kBN * P, sQ = sV + kBN * P, sO = sQ + 2 * BQ * P;
+  float* stat = reinterpret_cast<float*>(smem + 2 * kBN * P + 4 * BQ * P);  // [2][2][BQ]: lse2, delta
+  const int len = kv_len(a, b);
+  const T* qb = static_cast<const T*>(a.q) + (int64_t)b * a.qs[0];
+  const T* ob = static_cast<const T*>(a.dout) + (int64_t)b * a.dos[0];
+  const T* kb = static_cast<const T*>(a.k) + (int64_t)b * a.ks[0] + (int64_t)kh * a.ks[2];
+  const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.vs[0] + (int64_t)kh * a.vs[2];
+  const uint8_t* mb = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
+  auto alive = [&](int j) { return j < len && (!mb || mb[(int64_t)j * a.mask_k]); };
+  stage_rows<T, DP>(sK, kBN, a.D, vec_kv, tid,
+                    [&](int r) -> const T* { return alive(j0 + r) ? kb + (int64_t)(j0 + r) * a.ks[1] : nullptr; });
+  stage_rows<T, DP>(sV, kBN, a.D, vec_kv, tid,
+                    [&](int r) -> const T* { return alive(j0 + r) ? vb + (int64_t)(j0 + r) * a.vs[1] : nullptr; });
+  // rows of one head at a time, so a tile never holds two heads; with a causal
+  // mask only queries with i + q_off >= j0 meet these keys
+  long long ifirst = 0;
+  if (a.causal) ifirst = max(0ll, (long long)j0 - a.q_off) / BQ * BQ;
+  const int per = j0 < len && ifirst < a.Lq ? (int)((a.Lq - ifirst + BQ - 1) / BQ) : 0;
+  const long long tiles = (long long)per * G;
+  auto load = [&](long long tile, int st) {
+    const int h = kh * G + (int)(tile / per);
+    const long long i0 = ifirst + (tile % per) * BQ;
+    stage_rows<T, DP>(sQ + st * BQ * P, BQ, a.D, vec_q, tid, [&](int r) -> const T* {
+      return i0 + r < a.Lq ? qb + (i0 + r) * a.qs[1] + (int64_t)h * a.qs[2] : nullptr;
+    });
+    stage_rows<T, DP>(sO + st * BQ * P, BQ, a.D, vec_do, tid, [&](int r) -> const T* {
+      return i0 + r < a.Lq ? ob + (i0 + r) * a.dos[1] + (int64_t)h * a.dos[2] : nullptr;
+    });
+    if (tid < BQ) {
+      const bool in = i0 + tid < a.Lq;
+      const long long row = ((long long)b * a.Hq + h) * a.Lq + i0 + tid;
+      const float z = in ? a.lse[row] : -INFINITY;
+      stat[(st * 2) * BQ + tid] = z != -INFINITY ? z * kLog2e : INFINITY;
+      stat[(st * 2 + 1) * BQ + tid] = in ? a.delta[row] : 0.f;
+    }
+    cp_commit();
+  };
+  if (tiles > 0) load(0, 0);
+  int key[2];
+  bool on[2];
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    key[y] = j0 + warp * 16 + g + 8 * y;
+    on[y] = alive(key[y]);
+  }
+  const float sc = a.scale * kLog2e;
+  float dk[DP / 8][4], dv[DP / 8][4];
+#pragma unroll
+  for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) dk[d][x] = dv[d][x] = 0.f;
+  for (long long tile = 0; tile < tiles; ++tile) {
+    const int st = (int)(tile & 1);
+    if (tile + 1 < tiles) {
+      load(tile + 1, st ^ 1);
+      cp_wait<1>();
+    } else {
+      cp_wait<0>();
+    }
+    __syncthreads();
+    const int h = kh * G + (int)(tile / per);
+    const long long i0 = ifirst + (tile % per) * BQ;
+    const float* bias = a.diag ? a.diag + h * a.diag_ld + a.diag0 : nullptr;
+    float s[NT][4], dp[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[n][x] = dp[n][x] = 0.f;
+    mma_abt<T, DP, NT>(s, sK + warp * 16 * P, sQ + st * BQ * P, lane);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int c = n * 8 + 2 * t + (x & 1), y = x >> 1;
+        const long long i = i0 + c;
+        float v = s[n][x] * sc;
+        if (bias && i < a.Lq && key[y] < a.Lk) v += __ldg(bias + key[y] - i);
+        const bool live = on[y] && (!a.causal || key[y] <= i + a.q_off);
+        s[n][x] = live ? exp2_approx(v - stat[st * 2 * BQ + c]) : 0.f;
+      }
+    mma_pb<T, DP, NT>(dv, s, sO + st * BQ * P, lane);
+    mma_abt<T, DP, NT>(dp, sV + warp * 16 * P, sO + st * BQ * P, lane);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float de = stat[(st * 2 + 1) * BQ + n * 8 + 2 * t + (x & 1)];
+        s[n][x] = s[n][x] != 0.f ? s[n][x] * (dp[n][x] - de) : 0.f;
+      }
+    mma_pb<T, DP, NT>(dk, s, sQ + st * BQ * P, lane);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    if (key[y] >= a.Lk) continue;
+    const long long at = (((long long)b * a.Lk + key[y]) * a.Hkv + kh) * a.D;
+    T* pk = static_cast<T*>(a.dk) + at;
+    T* pv = static_cast<T*>(a.dv) + at;
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+      for (int z = 0; z < 2; ++z)
+        if (d * 8 + 2 * t + z < a.D) {
+          pk[d * 8 + 2 * t + z] = from_f<T>(dk[d][2 * y + z] * a.scale);
+          pv[d * 8 + 2 * t + z] = from_f<T>(dv[d][2 * y + z]);
+        }
+  }
+}
+
+void allow_smem(const void* f, size_t smem) {
+  if (smem > 48 * 1024)
+    RVC_CUDA_TRY(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+}
+
+template <typename T, int DP>
+void fwd_dp(const AttnArgs& a, cudaStream_t st) {
+  const int vq = aligned16(a, a.q, a.qs), vkv = aligned16(a, a.k, a.ks) && aligned16(a, a.v, a.vs);
+  const long long rows = (long long)(a.Hq / a.Hkv) * a.Lq;
+  constexpr int P = pitch<T, DP>();
+  const bool few = rows <= 16;
+  const int R = few ? 16 : kBM;
+  size_t smem = (size_t)(R + 4 * kBN) * P;
+  if (few) smem = std::max(smem, (size_t)(4 * 16 * (DP + 4) + 128) * 4);
+  const dim3 grid((unsigned)((rows + R - 1) / R * a.B * a.Hkv), a.nsplit);
+  if (few) {
+    allow_smem((const void*)attn_mma_fwd_kernel<T, DP, 16>, smem);
+    attn_mma_fwd_kernel<T, DP, 16><<<grid, kT, smem, st>>>(a, vq, vkv);
+  } else {
+    allow_smem((const void*)attn_mma_fwd_kernel<T, DP, kBM>, smem);
+    attn_mma_fwd_kernel<T, DP, kBM><<<grid, kT, smem, st>>>(a, vq, vkv);
+  }
+  note_launch();
+  RVC_CUDA_TRY(cudaGetLastError());
+  if (a.nsplit > 1) {
+    const long long n = (long long)a.B * a.Hq * a.Lq;
+    attn_join_kernel<T><<<(unsigned)((n + 7) / 8), 256, 0, st>>>(a, n);
+    note_launch();
+    RVC_CUDA_TRY(cudaGetLastError());
+  }
+}
+
+template <typename T, int DP>
+void bwd_dp(const AttnArgs& a, cudaStream_t st) {
+  const int vq = aligned16(a, a.q, a.qs), vkv = aligned16(a, a.k, a.ks) && aligned16(a, a.v, a.vs),
+            vdo = aligned16(a, a.dout, a.dos);
+  constexpr int P = pitch<T, DP>();
+  constexpr int BN = sizeof(T) == 4 && DP > 64 ? 32 : 64;  // fp32 rows of 96 / 128: half the tile, to fit shared memory
+  const long long n = (long long)a.B * a.Hq * a.Lq;
+  if (n > 0) {
+    attn_delta_kernel<T><<<(unsigned)((n + 7) / 8), 256, 0, st>>>(a, n);
+    note_launch();
+    RVC_CUDA_TRY(cudaGetLastError());
+    const size_t smem = (size_t)(2 * kBM + 4 * BN) * P + (a.dws ? (size_t)(kBM * (BN + 1) + kBM) * 4 : 0);
+    allow_smem((const void*)attn_mma_dq_kernel<T, DP, BN>, smem);
+    attn_mma_dq_kernel<T, DP, BN>
+        <<<(unsigned)((a.Lq + kBM - 1ll) / kBM * a.B * a.Hq), kT, smem, st>>>(a, vq, vkv, vdo);
+    note_launch();
+    RVC_CUDA_TRY(cudaGetLastError());
+  }
+  if (a.Lk > 0) {
+    const size_t smem = (size_t)(2 * kBN + 4 * BN) * P + 4 * BN * 4;
+    allow_smem((const void*)attn_mma_dkv_kernel<T, DP, BN>, smem);
+    attn_mma_dkv_kernel<T, DP, BN>
+        <<<(unsigned)((a.Lk + kBN - 1ll) / kBN * a.B * a.Hkv), kT, smem, st>>>(a, vq, vkv, vdo);
+    note_launch();
+    RVC_CUDA_TRY(cudaGetLastError());
+  }
+}
+
+template <typename T>
+void fwd_t(const AttnArgs& a, cudaStream_t st) {
+  if (a.D <= 32) fwd_dp<T, 32>(a, st);
+  else if (a.D <= 64) fwd_dp<T, 64>(a, st);
+  else if (a.D <= 96) fwd_dp<T, 96>(a, st);
+  else fwd_dp<T, 128>(a, st);
+}
+template <typename T>
+void bwd_t(const AttnArgs& a, cudaStream_t st) {
+  if (a.D <= 32) bwd_dp<T, 32>(a, st);
+  else if (a.D <= 64) bwd_dp<T, 64>(a, st);
+  else if (a.D <= 96) bwd_dp<T, 96>(a, st);
+  else bwd_dp<T, 128>(a, st);
+}
+
+}  // namespace
+
+// Splits of the keys: enough blocks for every SM to hold a few, at least two
+// key tiles each.
+int attn_mma_splits(const AttnArgs& a, int sms) {
+  const long long rows = (long long)(a.Hq / a.Hkv) * a.Lq;
+  const int R = rows <= 16 ? 16 : kBM;
+  const long long blocks = (rows + R - 1) / R * a.B * a.Hkv;
+  const int tiles = (a.Lk + kBN - 1) / kBN;
+  if (blocks == 0 || tiles < 2) return 1;
+  const long long want = (2ll * sms + blocks - 1) / blocks;
+  return (int)std::max(1ll, std::min({want, (long long)(tiles / 2), 64ll}));
+}
+
+void attn_mma_forward(const AttnArgs& a, cudaStream_t st) {
+  switch (a.type) {
+    case kF32: return fwd_t<float>(a, st);
+    case kBf16: return fwd_t<__nv_bfloat16>(a, st);
+    default: return fwd_t<__half>(a, st);
+  }
+}
+
+void attn_mma_backward(const AttnArgs& a, cudaStream_t st) {
+  switch (a.type) {
+    case kF32: return bwd_t<float>(a, st);
+    case kBf16: return bwd_t<__nv_bfloat16>(a, st);
+    default: return bwd_t<__half>(a, st);
+  }
+}
+
+}  // namespace rvc

@@ -1,0 +1,419 @@
+"""Attention operators on device tensors, with their gradients.
+
+* ``attention`` / ``attention_backward``: softmax attention of queries over
+  keys and values of another length (an encoder's states, a cache) or their
+  own, with padded batches, shared key/value heads, a causal limit and a
+  learned bias of the distance;
+* ``relative_bias`` / ``relative_bias_backward``: that bias as a tensor, and
+  the gradient of its table from a gradient of the tensor;
+* ``qk_norm_rope`` / ``qk_norm_rope_backward``: the RMS norm of every query and
+  key head with the rotation of its position, in one pass.
+
+The functions take CUDA tensors (``torch.float32``, ``bfloat16`` or
+``float16``), run on the tensors' device and its current stream without
+synchronising, and return new contiguous tensors; scratch memory comes from
+torch's allocator, so a call can be captured into a CUDA graph.  Nothing is
+kept between calls.  ``rvc_cuda.ops`` has the forms for numpy arrays.  The
+device code and its C entry points (``include/rvc_cuda.h``) have no counterpart
+in the reference, whose attention (``runtime/models/vits.py:993-1014``,
+``runtime/models/hubert.py:1315-1400``) has one length, no padding and no
+gradient.  A shape, type or argument that is not served raises ``ValueError``.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import functools
+import math
+from typing import Optional
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import check, lib
+
+__all__ = ["BucketBias", "attention", "attention_backward", "relative_bias", "relative_bias_backward",
+           "qk_norm_rope", "qk_norm_rope_backward", "rope_table"]
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_HEAD_DIM = 128
+MAX_BUCKETS = 1024
+
+_Desc29 = C.c_int64 * 29
+_Desc25 = C.c_int64 * 25
+_Desc11 = C.c_int64 * 11
+
+
+@functools.lru_cache(maxsize=64)
+def bucket_borders(num_buckets: int, max_distance: int, bidirectional: bool = True) -> tuple:
+    """Smallest distances of the buckets 1, 2, ... of one direction.
+
+    With ``n`` buckets to a direction and ``e = n // 2``, distances below ``e``
+    have a bucket each; bucket ``e + k`` begins where ``(r / e)^(n - e)``
+    reaches ``(max_distance / e)^k``, decided on whole numbers so that no
+    rounding of a logarithm moves a border.
+    """
+    n = num_buckets // 2 if bidirectional else num_buckets
+    e = n // 2
+    borders = list(range(1, e + 1))
+    lo = e
+    for k in range(1, n - e):
+        want = max_distance ** k * e ** (n - e)
+        hi = max_distance
+        while lo < hi:  # smallest r with r^(n-e) e^k >= want
+            mid = (lo + hi) // 2
+            if mid ** (n - e) * e ** k >= want:
+                hi = mid
+            else:
+                lo = mid + 1
+        borders.append(lo)
+    return tuple(borders)
+
+
+class BucketBias:
+    """A learned bias of relative position: ``table [num_buckets, heads]``.
+
+    The bias of query ``i`` and key ``j`` is ``table[bucket(j - i), head]``.
+    ``bidirectional``: the first half of the rows holds distances of keys at or
+    behind the query, the second half those of keys ahead; otherwise every key
+    ahead counts as distance 0.  Distances of ``max_distance`` and more share
+    the last bucket.  The object holds the table itself (an optimiser may
+    change it in place between calls) and the borders of the buckets.
+    """
+
+    def __init__(self, table, max_distance: int = 128, bidirectional: bool = True):
+        if table.ndim != 2:
+            raise ValueError(f"BucketBias: table [num_buckets, heads] expected, got shape {tuple(table.shape)}")
+        n, max_distance = int(table.shape[0]), int(max_distance)
+        if bidirectional and n % 2:
+            raise ValueError(f"BucketBias: {n} buckets cannot be shared by two directions")
+        half = n // 2 if bidirectional else n
+        if half < 2 or n > MAX_BUCKETS:
+            raise ValueError(f"BucketBias: {n} buckets; 2 to {MAX_BUCKETS // (1 + bool(bidirectional))} to a direction "
+                             "are supported")
+        if not half // 2 < max_distance < 1 << 30:
+            raise ValueError(f"BucketBias: max_distance {max_distance} must exceed the {half // 2} single distances")
+        self.table = table
+        self.num_buckets, self.max_distance, self.bidirectional = n, max_distance, bool(bidirectional)
+        b = bucket_borders(n, max_distance, self.bidirectional)
+        self._borders = (C.c_int32 * max(1, len(b)))(*b)
+        self._nborders = len(b)
+
+
+# ------------------------------------------------------------------ plumbing
+
+
+def _tensor(x, name: str, ndim: int, like=None):
+    if not isinstance(x, torch.Tensor):
+        raise ValueError(f"{name}: a tensor is expected")
+    if x.dim() != ndim:
+        raise ValueError(f"{name}: {ndim} dimensions expected, got shape {tuple(x.shape)}")
+    if like is None:
+        if x.dtype not in _TYPES:
+            raise ValueError(f"{name}: float32, bfloat16 or float16 expected, got {x.dtype}")
+    else:
+        if x.dtype != like.dtype:
+            raise ValueError(f"{name}: {like.dtype} expected, got {x.dtype}")
+        if x.device != like.device:
+            raise ValueError(f"{name}: on {x.device}, expected {like.device}")
+    return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
+
+
+def _where(x):
+    """(context handle, stream of the tensor's device)."""
+    if not x.is_cuda:
+        raise ValueError(f"CUDA tensors are expected, got one on {x.device}")
+    i = x.device.index
+    return _lib.get_context(i).handle, torch.cuda.current_stream(i).cuda_stream
+
+
+def _scratch(nbytes: int, like):
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+
+
+def _ptr(x):
+    return x.data_ptr() if x is not None else None
+
+
+def _qkv(q, k, v):
+    q = _tensor(q, "q", 4)
+    k, v = _tensor(k, "k", 4, q), _tensor(v, "v", 4, q)
+    B, Lq, Hq, D = q.shape
+    Lk, Hkv = k.shape[1], k.shape[2]
+    if k.shape[0] != B or k.shape[3] != D or v.shape != k.shape:
+        raise ValueError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match "
+                         "[B, Lq, Hq, D] and [B, Lk, Hkv, D]")
+    if not 1 <= D <= MAX_HEAD_DIM:
+        raise ValueError(f"attention: head dimension {D}; 1 to {MAX_HEAD_DIM} are supported")
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"attention: {Hq} query heads are no multiple of {Hkv} key heads")
+    return q, k, v, B, Lq, Lk, Hq, Hkv, D
+
+
+def _lens(kv_lens, B: int, like):
+    if kv_lens is None:
+        return None, 0
+    if not isinstance(kv_lens, torch.Tensor) or kv_lens.device != like.device:
+        raise ValueError(f"kv_lens: a tensor on {like.device} is expected")
+    if kv_lens.shape != (B,) or kv_lens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"kv_lens: int32 or int64 [{B}] expected, got {kv_lens.dtype} {tuple(kv_lens.shape)}")
+    return kv_lens.contiguous(), 32 if kv_lens.dtype == torch.int32 else 64
+
+
+def _mask(key_mask, B: int, Lk: int, like):
+    if key_mask is None:
+        return None, 0, 0
+    if not isinstance(key_mask, torch.Tensor) or key_mask.device != like.device:
+        raise ValueError(f"key_mask: a tensor on {like.device} is expected")
+    if key_mask.shape != (B, Lk) or key_mask.dtype not in (torch.bool, torch.uint8):
+        raise ValueError(f"key_mask: bool or uint8 [{B}, {Lk}] expected, got {key_mask.dtype} {tuple(key_mask.shape)}")
+    return key_mask, key_mask.stride(0), key_mask.stride(1)
+
+
+def _table(bias, H: int, like):
+    """The table as the kernels read it (contiguous), its size and borders."""
+    if bias is None:
+        return None, 0, 0, None, 0
+    if not isinstance(bias, BucketBias):
+        raise ValueError("bias: a BucketBias is expected")
+    t = _tensor(bias.table, "bias table", 2, like)
+    if t.shape != (bias.num_buckets, H):
+        raise ValueError(f"bias: table {tuple(t.shape)}, expected [{bias.num_buckets}, {H}] for {H} query heads")
+    return t.contiguous(), bias.num_buckets, int(bias.bidirectional), bias._borders, bias._nborders
+
+
+def _scale(scale, D: int) -> float:
+    s = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not math.isfinite(s):
+        raise ValueError(f"attention: scale {s} is not finite")
+    return s
+
+
+# ----------------------------------------------------------------- attention
+
+
+def attention(q, k, v, *, kv_lens=None, key_mask=None, scale: Optional[float] = None, causal: bool = False,
+              q_offset: int = 0, bias: Optional[BucketBias] = None):
+    """Attention of ``q [B, Lq, Hq, D]`` over ``k, v [B, Lk, Hkv, D]``.
+
+    ``softmax(scale q k^T + bias) v`` over the live keys of each batch entry:
+    those before ``kv_lens [B]`` (int32 or int64, clamped to ``[0, Lk]``), with
+    ``key_mask [B, Lk]`` (bool or uint8) set, and, when ``causal``, not past
+    ``i + q_offset`` for query ``i`` (``q_offset = Lk - Lq`` aligns the last
+    query with the last key).  Whatever a dead key holds reaches no result.
+    Query head ``h`` reads key head ``h // (Hq / Hkv)``.  ``scale`` is
+    ``1 / sqrt(D)`` by default; ``bias`` adds ``table[bucket(j - i - q_offset),
+    h]``.  Returns ``out [B, Lq, Hq, D]`` in the type of ``q`` and the float32
+    log sums ``lse [B, Hq, Lq]`` that the backward pass takes; a query without
+    a live key gives 0 and ``-inf``.  Heads of 1 to 128 values; any strides
+    (the parts of a packed projection are taken where they lie).
+    """
+    q, k, v, B, Lq, Lk, Hq, Hkv, D = _qkv(q, k, v)
+    lens, bits = _lens(kv_lens, B, q)
+    mask, mb, mk = _mask(key_mask, B, Lk, q)
+    table, nb, both, borders, nborders = _table(bias, Hq, q)
+    ctx, stream = _where(q)
+    desc = _Desc29(_TYPES[q.dtype], B, Hq, Hkv, Lq, Lk, D, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], bits, mb,
+                   mk, int(bool(causal)), int(q_offset), nb, both)
+    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device)
+    need = C.c_int64(0)
+    check(lib.rvc_cuda_attention_workspace(ctx, desc, 29, 0, need))
+    ws = _scratch(need.value, q)
+    check(lib.rvc_cuda_attention_device(ctx, stream, desc, 29, _scale(scale, D), q.data_ptr(), k.data_ptr(),
+                                        v.data_ptr(), _ptr(lens), _ptr(mask), _ptr(table), borders, nborders,
+                                        out.data_ptr(), lse.data_ptr(), _ptr(ws), need.value))
+    return out, lse
+
+
+def attention_backward(dout, q, k, v, out, lse, *, kv_lens=None, key_mask=None, scale: Optional[float] = None,
+                       causal: bool = False, q_offset: int = 0, bias: Optional[BucketBias] = None):
+    """Gradients of ``attention`` for ``dout [B, Lq, Hq, D]``.
+
+    ``out`` and ``lse`` are what ``attention`` returned for the same arguments.
+    Returns ``(dq, dk, dv)``, and ``dtable [num_buckets, Hq]`` behind them when
+    a ``bias`` is given, in the types of their inputs; a key head's gradient is
+    the sum over the query heads that share it.  Dead keys and queries without
+    a live key get zeros.  Sums run in a fixed order: the same call gives the
+    same bits.
+    """
+    q, k, v, B, Lq, Lk, Hq, Hkv, D = _qkv(q, k, v)
+    dout, out = _tensor(dout, "dout", 4, q), _tensor(out, "out", 4, q)
+    if dout.shape != q.shape or out.shape != q.shape:
+        raise ValueError(f"attention_backward: dout {tuple(dout.shape)} and out {tuple(out.shape)} must have the shape "
+                         f"of q {tuple(q.shape)}")
+    if (not isinstance(lse, torch.Tensor) or lse.dtype != torch.float32 or lse.shape != (B, Hq, Lq)
+            or lse.device != q.device):
+        raise ValueError(f"attention_backward: lse must be float32 [{B}, {Hq}, {Lq}] on {q.device}")
+    lse = lse.contiguous()
+    lens, bits = _lens(kv_lens, B, q)
+    mask, mb, mk = _mask(key_mask, B, Lk, q)
+    table, nb, both, borders, nborders = _table(bias, Hq, q)
+    ctx, stream = _where(q)
+    desc = _Desc29(_TYPES[q.dtype], B, Hq, Hkv, Lq, Lk, D, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], bits, mb,
+                   mk, int(bool(causal)), int(q_offset), nb, both, *dout.stride()[:3], *out.stride()[:3])
+    dq = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
+    dk = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=q.device)
+    dv = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=q.device)
+    dtable = torch.empty((nb, Hq), dtype=q.dtype, device=q.device) if nb else None
+    need = C.c_int64(0)
+    check(lib.rvc_cuda_attention_workspace(ctx, desc, 29, 1, need))
+    ws = _scratch(need.value, q)
+    check(lib.rvc_cuda_attention_backward_device(
+        ctx, stream, desc, 29, _scale(scale, D), dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        out.data_ptr(), lse.data_ptr(), _ptr(lens), _ptr(mask), _ptr(table), borders, nborders, dq.data_ptr(),
+        dk.data_ptr(), dv.data_ptr(), _ptr(dtable), _ptr(ws), need.value))
+    return (dq, dk, dv) if dtable is None else (dq, dk, dv, dtable)
+
+
+# ------------------------------------------------------------- bias of distance
+
+
+def relative_bias(bias: BucketBias, Lq: int, Lk: int, *, q_offset: int = 0):
+    """The bias as a tensor: ``[heads, Lq, Lk]`` in the table's type, entry
+    ``(h, i, j)`` is ``table[bucket(j - i - q_offset), h]``."""
+    if not isinstance(bias, BucketBias):
+        raise ValueError("relative_bias: a BucketBias is expected")
+    t = _tensor(bias.table, "bias table", 2).contiguous()
+    Lq, Lk, H = int(Lq), int(Lk), t.shape[1]
+    if Lq < 0 or Lk < 0:
+        raise ValueError(f"relative_bias: lengths {Lq} and {Lk}")
+    ctx, stream = _where(t)
+    out = torch.empty((H, Lq, Lk), dtype=t.dtype, device=t.device)
+    desc = _Desc11(_TYPES[t.dtype], 1, H, Lq, Lk, int(q_offset), bias.num_buckets, int(bias.bidirectional))
+    check(lib.rvc_cuda_relative_bias_device(ctx, stream, desc, 11, t.data_ptr(), bias._borders, bias._nborders,
+                                            out.data_ptr()))
+    return out
+
+
+def relative_bias_backward(bias: BucketBias, dbias, *, q_offset: int = 0):
+    """Gradient of the table from ``dbias [heads, Lq, Lk]``, or ``[B, heads, Lq,
+    Lk]`` for a bias that was broadcast over a batch: ``[num_buckets, heads]``
+    in the type of the table.  Sums are held in 32 bits along a diagonal's part
+    and in 64 bits beyond, in a fixed order."""
+    if not isinstance(bias, BucketBias):
+        raise ValueError("relative_bias_backward: a BucketBias is expected")
+    if isinstance(dbias, torch.Tensor) and dbias.dim() == 3:
+        dbias = dbias[None]
+    d = _tensor(dbias, "dbias", 4, bias.table)
+    if d.dtype not in _TYPES:
+        raise ValueError(f"dbias: float32, bfloat16 or float16 expected, got {d.dtype}")
+    B, H, Lq, Lk = d.shape
+    if H != bias.table.shape[1]:
+        raise ValueError(f"relative_bias_backward: {H} heads, the table has {bias.table.shape[1]}")
+    ctx, stream = _where(d)
+    desc = _Desc11(_TYPES[d.dtype], B, H, Lq, Lk, int(q_offset), bias.num_buckets, int(bias.bidirectional),
+                   *d.stride()[:3])
+    dtable = torch.empty((bias.num_buckets, H), dtype=d.dtype, device=d.device)
+    need = C.c_int64(0)
+    check(lib.rvc_cuda_relative_bias_workspace(ctx, desc, 11, need))
+    ws = _scratch(need.value, d)
+    check(lib.rvc_cuda_relative_bias_backward_device(ctx, stream, desc, 11, d.data_ptr(), bias._borders,
+                                                     bias._nborders, dtable.data_ptr(), _ptr(ws), need.value))
+    return dtable
+
+
+# ---------------------------------------------------------- norm and rotation
+
+
+def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0, device=None):
+    """Cosines and sines ``[max_positions, rotary_dim / 2]`` (float32) of the
+    angles ``position * base^(-2 i / rotary_dim)``, formed in 64 bits."""
+    if rotary_dim < 2 or rotary_dim % 2 or max_positions < 1:
+        raise ValueError(f"rope_table: {max_positions} positions, rotary dimension {rotary_dim}")
+    f = float(base) ** (-np.arange(0, rotary_dim, 2, dtype=np.float64) / rotary_dim)
+    a = np.arange(max_positions, dtype=np.float64)[:, None] * f
+    device = torch.device("cuda") if device is None else device
+    return (torch.from_numpy(np.cos(a).astype(np.float32)).to(device),
+            torch.from_numpy(np.sin(a).astype(np.float32)).to(device))
+
+
+def _rope(q, k, q_weight, k_weight, cos, sin, positions, interleaved, name):
+    q = _tensor(q, "q", 4)
+    k = _tensor(k, "k", 4, q)
+    B, L, Hq, D = q.shape
+    Hk = k.shape[2]
+    if k.shape[:2] != q.shape[:2] or k.shape[3] != D:
+        raise ValueError(f"{name}: q {tuple(q.shape)} and k {tuple(k.shape)} do not match [B, L, heads, D]")
+    if D < 2 or D > 256 or D % 2:
+        raise ValueError(f"{name}: head dimension {D}; even ones from 2 to 256 are supported")
+    for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if not isinstance(w, torch.Tensor) or w.shape != (D,) or w.device != q.device:
+            raise ValueError(f"{name}: {n} [{D}] on {q.device} expected")
+        if w.dtype not in (torch.float32, q.dtype) or w.dtype != q_weight.dtype:
+            raise ValueError(f"{name}: the weights are both float32 or both {q.dtype}")
+    for t, n in ((cos, "cos"), (sin, "sin")):
+        if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.dtype != torch.float32 or t.device != q.device:
+            raise ValueError(f"{name}: {n} must be a float32 [positions, rotary_dim / 2] on {q.device}")
+    if cos.shape != sin.shape or 2 * cos.shape[1] > D:
+        raise ValueError(f"{name}: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} do not fit head dimension {D}")
+    bits = pb = pl = 0
+    if positions is not None:
+        if not isinstance(positions, torch.Tensor) or positions.device != q.device:
+            raise ValueError(f"{name}: positions must be a tensor on {q.device}")
+        if positions.dtype not in (torch.int32, torch.int64) or positions.shape not in ((B, L), (L,)):
+            raise ValueError(f"{name}: positions int32 or int64 [{B}, {L}] or [{L}] expected, got {positions.dtype} "
+                             f"{tuple(positions.shape)}")
+        bits = 32 if positions.dtype == torch.int32 else 64
+        positions = positions.expand(B, L)
+        pb, pl = positions.stride()
+    elif L > cos.shape[0] and cos.shape[1]:
+        raise ValueError(f"{name}: the tables hold {cos.shape[0]} positions, fewer than the {L} rows")
+    if B * L == 0:
+        positions = None
+        bits = 0
+    head = (_TYPES[q.dtype], _TYPES[q_weight.dtype], B, L, Hq, Hk, D, 2 * cos.shape[1], cos.shape[0],
+            int(bool(interleaved)), bits, pb, pl)
+    return q, k, q_weight.contiguous(), k_weight.contiguous(), cos.contiguous(), sin.contiguous(), positions, head
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps: float = 1e-6, interleaved: bool = False):
+    """RMS norm of each head of ``q [B, L, Hq, D]`` and ``k [B, L, Hk, D]`` with
+    ``q_weight`` / ``k_weight [D]`` (float32 or the type of ``q``), then the
+    rotation of its position, in one pass: ``(q', k')``, contiguous.
+
+    ``cos``, ``sin [P, R / 2]`` (float32, ``rope_table``) rotate the first ``R``
+    values of a head: pairs ``(x, x + R / 2)``, or ``(2x, 2x + 1)`` when
+    ``interleaved``.  ``positions [B, L]`` or ``[L]`` (int32 or int64) are rows
+    of the tables, ``0 .. L - 1`` by default; a row whose position lies outside
+    them comes out as NaN.
+    """
+    q, k, wq, wk, cos, sin, pos, head = _rope(q, k, q_weight, k_weight, cos, sin, positions, interleaved,
+                                              "qk_norm_rope")
+    ctx, stream = _where(q)
+    desc = _Desc25(*head, *q.stride()[:3], *k.stride()[:3])
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    check(lib.rvc_cuda_qk_norm_rope_device(ctx, stream, desc, 25, float(eps), q.data_ptr(), k.data_ptr(),
+                                           wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ptr(pos),
+                                           qo.data_ptr(), ko.data_ptr()))
+    return qo, ko
+
+
+def qk_norm_rope_backward(dqo, dko, q, k, q_weight, k_weight, cos, sin, *, positions=None, eps: float = 1e-6,
+                          interleaved: bool = False):
+    """Gradients of ``qk_norm_rope`` for ``dqo``, ``dko``: ``(dq, dk, dq_weight,
+    dk_weight)``, each in the type of its input; the weights' sums over the rows
+    are held in 32 and 64 bits and run in a fixed order."""
+    q, k, wq, wk, cos, sin, pos, head = _rope(q, k, q_weight, k_weight, cos, sin, positions, interleaved,
+                                              "qk_norm_rope_backward")
+    gq, gk = _tensor(dqo, "dqo", 4, q), _tensor(dko, "dko", 4, q)
+    if gq.shape != q.shape or gk.shape != k.shape:
+        raise ValueError(f"qk_norm_rope_backward: dqo {tuple(gq.shape)}, dko {tuple(gk.shape)} for q {tuple(q.shape)}, "
+                         f"k {tuple(k.shape)}")
+    ctx, stream = _where(q)
+    desc = _Desc25(*head, *q.stride()[:3], *k.stride()[:3], *gq.stride()[:3], *gk.stride()[:3])
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
+    if k.shape[2] == 0:
+        dwk.zero_()
+    need = C.c_int64(0)
+    check(lib.rvc_cuda_qk_norm_rope_workspace(ctx, desc, 25, need))
+    ws = _scratch(need.value, q)
+    check(lib.rvc_cuda_qk_norm_rope_backward_device(
+        ctx, stream, desc, 25, float(eps), gq.data_ptr(), gk.data_ptr(), q.data_ptr(), k.data_ptr(), wq.data_ptr(),
+        wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ptr(pos), dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(),
+        dwk.data_ptr(), _ptr(ws), need.value))
+    return dq, dk, dwq, dwk

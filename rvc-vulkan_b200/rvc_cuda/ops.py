@@ -22,7 +22,8 @@ from ._lib import check, fptr, iptr, lib
 __all__ = [
     "matmul", "add", "mul", "relu", "conv1d", "conv_transpose1d", "embedding",
     "add_inplace", "mul_inplace", "layer_norm", "softmax", "leaky_relu", "gelu",
-    "gating", "rel_attention", "im2col_1d",
+    "gating", "rel_attention", "im2col_1d", "attention", "attention_backward", "relative_bias",
+    "relative_bias_backward", "qk_norm_rope", "qk_norm_rope_backward",
 ]
 
 
@@ -302,3 +303,90 @@ def im2col_1d(x, kernel_size, stride=1, padding=0, dilation=1):
     if oL > 0:
         check(lib.rvc_cuda_im2col1d(_ctx(), fptr(x), B, Cc, T, K, int(stride), pl, int(dilation), oL, fptr(out)))
     return out
+
+
+# ------------------------------------------------------- attention operators
+# Host forms of rvc_cuda.attention: float32 numpy arrays in and out, on the
+# default context's device.
+
+
+def _on_device(fn, arrays, **kw):
+    """``fn`` of ``rvc_cuda.attention`` on device copies of ``arrays``."""
+    import torch  # noqa: PLC0415
+
+    dev = torch.device("cuda", _lib.get_context().device)
+
+    def up(a, dtype):
+        return torch.from_numpy(np.ascontiguousarray(a, dtype=dtype)).to(dev)
+
+    for n in ("kv_lens", "positions"):
+        if kw.get(n) is not None:
+            if not np.issubdtype(np.asarray(kw[n]).dtype, np.integer):
+                raise ValueError(f"{n}: integers are expected")
+            kw[n] = up(kw[n], np.int64)
+    if kw.get("key_mask") is not None:
+        kw["key_mask"] = up(kw["key_mask"], np.bool_)
+    if kw.get("bias") is not None:
+        kw["bias"] = _device_bias(kw["bias"], dev)
+    r = fn(*[up(a, np.float32) for a in arrays], **kw)
+    return tuple(x.cpu().numpy() for x in r) if isinstance(r, tuple) else r.cpu().numpy()
+
+
+def _device_bias(bias, dev):
+    import torch  # noqa: PLC0415
+
+    from . import attention as A  # noqa: PLC0415
+
+    if not isinstance(bias, A.BucketBias):
+        raise ValueError("bias: an rvc_cuda.attention.BucketBias is expected")
+    t = torch.from_numpy(_f32(bias.table)).to(dev)
+    return A.BucketBias(t, bias.max_distance, bias.bidirectional)
+
+
+def attention(q, k, v, kv_lens=None, key_mask=None, scale=None, causal=False, q_offset=0, bias=None):
+    """``rvc_cuda.attention.attention`` for numpy arrays: ``q [B, Lq, Hq, D]``,
+    ``k, v [B, Lk, Hkv, D]`` -> ``(out, lse)``; the table of ``bias`` (a
+    ``BucketBias``) is a numpy array too."""
+    from . import attention as A  # noqa: PLC0415
+
+    return _on_device(A.attention, (q, k, v), kv_lens=kv_lens, key_mask=key_mask, scale=scale, causal=causal,
+                      q_offset=q_offset, bias=bias)
+
+
+def attention_backward(dout, q, k, v, out, lse, kv_lens=None, key_mask=None, scale=None, causal=False, q_offset=0,
+                       bias=None):
+    """``rvc_cuda.attention.attention_backward`` for numpy arrays."""
+    from . import attention as A  # noqa: PLC0415
+
+    return _on_device(A.attention_backward, (dout, q, k, v, out, lse), kv_lens=kv_lens, key_mask=key_mask, scale=scale,
+                      causal=causal, q_offset=q_offset, bias=bias)
+
+
+def relative_bias(bias, Lq, Lk, q_offset=0):
+    """``rvc_cuda.attention.relative_bias`` with a numpy table -> ``[heads, Lq, Lk]``."""
+    from . import attention as A  # noqa: PLC0415
+
+    return _on_device(lambda **kw: A.relative_bias(kw["bias"], Lq, Lk, q_offset=q_offset), (), bias=bias)
+
+
+def relative_bias_backward(bias, dbias, q_offset=0):
+    """``rvc_cuda.attention.relative_bias_backward`` for numpy arrays."""
+    from . import attention as A  # noqa: PLC0415
+
+    return _on_device(lambda d, bias: A.relative_bias_backward(bias, d, q_offset=q_offset), (dbias,), bias=bias)
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, interleaved=False):
+    """``rvc_cuda.attention.qk_norm_rope`` for numpy arrays."""
+    from . import attention as A  # noqa: PLC0415
+
+    return _on_device(A.qk_norm_rope, (q, k, q_weight, k_weight, cos, sin), positions=positions, eps=eps,
+                      interleaved=interleaved)
+
+
+def qk_norm_rope_backward(dqo, dko, q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, interleaved=False):
+    """``rvc_cuda.attention.qk_norm_rope_backward`` for numpy arrays."""
+    from . import attention as A  # noqa: PLC0415
+
+    return _on_device(A.qk_norm_rope_backward, (dqo, dko, q, k, q_weight, k_weight, cos, sin), positions=positions,
+                      eps=eps, interleaved=interleaved)
