@@ -21,25 +21,37 @@ __global__ void expand_bias_kernel(const T* __restrict__ table, int H, long long
   for (int h = 0; h < H; ++h) diag[h * ld + x] = to_f(table[(long long)b * H + h]) * mul;
 }
 
-// sums[h][x] = sum over batch entries and query tiles of the diagonal
-// j - i = x - (Lq - 1); tile t of BM queries holds it at x - (Lq - 1) + BM - 1 + t BM.
-__global__ void diag_sums_kernel(const float* __restrict__ ws, int B, int H, int nq, int BM, long long ld,
-                                 long long Lq, long long Lk, double* __restrict__ sums) {
+// sums[h][x] = sum over batch entries and tiles of the diagonal j - i = x - (Lq - 1).
+// Tiles of BM queries (by_key = 0) hold it at x - (Lq - 1) + BM - 1 + t BM, tiles
+// of BM keys at (Lq - 1) - x + BM - 1 + t BM; there the last two entries of a
+// tile are sums that lie whole in the last bucket behind / ahead.
+__global__ void diag_sums_kernel(const float* __restrict__ ws, int B, int H, int nt, int BM, int by_key, long long ld,
+                                 long long Lq, long long Lk, double* __restrict__ sums, double* __restrict__ far) {
   const long long x = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   const int h = blockIdx.y;
-  if (x >= Lq + Lk - 1) return;
+  const long long n = Lq + Lk - 1;
+  if (x >= n + 2) return;
   double s = 0.0;
-  for (int t = 0; t < nq; ++t) {
-    const long long e = x - (Lq - 1) + BM - 1 + (long long)t * BM;
-    if (e < 0 || e >= ld) continue;
-    for (int b = 0; b < B; ++b) s += ws[(((long long)b * H + h) * nq + t) * ld + e];
+  if (x < n) {
+    const long long d = x - (Lq - 1), top = by_key ? ld - 2 : ld;
+    for (int t = 0; t < nt; ++t) {
+      const long long e = (by_key ? -d : d) + BM - 1 + (long long)t * BM;
+      if (e < 0 || e >= top) continue;
+      for (int b = 0; b < B; ++b) s += ws[(((long long)b * H + h) * nt + t) * ld + e];
+    }
+    sums[h * n + x] = s;
+  } else {
+    if (by_key)
+      for (long long e = 0; e < (long long)B * nt; ++e)
+        s += ws[(((e / nt) * H + h) * nt + e % nt) * ld + ld - 2 + (x - n)];
+    far[h * 2 + (x - n)] = s;
   }
-  sums[h * (Lq + Lk - 1) + x] = s;
 }
 
 // One block per (bucket, head): its diagonals are a run, found with the borders.
 template <typename T>
-__global__ void bucket_sums_kernel(const double* __restrict__ sums, int H, long long Lq, long long Lk, long long q_off,
+__global__ void bucket_sums_kernel(const double* __restrict__ sums, const double* __restrict__ far_sums, int H,
+                                   long long Lq, long long Lk, long long q_off,
                                    const __grid_constant__ BucketRule rule, T* __restrict__ dtable) {
   __shared__ double red[128];
   const int b = blockIdx.x, h = blockIdx.y;
@@ -62,6 +74,10 @@ __global__ void bucket_sums_kernel(const double* __restrict__ sums, int H, long 
   const long long x0 = max(0ll, lo + (Lq - 1) + q_off), x1 = min(Lq + Lk - 1, hi + (Lq - 1) + q_off);
   double s = 0.0;
   for (long long x = x0 + threadIdx.x; x < x1; x += 128) s += sums[h * (Lq + Lk - 1) + x];
+  if (far_sums && threadIdx.x == 0) {
+    if (!ahead && f == rule.nb) s += far_sums[2 * h];
+    if (rule.both ? ahead && f == rule.nb : f == 0) s += far_sums[2 * h + 1];
+  }
   red[threadIdx.x] = s;
   __syncthreads();
   for (int n = 64; n; n >>= 1) {
@@ -72,14 +88,15 @@ __global__ void bucket_sums_kernel(const double* __restrict__ sums, int H, long 
 }
 
 struct Layout {
-  int64_t diag = -1, po = -1, pml = -1, delta = -1, dws = -1, sums = -1, bytes = 0;
-  int nsplit = 1, BM = 64;
-  int64_t diag_ld = 0, diag0 = 0, dws_ld = 0;
-  int nq = 0;
+  int64_t diag = -1, po = -1, pml = -1, delta = -1, lse2 = -1, dws = -1, sums = -1, far = -1, bytes = 0;
+  int nsplit = 1, BM = 64, nt = 0;
+  int64_t diag_ld = 0, diag0 = 0, dws_ld = 0, row_ld = 0;
+  bool tc = false;
 };
 
-Layout plan(const AttnArgs& a, bool bias, bool backward, int sms) {
+Layout plan(const AttnArgs& a, bool bias, bool backward, int sms, bool tc) {
   Layout l;
+  l.tc = tc;
   auto take = [&](int64_t n) {
     const int64_t at = l.bytes;
     l.bytes += up(n);
@@ -89,26 +106,33 @@ Layout plan(const AttnArgs& a, bool bias, bool backward, int sms) {
   if (rows == 0 || (backward && a.Lk == 0)) return l;  // no launch
   if (bias) {
     l.diag0 = up(a.Lq, kDiagTile);
-    l.diag_ld = l.diag0 + up(a.Lk, kDiagTile) + kDiagTile;
+    l.diag_ld = l.diag0 + up(a.Lk, 128) + 128;
     l.diag = take(4 * l.diag_ld * a.Hq);
   }
   if (!backward) {
-    l.nsplit = attn_mma_splits(a, sms);
+    l.nsplit = tc ? 1 : attn_mma_splits(a, sms);
     if (l.nsplit > 1) {
       l.po = take(4 * rows * a.D * l.nsplit);
       l.pml = take(8 * rows * l.nsplit);
     }
-  } else {
-    l.delta = take(4 * rows);
-    if (bias) {
-      l.nq = (int)((a.Lq + l.BM - 1) / l.BM);
-      l.dws_ld = up(a.Lk, l.BM) + l.BM;
-      l.dws = take(4 * l.dws_ld * l.nq * a.B * a.Hq);
-      l.sums = take(8 * ((int64_t)a.Lq + a.Lk - 1) * a.Hq);
-    }
+    return l;
+  }
+  l.row_ld = tc ? up(a.Lq, 128) : a.Lq;
+  l.delta = take(4 * l.row_ld * a.B * a.Hq);
+  if (tc) l.lse2 = take(4 * l.row_ld * a.B * a.Hq);
+  if (bias) {
+    l.BM = tc ? 128 : 64;
+    const int64_t tiled = tc ? a.Lk : a.Lq, along = tc ? a.Lq : a.Lk;
+    l.nt = (int)((tiled + l.BM - 1) / l.BM);
+    l.dws_ld = up(along, l.BM) + l.BM + (tc ? 2 : 0);
+    l.dws = take(4 * l.dws_ld * l.nt * a.B * a.Hq);
+    l.sums = take(8 * ((int64_t)a.Lq + a.Lk - 1) * a.Hq);
+    l.far = take(16 * a.Hq);
   }
   return l;
 }
+
+bool use_tc(const AttnArgs& a, bool backward) { return backward ? attn_tc_bwd_fits(a) : attn_tc_fits(a); }
 
 template <typename P>
 P* at(void* ws, int64_t off) {
@@ -123,6 +147,8 @@ void apply(AttnArgs& a, const Layout& l, void* ws) {
   a.po = at<float>(ws, l.po);
   a.pml = at<float>(ws, l.pml);
   a.delta = at<float>(ws, l.delta);
+  a.lse2 = at<float>(ws, l.lse2);
+  a.row_ld = l.row_ld;
   a.dws = at<float>(ws, l.dws);
   a.dws_ld = l.dws_ld;
 }
@@ -147,42 +173,55 @@ void attn_expand_bias(const AttnArgs& a, const void* table, const BucketRule& ru
 }
 
 void relbias_bucket_sums(int type, int H, int64_t Lq, int64_t Lk, int64_t q_off, const double* sums,
-                         const BucketRule& rule, void* dtable, cudaStream_t st) {
+                         const double* far, const BucketRule& rule, void* dtable, cudaStream_t st) {
   const dim3 grid(rule.n, H);
   switch (type) {
-    case kF32: bucket_sums_kernel<<<grid, 128, 0, st>>>(sums, H, Lq, Lk, q_off, rule, (float*)dtable); break;
-    case kBf16: bucket_sums_kernel<<<grid, 128, 0, st>>>(sums, H, Lq, Lk, q_off, rule, (__nv_bfloat16*)dtable); break;
-    default: bucket_sums_kernel<<<grid, 128, 0, st>>>(sums, H, Lq, Lk, q_off, rule, (__half*)dtable);
+    case kF32: bucket_sums_kernel<<<grid, 128, 0, st>>>(sums, far, H, Lq, Lk, q_off, rule, (float*)dtable); break;
+    case kBf16: bucket_sums_kernel<<<grid, 128, 0, st>>>(sums, far, H, Lq, Lk, q_off, rule, (__nv_bfloat16*)dtable); break;
+    default: bucket_sums_kernel<<<grid, 128, 0, st>>>(sums, far, H, Lq, Lk, q_off, rule, (__half*)dtable);
   }
   note_launch();
   RVC_CUDA_TRY(cudaGetLastError());
 }
 
+// Enough for either choice of kernel: the choice asks for aligned pointers,
+// which a query for the size does not have.
 int64_t attn_workspace(const AttnArgs& a, bool bias, bool backward, int sms) {
-  return plan(a, bias, backward, sms).bytes;
+  const int64_t n = plan(a, bias, backward, sms, false).bytes;
+  return use_tc(a, backward) ? std::max(n, plan(a, bias, backward, sms, true).bytes) : n;
 }
 
 void attn_forward(AttnArgs a, const void* table, const BucketRule* rule, void* ws, int sms, cudaStream_t st) {
-  const Layout l = plan(a, rule != nullptr, false, sms);
+  const Layout l = plan(a, rule != nullptr, false, sms, use_tc(a, false));
   apply(a, l, ws);
   if (rule) attn_expand_bias(a, table, *rule, const_cast<float*>(a.diag), st);
-  attn_mma_forward(a, st);
+  if (l.tc)
+    attn_tc_forward(a, st);
+  else
+    attn_mma_forward(a, st);
 }
 
 void attn_backward(AttnArgs a, const void* table, const BucketRule* rule, void* dtable, void* ws, int sms,
                    cudaStream_t st) {
-  const Layout l = plan(a, rule != nullptr, true, sms);
+  const Layout l = plan(a, rule != nullptr, true, sms, use_tc(a, true));
   apply(a, l, ws);
-  if (rule) attn_expand_bias(a, table, *rule, const_cast<float*>(a.diag), st);
-  attn_mma_backward(a, st);
   if (rule) {
-    double* sums = at<double>(ws, l.sums);
-    const int64_t n = (int64_t)a.Lq + a.Lk - 1;
-    diag_sums_kernel<<<dim3((unsigned)((n + 127) / 128), a.Hq), 128, 0, st>>>(a.dws, a.B, a.Hq, l.nq, l.BM, l.dws_ld, a.Lq,
-                                                                      a.Lk, sums);
+    a.far = rule->nb ? rule->border[rule->nb - 1] : 1;
+    a.far_both = rule->both;
+    attn_expand_bias(a, table, *rule, const_cast<float*>(a.diag), st);
+  }
+  if (l.tc)
+    attn_tc_backward(a, st);
+  else
+    attn_mma_backward(a, st);
+  if (rule) {
+    double *sums = at<double>(ws, l.sums), *far = at<double>(ws, l.far);
+    const int64_t n = (int64_t)a.Lq + a.Lk + 1;
+    diag_sums_kernel<<<dim3((unsigned)((n + 127) / 128), a.Hq), 128, 0, st>>>(
+        a.dws, a.B, a.Hq, l.nt, l.BM, l.tc ? 1 : 0, l.dws_ld, a.Lq, a.Lk, sums, far);
     note_launch();
     RVC_CUDA_TRY(cudaGetLastError());
-    relbias_bucket_sums(a.type, a.Hq, a.Lq, a.Lk, a.q_off, sums, *rule, dtable, st);
+    relbias_bucket_sums(a.type, a.Hq, a.Lq, a.Lk, a.q_off, sums, far, *rule, dtable, st);
   }
 }
 

@@ -128,7 +128,7 @@ int32_t rvc_cuda_attention_device(int64_t ctx, void* stream, const int64_t* desc
     RVC_CHECK_ARG((desc[16] != 0) == (kv_lens != nullptr), "attention: kv_lens and their width do not agree");
     RVC_CHECK_ARG((desc[21] != 0) == (table != nullptr), "attention: table and bucket count do not agree");
     a.q = q, a.k = k, a.v = v, a.lens = kv_lens, a.mask = key_mask;
-    a.out = out, a.lse = lse, a.scale = (float)scale;
+    a.out = out, a.lse = lse, a.scale = (float)scale, a.err = c->d_err;
     BucketRule rule;
     if (desc[21]) rule = bucket_rule(desc[21], desc[22], borders, nborders, who);
     check_ws(who, ws, ws_bytes, attn_workspace(a, desc[21] > 0, false, c->num_sms()));
@@ -173,7 +173,7 @@ int32_t rvc_cuda_attention_backward_device(int64_t ctx, void* stream, const int6
     }
     a.q = q, a.k = k, a.v = v, a.lens = kv_lens, a.mask = key_mask;
     a.dout = dout, a.fout = out, a.lse = const_cast<float*>(lse), a.scale = (float)scale;
-    a.dq = dq, a.dk = dk, a.dv = dv;
+    a.dq = dq, a.dk = dk, a.dv = dv, a.err = c->d_err;
     check_ws(who, ws, ws_bytes, attn_workspace(a, desc[21] > 0, true, c->num_sms()));
     attn_backward(a, table, desc[21] ? &rule : nullptr, dtable, ws, c->num_sms(), st);
   });

@@ -21,7 +21,7 @@ struct Context;
 
 enum AttnType : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
 constexpr int kMaxBuckets = 1024;  // rows of a bias table (the rule travels as a kernel parameter, 4 KB)
-constexpr int kDiagTile = 128;     // granule of the expanded bias (one value per diagonal)
+constexpr int kDiagTile = 256;     // granule of the expanded bias (one value per diagonal)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -70,10 +70,14 @@ struct AttnArgs {
   // backward
   const void *dout = nullptr, *fout = nullptr;
   int64_t dos[3] = {0, 0, 0}, os[3] = {0, 0, 0};
-  float* delta = nullptr;        // [B, Hq, Lq] rowsum(dout * out)
+  float* delta = nullptr;        // [B, Hq, row_ld] sum_j P dP of every query
+  float* lse2 = nullptr;         // [B, Hq, row_ld] log2 sums, +inf for a row without a key (attn_tc_bwd.cu)
+  int64_t row_ld = 0;
   void *dq = nullptr, *dk = nullptr, *dv = nullptr;  // contiguous [B, L, H, D]
-  float* dws = nullptr;          // diagonal sums of dS: [B][Hq][query tiles][dws_ld]
+  float* dws = nullptr;          // diagonal sums of dS: [B][Hq][tiles][dws_ld], see attn_api.cu
   int64_t dws_ld = 0;
+  int far = 0, far_both = 0;     // first distance of the last bucket; both directions have one
+  int* err = nullptr;            // the context's error word, set by a bounded wait that gave up
 };
 
 __device__ __forceinline__ int kv_len(const AttnArgs& a, int b) {
@@ -129,13 +133,20 @@ void attn_mma_forward(const AttnArgs& a, cudaStream_t st);
 void attn_mma_backward(const AttnArgs& a, cudaStream_t st);
 int attn_mma_splits(const AttnArgs& a, int sms);
 
+// kernels of attn_tc.cu (16-bit types, rows aligned to 16 bytes, many queries)
+bool attn_tc_fits(const AttnArgs& a);
+void attn_tc_forward(const AttnArgs& a, cudaStream_t st);
+bool attn_tc_bwd_fits(const AttnArgs& a);
+void attn_tc_backward(const AttnArgs& a, cudaStream_t st);
+
 void relbias_forward(int type, int H, int64_t Lq, int64_t Lk, int64_t q_off, const void* table, const BucketRule& rule,
                      void* out, cudaStream_t st);
 int64_t relbias_backward_workspace(int B, int H, int64_t Lq, int64_t Lk, int sms);
 void relbias_backward(int type, int B, int H, int64_t Lq, int64_t Lk, const int64_t* strides, int64_t q_off,
                       const void* dbias, const BucketRule& rule, void* dtable, void* ws, int sms, cudaStream_t st);
-// diagonal sums [H][Lq + Lk - 1] (fp64) -> dtable [n][H] in `type`
+// diagonal sums [H][Lq + Lk - 1] (fp64) -> dtable [n][H] in `type`; far [H][2]
+// (or nullptr): sums that lie whole in the last bucket behind / ahead
 void relbias_bucket_sums(int type, int H, int64_t Lq, int64_t Lk, int64_t q_off, const double* sums,
-                         const BucketRule& rule, void* dtable, cudaStream_t st);
+                         const double* far, const BucketRule& rule, void* dtable, cudaStream_t st);
 
 }  // namespace rvc

@@ -72,9 +72,15 @@ __device__ __forceinline__ void mma8x3(float (&c)[4], const Split4& a, float b0,
   uint32_t h0, l0, h1, l1;
   split_tf32(b0, h0, l0);
   split_tf32(b1, h1, l1);
-  mma8(c, a.lo, h0, h1);
-  mma8(c, a.hi, l0, l1);
-  mma8(c, a.hi, h0, h1);
+  // The tensor cores cut their sums off instead of rounding them: a chain of
+  // products in one accumulator drifts (6e-6 over 1500 keys).  Each product of
+  // eight values is formed alone and added in fp32 with rounding.
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+  mma8(t, a.lo, h0, h1);
+  mma8(t, a.hi, l0, l1);
+  mma8(t, a.hi, h0, h1);
+#pragma unroll
+  for (int x = 0; x < 4; ++x) c[x] += t[x];
 }
 __device__ __forceinline__ float lds_f(uint32_t addr) {
   float v;
@@ -431,17 +437,19 @@ __global__ void attn_join_kernel(const __grid_constant__ AttnArgs a, long long r
 }
 
 // --------------------------------------------------------------- backward
-// delta_i = dout_i . out_i, one warp per row.
-template <typename T>
+// delta_i = sum_j P dP.  For fp32 it is dout_i . out_i, one warp per row; a
+// 16-bit out is too coarse for it (where the softmax is narrow, or a wide bucket
+// of the bias is summed, dP - delta cancels), so there the dQ kernel runs once
+// more before, for delta alone.
 __global__ void attn_delta_kernel(const __grid_constant__ AttnArgs a, long long rows) {
   const long long row = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= rows) return;
   const long long i = row % a.Lq, bh = row / a.Lq, b = bh / a.Hq, h = bh % a.Hq;
-  const T* x = static_cast<const T*>(a.dout) + b * a.dos[0] + i * a.dos[1] + h * a.dos[2];
-  const T* y = static_cast<const T*>(a.fout) + b * a.os[0] + i * a.os[1] + h * a.os[2];
+  const float* x = static_cast<const float*>(a.dout) + b * a.dos[0] + i * a.dos[1] + h * a.dos[2];
+  const float* y = static_cast<const float*>(a.fout) + b * a.os[0] + i * a.os[1] + h * a.os[2];
   float s = 0.f;
-  for (int d = lane; d < a.D; d += 32) s = fmaf(to_f(x[d]), to_f(y[d]), s);
+  for (int d = lane; d < a.D; d += 32) s = fmaf(x[d], y[d], s);
 #pragma unroll
   for (int z = 16; z; z >>= 1) s += __shfl_xor_sync(0xffffffffu, s, z);
   if (lane == 0) a.delta[row] = s;
@@ -451,7 +459,7 @@ __global__ void attn_delta_kernel(const __grid_constant__ AttnArgs a, long long 
 // the diagonals of every tile when the table's gradient is wanted: thread u
 // adds the entries (y, x) with x - y = u - 63, in the order of the rows; the
 // upper half of a tile's diagonals goes on in the next tile.
-template <typename T, int DP, int BN>
+template <typename T, int DP, int BN, bool DELTA>
 __global__ void __launch_bounds__(kT) attn_mma_dq_kernel(const __grid_constant__ AttnArgs a, int vec_q, int vec_kv,
                                                          int vec_do) {
   extern __shared__ __align__(16) uint8_t smem[];
@@ -500,7 +508,7 @@ __global__ void __launch_bounds__(kT) attn_mma_dq_kernel(const __grid_constant__
     const float z = a.lse[row];
     const bool live = z != -INFINITY && i0 + warp * 16 + g + 8 * y < a.Lq;
     lse2[y] = live ? z * kLog2e : INFINITY;  // a row that is not there or has no key: P = 0
-    delta[y] = a.delta[row];
+    delta[y] = DELTA ? 0.f : a.delta[row];
     bias[y] = a.diag ? a.diag + h * a.diag_ld + a.diag0 - qi[y] : nullptr;
   }
   const float sc = a.scale * kLog2e;
@@ -509,7 +517,7 @@ __global__ void __launch_bounds__(kT) attn_mma_dq_kernel(const __grid_constant__
   for (int d = 0; d < DP / 8; ++d)
 #pragma unroll
     for (int x = 0; x < 4; ++x) acc[d][x] = 0.f;
-  float* dws = a.dws ? a.dws + (long long)blockIdx.x * a.dws_ld : nullptr;
+  float* dws = a.dws && !DELTA ? a.dws + (long long)blockIdx.x * a.dws_ld : nullptr;
   if (dws && tid < kBM) carry[tid] = 0.f;
   for (int tile = 0; tile < tiles; ++tile) {
     const int st = tile & 1;
@@ -537,10 +545,11 @@ __global__ void __launch_bounds__(kT) attn_mma_dq_kernel(const __grid_constant__
         if (a.diag && j < a.Lk) v += __ldg(bias[y] + j);
         const bool on = j < len && (!mb || mb[(int64_t)j * a.mask_k]) && (!a.causal || j <= qi[y] + a.q_off);
         const float p = on ? exp2_approx(v - lse2[y]) : 0.f;
-        s[n][x] = p != 0.f ? p * (dp[n][x] - delta[y]) : 0.f;
+        s[n][x] = p != 0.f ? p * (dp[n][x] - (DELTA ? 0.f : delta[y])) : 0.f;
+        if (DELTA) delta[y] += s[n][x];
         if (dws) sD[(warp * 16 + g + 8 * y) * SL + n * 8 + 2 * t + (x & 1)] = s[n][x];
       }
-    mma_pb<T, DP, NT>(acc, s, sK + st * BN * P, lane);
+    if (!DELTA) mma_pb<T, DP, NT>(acc, s, sK + st * BN * P, lane);
     __syncthreads();
     if (dws) {  // diagonals u = x - y + 63 of this tile, 0 <= u < 63 + BN
       const int u = tid;
@@ -554,6 +563,16 @@ __global__ void __launch_bounds__(kT) attn_mma_dq_kernel(const __grid_constant__
       if (u >= BN && u < kBM - 1 + BN) carry[u - BN] = v;
       __syncthreads();
     }
+  }
+  if (DELTA) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      delta[y] += __shfl_xor_sync(0xffffffffu, delta[y], 1);
+      delta[y] += __shfl_xor_sync(0xffffffffu, delta[y], 2);
+      const long long i = i0 + warp * 16 + g + 8 * y;
+      if (t == 0 && i < a.Lq) a.delta[((long long)b * a.Hq + h) * a.Lq + i] = delta[y];
+    }
+    return;
   }
   if (dws) {  // the last diagonals, and zeros where no tile was
     const long long at = (long long)tiles * BN;
@@ -735,12 +754,18 @@ void bwd_dp(const AttnArgs& a, cudaStream_t st) {
   constexpr int BN = sizeof(T) == 4 && DP > 64 ? 32 : 64;  // fp32 rows of 96 / 128: half the tile, to fit shared memory
   const long long n = (long long)a.B * a.Hq * a.Lq;
   if (n > 0) {
-    attn_delta_kernel<T><<<(unsigned)((n + 7) / 8), 256, 0, st>>>(a, n);
+    const size_t smem = (size_t)(2 * kBM + 4 * BN) * P + (a.dws ? (size_t)(kBM * (BN + 1) + kBM) * 4 : 0);
+    if constexpr (sizeof(T) == 4) {
+      attn_delta_kernel<<<(unsigned)((n + 7) / 8), 256, 0, st>>>(a, n);
+    } else {
+      allow_smem((const void*)attn_mma_dq_kernel<T, DP, BN, true>, smem);
+      attn_mma_dq_kernel<T, DP, BN, true>
+          <<<(unsigned)((a.Lq + kBM - 1ll) / kBM * a.B * a.Hq), kT, smem, st>>>(a, vq, vkv, vdo);
+    }
     note_launch();
     RVC_CUDA_TRY(cudaGetLastError());
-    const size_t smem = (size_t)(2 * kBM + 4 * BN) * P + (a.dws ? (size_t)(kBM * (BN + 1) + kBM) * 4 : 0);
-    allow_smem((const void*)attn_mma_dq_kernel<T, DP, BN>, smem);
-    attn_mma_dq_kernel<T, DP, BN>
+    allow_smem((const void*)attn_mma_dq_kernel<T, DP, BN, false>, smem);
+    attn_mma_dq_kernel<T, DP, BN, false>
         <<<(unsigned)((a.Lq + kBM - 1ll) / kBM * a.B * a.Hq), kT, smem, st>>>(a, vq, vkv, vdo);
     note_launch();
     RVC_CUDA_TRY(cudaGetLastError());

@@ -1,0 +1,423 @@
+// Attention on the fifth-generation tensor cores (16-bit inputs, many queries).
+//
+// One block takes 256 queries of one head, as two tiles of 128, and walks over
+// the keys in tiles of 128:
+//   warp 8    loads Q once and K, V (and the bias of the tile's diagonals) per
+//             key tile by TMA into 128-byte swizzled slabs, two stages each;
+//   warp 9    issues S = Q K^T (fp32 in tensor memory) and O += P V with P read
+//             from tensor memory, in the order S0 S1 | O0 S0' | O1 S1' ..., so
+//             that one tile's products run while the other's softmax does;
+//   warps 0-3 and 4-7: the softmax of one query tile each, one row to a thread,
+//             so that row maxima and sums need no exchange.  P = 2^(s - m) is
+//             written back as 16-bit pairs over the columns of S.
+// The output stays in tensor memory over all key tiles.  It is rescaled only
+// when a row's maximum has grown by more than 2^8 over the one in use (P then
+// stays below 256, far inside either 16-bit type, and the sums are fp32).
+// P is rounded to the inputs' type: the same relative step as the output's own.
+//
+// A tile's dead keys get s = -inf; their rows of V are zeroed in shared memory
+// first, so that nothing a padded buffer holds reaches a product.
+//
+// Every wait is bounded; one that gives up sets the context's error word and
+// lets the block wind down.
+#include "attn_tc.cuh"
+#include "context.cuh"
+
+#include <algorithm>
+#include <atomic>
+#include <mutex>
+
+namespace rvc {
+
+namespace atc {
+
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  if (!fn) throw Error{kErrCuda, "cuTensorMapEncodeTiled is not available from the driver"};
+  return fn;
+}
+
+// TMA wants 16-byte aligned starts and strides; a stride of a dimension that
+// has one entry is never used, any other must be positive and below 2^40 bytes.
+bool map_ok(const AttnArgs& a, const void* p, const int64_t* s, int L, int H) {
+  const int64_t n[3] = {a.B, L, H};
+  if (reinterpret_cast<uintptr_t>(p) % 16 || a.D * 2 % 16) return false;
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (s[i] <= 0 || s[i] * 2 % 16 || s[i] * 2 >= (1ll << 40))) return false;
+  return true;
+}
+
+void make_map(CUtensorMap* m, int type, const void* p, const int64_t* s, int B, int L, int H, int D, int rows) {
+  const cuuint64_t row = (cuuint64_t)(D * 2 + 15) / 16 * 16;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)L, (cuuint64_t)B};
+  cuuint64_t strides[3] = {H > 1 ? (cuuint64_t)s[2] * 2 : row, L > 1 ? (cuuint64_t)s[1] * 2 : row,
+                           B > 1 ? (cuuint64_t)s[0] * 2 : row};
+  cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
+  cuuint32_t es[4] = {1, 1, 1, 1};
+  CUresult r = encode_fn()(m, type == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                           const_cast<void*>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw Error{kErrCuda, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")"};
+}
+
+}  // namespace atc
+
+namespace {
+
+using namespace atc;
+
+constexpr int kFwdThreads = 320;
+constexpr float kGrow = 8.f;  // log2 of the growth of a maximum that is taken without rescaling
+
+struct FwdMaps {
+  CUtensorMap q, k, v;
+};
+
+// shared memory: Q [2 tiles][NS], K [2 stages][NS], V [2][NS] slabs, bias [2][384], barriers
+template <int NS> constexpr uint32_t fwd_smem() { return 6 * NS * kSlab + 2 * 384 * 4 + 256 + 1024; }
+
+template <typename T, int NS>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+    attn_tc_fwd_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ FwdMaps maps) {
+  extern __shared__ uint8_t raw[];
+  const uint32_t base = (ptx::smem_u32(raw) + 1023) & ~1023u;
+  uint8_t* gen = raw + (base - ptx::smem_u32(raw));
+  const uint32_t sQ = base, sK = sQ + 2 * NS * kSlab, sV = sK + 2 * NS * kSlab;
+  const uint32_t oB = 6 * NS * kSlab, oBar = oB + 2 * 384 * 4;
+  const float* bias_s = reinterpret_cast<const float*>(gen + oB);
+  const uint32_t bar = base + oBar;
+  const uint32_t Q_FULL = bar, K_FULL = bar + 8, V_FULL = bar + 24, K_EMPTY = bar + 40, V_EMPTY = bar + 56,
+                 S_FULL = bar + 72, P_FULL = bar + 88, O_DONE = bar + 104, DRAIN = bar + 120;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(gen + oBar + 128);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const int npair = (a.Lq + 255) / 256;
+  const int pair = a.causal ? npair - 1 - (int)(blockIdx.x % npair) : (int)(blockIdx.x % npair);
+  const int bh = blockIdx.x / npair, b = bh / a.Hq, h = bh % a.Hq, kh = h / (a.Hq / a.Hkv);
+  const int q0 = pair * 256;
+  const int len = kv_len(a, b);
+  long long kend = len;
+  if (a.causal) kend = max(0ll, min(kend, (long long)min(a.Lq, q0 + 256) + a.q_off));
+  const int tiles = (int)((kend + 127) / 128);
+
+  if (threadIdx.x == 0) {
+    ptx::mbar_init(Q_FULL, 1);
+    for (int s = 0; s < 2; ++s) {
+      ptx::mbar_init(K_FULL + 8 * s, 1);
+      ptx::mbar_init(V_FULL + 8 * s, 1);
+      ptx::mbar_init(K_EMPTY + 8 * s, a.diag ? 9 : 1);  // the softmax warps read the bias of the stage
+      ptx::mbar_init(V_EMPTY + 8 * s, 1);
+      ptx::mbar_init(S_FULL + 8 * s, 1);
+      ptx::mbar_init(P_FULL + 8 * s, 4);
+      ptx::mbar_init(O_DONE + 8 * s, 1);
+    }
+    ptx::mbar_init(DRAIN, 1);
+    ptx::fence_mbar_init();
+  }
+  if (warp == 9) {
+    ptx::tmem_alloc(ptx::smem_u32(slot), 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *slot;
+  const uint32_t tS = tmem, tO = tmem + 256;  // S0 S1 (128 columns each), O0 O1 (64 NS each)
+
+  if (warp == 8) {
+    if (lane == 0 && tiles > 0) {
+      ptx::mbar_expect_tx(Q_FULL, 2 * NS * kSlab);
+      for (int w = 0; w < 2; ++w)
+        for (int s = 0; s < NS; ++s)
+          ptx::tma_load_4d(sQ + (w * NS + s) * kSlab, &maps.q, 64 * s, h, q0 + 128 * w, b, Q_FULL);
+      bool ok = true;
+      int nk = 0, nv = 0;  // tiles asked for
+      for (int t = 0; t < tiles && ok; ++t) {
+        const int st = t & 1;
+        const uint32_t ph = ((t >> 1) & 1) ^ 1;
+        if (!ptx::mbar_wait(K_EMPTY + 8 * st, ph, kWaitNs)) {
+          ok = false;
+          break;
+        }
+        ptx::mbar_expect_tx(K_FULL + 8 * st, NS * kSlab + (a.diag ? 384 * 4 : 0));
+        for (int s = 0; s < NS; ++s)
+          ptx::tma_load_4d(sK + (st * NS + s) * kSlab, &maps.k, 64 * s, kh, t * 128, b, K_FULL + 8 * st);
+        nk = t + 1;
+        if (a.diag)
+          ptx::bulk_g2s(base + oB + st * 384 * 4, a.diag + h * a.diag_ld + (t * 128 - q0 - 256 + a.diag0), 384 * 4,
+                        K_FULL + 8 * st);
+        if (!ptx::mbar_wait(V_EMPTY + 8 * st, ph, kWaitNs)) {
+          ok = false;
+          break;
+        }
+        ptx::mbar_expect_tx(V_FULL + 8 * st, NS * kSlab);
+        for (int s = 0; s < NS; ++s)
+          ptx::tma_load_4d(sV + (st * NS + s) * kSlab, &maps.v, 64 * s, kh, t * 128, b, V_FULL + 8 * st);
+        nv = t + 1;
+      }
+      if (!ok) atomicExch(a.err, 41);
+      // no copy left in flight when the block ends
+      ptx::mbar_wait(Q_FULL, 0, kWaitNs);
+      for (int x = max(0, nk - 2); x < nk; ++x) ptx::mbar_wait(K_FULL + 8 * (x & 1), (x >> 1) & 1, kWaitNs);
+      for (int x = max(0, nv - 2); x < nv; ++x) ptx::mbar_wait(V_FULL + 8 * (x & 1), (x >> 1) & 1, kWaitNs);
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (lane == 0 && tiles > 0) {
+      const uint32_t id_s = idesc<T>(128, false, false);
+      const int DK = (a.D + 15) / 16;
+      const uint32_t id_o = idesc<T>(16 * DK, false, true);
+      bool ok = ptx::mbar_wait(Q_FULL, 0, kWaitNs);
+      auto issue_s = [&](int w, int t) {
+        const int st = t & 1;
+        if (ok) ok = ptx::mbar_wait(K_FULL + 8 * st, (t >> 1) & 1, kWaitNs);
+        if (!ok) return;
+        ptx::tc_fence_after();
+        const uint64_t dq = desc_k(sQ + w * NS * kSlab), dk = desc_k(sK + st * NS * kSlab);
+#pragma unroll
+        for (int kk = 0; kk < 4 * NS; ++kk) {
+          if (kk >= DK) break;
+          const uint64_t off = (uint64_t)(((kk >> 2) * kSlab + (kk & 3) * 32) >> 4);
+          mma_ss(tS + 128 * w, dq + off, dk + off, id_s, kk > 0);
+        }
+        ptx::mma_commit(S_FULL + 8 * w);
+        if (w == 1) ptx::mma_commit(K_EMPTY + 8 * st);
+      };
+      auto issue_o = [&](int w, int t) {
+        const int st = t & 1;
+        if (ok) ok = ptx::mbar_wait(V_FULL + 8 * st, (t >> 1) & 1, kWaitNs);
+        if (ok) ok = ptx::mbar_wait(P_FULL + 8 * w, t & 1, kWaitNs);
+        if (!ok) return;
+        ptx::tc_fence_after();
+        const uint64_t dv = desc_mn(sV + st * NS * kSlab);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          mma_ts(tO + 64 * NS * w, tS + 128 * w + 8 * kk, dv + (uint64_t)(kk * 2048 >> 4), id_o, t > 0 || kk > 0);
+        ptx::mma_commit(O_DONE + 8 * w);
+        if (w == 1) ptx::mma_commit(V_EMPTY + 8 * st);
+      };
+      issue_s(0, 0);
+      issue_s(1, 0);
+      for (int t = 0; t < tiles && ok; ++t) {
+        issue_o(0, t);
+        if (t + 1 < tiles) issue_s(0, t + 1);
+        issue_o(1, t);
+        if (t + 1 < tiles) issue_s(1, t + 1);
+      }
+      if (!ok) atomicExch(a.err, 42);
+      ptx::mma_commit(DRAIN);
+      ptx::mbar_wait(DRAIN, 0, kWaitNs);  // every product done before tensor memory is freed
+    }
+    __syncwarp();
+  } else {
+    const int w = warp >> 2;  // query tile
+    const int row = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_col = tS + 128 * w + lanes, o_col = tO + 64 * NS * w + lanes;
+    const long long i = (long long)q0 + 128 * w + row;
+    const float sc = a.scale * kLog2e;
+    // keys that this row may meet: [0, lim)
+    const long long lim = a.causal ? min((long long)len, i + a.q_off + 1) : (long long)len;
+    // the smallest limit of the warp: tiles below it need no comparison
+    const long long wlim =
+        a.causal ? min((long long)len, (long long)q0 + 128 * w + (warp & 3) * 32 + a.q_off + 1) : (long long)len;
+    const uint8_t* mb = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int t = 0; t < tiles && ok; ++t) {
+      const int st = t & 1, j0 = t * 128;
+      uint32_t alive[4] = {~0u, ~0u, ~0u, ~0u};
+      if (mb) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int j = j0 + 32 * x + lane;
+          alive[x] = __ballot_sync(0xffffffffu, j < len && mb[(int64_t)j * a.mask_k] != 0);
+        }
+      }
+      if (mb || j0 + 128 > len) {  // zero the dead rows of V (both query tiles do, with the same result)
+        const bool dead = j0 + row >= len || !((alive[row >> 5] >> (row & 31)) & 1);
+        if (!warp_wait(V_FULL + 8 * st, (t >> 1) & 1)) {
+          ok = false;
+          break;
+        }
+        if (dead) {
+          uint4* z = reinterpret_cast<uint4*>(gen + 4 * NS * kSlab + st * NS * kSlab + row * 128);
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int x = 0; x < 8; ++x) z[s * (kSlab / 16) + x] = make_uint4(0, 0, 0, 0);
+        }
+        ptx::fence_proxy_async_smem();
+      }
+      if (a.diag && !warp_wait(K_FULL + 8 * st, (t >> 1) & 1)) {
+        ok = false;
+        break;
+      }
+      if (!warp_wait(S_FULL + 8 * w, t & 1)) {
+        ok = false;
+        break;
+      }
+      ptx::tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) ptx::tmem_ld32_async(s_col + 32 * x, s[x]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) ptx::tmem_wait_ld(s[x]);
+      float mx = -INFINITY;
+      if (a.diag) {
+        const float* bb = bias_s + st * 384 + 256 - 128 * w - row;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int c = 0; c < 32; ++c) s[x][c] = __float_as_uint(fmaf(__uint_as_float(s[x][c]), sc, bb[32 * x + c]));
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(K_EMPTY + 8 * st);
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int c = 0; c < 32; ++c) s[x][c] = __float_as_uint(__uint_as_float(s[x][c]) * sc);
+      }
+      if (mb || j0 + 128 > wlim) {
+        const int n = (int)max(0ll, min(128ll, lim - j0));
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (32 * x + c >= n || !((alive[x] >> c) & 1)) s[x][c] = 0xff800000u;
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) mx = fmaxf(fmaxf(mx, __uint_as_float(s[x][c])), __uint_as_float(s[x][c + 1]));
+      const bool up = mx > m + kGrow;  // always on a row's first live key
+      if (__any_sync(0xffffffffu, up)) {
+        const float m_new = up ? mx : m;
+        const float f = m == -INFINITY ? 0.f : exp2_approx(m - m_new);
+        if (t > 0) {
+          if (!warp_wait(O_DONE + 8 * w, (t - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
+#pragma unroll 1
+          for (int x = 0; x < 64 * NS; x += 16) {
+            float o[16];
+            ptx::tmem_ld16(o_col + x, o);
+            uint32_t r[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) r[c] = __float_as_uint(o[c] * (up ? f : 1.f));
+            tmem_st16(o_col + x, r);
+          }
+        }
+        if (up) l *= f;
+        m = m_new;
+      }
+      const float mb2 = m == -INFINITY ? 0.f : m;
+      float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint32_t p[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float e0 = exp2_approx(__uint_as_float(s[2 * x + (c >> 4)][(2 * c) & 31]) - mb2);
+          const float e1 = exp2_approx(__uint_as_float(s[2 * x + (c >> 4)][(2 * c + 1) & 31]) - mb2);
+          l0 += e0;
+          l1 += e1;
+          p[c] = pack2<T>(e0, e1);
+        }
+        tmem_st32(s_col + 32 * x, p);
+      }
+      l += l0 + l1;
+      tmem_wait_st();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(P_FULL + 8 * w);
+    }
+    if (ok && tiles > 0) {
+      ok = warp_wait(O_DONE + 8 * w, (tiles - 1) & 1);
+      ptx::tc_fence_after();
+    }
+    if (!ok) {
+      if (lane == 0) atomicExch(a.err, 43);
+    } else {
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      T* dst = static_cast<T*>(a.out) + (((long long)b * a.Lq + i) * a.Hq + h) * a.D;
+#pragma unroll 1
+      for (int x = 0; x < 64 * NS; x += 16) {
+        if (x >= a.D) break;
+        float o[16];
+        if (tiles > 0) {
+          ptx::tmem_ld16(o_col + x, o);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) o[c] = 0.f;
+        }
+        if (i < a.Lq) {
+#pragma unroll
+          for (int c = 0; c < 16; c += 8)
+            if (x + c < a.D)  // D is a multiple of 8
+              *reinterpret_cast<uint4*>(dst + x + c) =
+                  make_uint4(pack2<T>(o[c] * inv, o[c + 1] * inv), pack2<T>(o[c + 2] * inv, o[c + 3] * inv),
+                             pack2<T>(o[c + 4] * inv, o[c + 5] * inv), pack2<T>(o[c + 6] * inv, o[c + 7] * inv));
+        }
+      }
+      if (i < a.Lq) a.lse[((long long)b * a.Hq + h) * a.Lq + i] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  if (warp == 9) ptx::tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int NS>
+void fwd(const AttnArgs& a, cudaStream_t st) {
+  FwdMaps maps;
+  make_map(&maps.q, a.type, a.q, a.qs, a.B, a.Lq, a.Hq, a.D, 128);
+  make_map(&maps.k, a.type, a.k, a.ks, a.B, a.Lk, a.Hkv, a.D, 128);
+  make_map(&maps.v, a.type, a.v, a.vs, a.B, a.Lk, a.Hkv, a.D, 128);
+  static std::atomic<uint64_t> done{0};  // one bit per device
+  int dev = 0;
+  RVC_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !(done.load() & (1ull << dev))) {
+    RVC_CUDA_TRY(cudaFuncSetAttribute(attn_tc_fwd_kernel<T, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)fwd_smem<NS>()));
+    if (dev < 64) done.fetch_or(1ull << dev);
+  }
+  const unsigned grid = (unsigned)((a.Lq + 255ll) / 256 * a.B * a.Hq);
+  attn_tc_fwd_kernel<T, NS><<<grid, kFwdThreads, fwd_smem<NS>(), st>>>(a, maps);
+  note_launch();
+  RVC_CUDA_TRY(cudaGetLastError());
+}
+
+}  // namespace
+
+// 16-bit operands that TMA can address, and enough queries to fill a tile of
+// 128 rows more than half.
+bool attn_tc_fits(const AttnArgs& a) {
+  return a.type != kF32 && a.Lq >= 64 && a.Lk >= 1 && atc::map_ok(a, a.q, a.qs, a.Lq, a.Hq) &&
+         atc::map_ok(a, a.k, a.ks, a.Lk, a.Hkv) && atc::map_ok(a, a.v, a.vs, a.Lk, a.Hkv) &&
+         reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+}
+
+void attn_tc_forward(const AttnArgs& a, cudaStream_t st) {
+  if (a.type == kBf16) {
+    if (a.D <= 64) fwd<__nv_bfloat16, 1>(a, st);
+    else fwd<__nv_bfloat16, 2>(a, st);
+  } else {
+    if (a.D <= 64) fwd<__half, 1>(a, st);
+    else fwd<__half, 2>(a, st);
+  }
+}
+
+}  // namespace rvc

@@ -115,7 +115,7 @@ void relbias_backward(int type, int B, int H, int64_t Lq, int64_t Lk, const int6
   relbias_join_kernel<<<dim3((unsigned)((n + 255) / 256), H), 256, 0, st>>>(part, chunks, B, H, n, sums);
   note_launch();
   RVC_CUDA_TRY(cudaGetLastError());
-  relbias_bucket_sums(type, H, Lq, Lk, q_off, sums, rule, dtable, st);
+  relbias_bucket_sums(type, H, Lq, Lk, q_off, sums, nullptr, rule, dtable, st);
 }
 
 }  // namespace rvc
