@@ -110,8 +110,9 @@ Layout plan(const AttnArgs& a, bool bias, bool backward, int sms, bool tc) {
     l.diag = take(4 * l.diag_ld * a.Hq);
   }
   if (!backward) {
-    l.nsplit = tc ? 1 : attn_mma_splits(a, sms);
-    if (l.nsplit > 1) {
+    bool parts = false;
+    if (!tc) l.nsplit = attn_mma_splits(a, sms, &parts);
+    if (parts) {
       l.po = take(4 * rows * a.D * l.nsplit);
       l.pml = take(8 * rows * l.nsplit);
     }

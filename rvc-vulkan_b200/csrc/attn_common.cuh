@@ -131,7 +131,7 @@ void attn_expand_bias(const AttnArgs& a, const void* table, const BucketRule& ru
 // kernels of attn_mma.cu (every type, stride and size)
 void attn_mma_forward(const AttnArgs& a, cudaStream_t st);
 void attn_mma_backward(const AttnArgs& a, cudaStream_t st);
-int attn_mma_splits(const AttnArgs& a, int sms);
+int attn_mma_splits(const AttnArgs& a, int sms, bool* workspace);
 
 // kernels of attn_tc.cu (16-bit types, rows aligned to 16 bytes, many queries)
 bool attn_tc_fits(const AttnArgs& a);

@@ -135,6 +135,30 @@ __device__ __forceinline__ void mma_abt(float (&c)[NT][4], uint32_t a, uint32_t 
   }
 }
 
+// The A operand of mma_abt held in registers over many calls (16-bit types).
+template <typename T, int DP>
+struct FragA {
+  uint32_t f[DP / 16][4];
+  __device__ __forceinline__ void load(uint32_t a, int lane) {
+    const int mi = lane >> 3, r8 = lane & 7;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+      ldsm4(f[kk], a + ((mi & 1) * 8 + r8) * pitch<T, DP>() + (kk * 16 + (mi >> 1) * 8) * 2);
+  }
+  // C[16][16] += A . B[16][DP]^T
+  __device__ __forceinline__ void abt(float (&c)[2][4], uint32_t b, int lane) const {
+    const int mi = lane >> 3, r8 = lane & 7;
+    const uint32_t at = b + ((mi >> 1) * 8 + r8) * pitch<T, DP>() + (mi & 1) * 16;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      uint32_t bf[4];
+      ldsm4(bf, at + kk * 32);
+      mma16(c[0], f[kk], bf[0], bf[1], T());
+      mma16(c[1], f[kk], bf[2], bf[3], T());
+    }
+  }
+};
+
 // C[16][DP] += A[16][8 NT] . B[8 NT][DP]: A are accumulator fragments (weights),
 // B staged rows.  fp32: the contraction runs over the columns in the order
 // 2t, 2t + 1, which is the accumulators' own, so no value changes lanes.
@@ -198,32 +222,29 @@ __device__ __forceinline__ void stage_rows(uint32_t dst, int rows, int D, bool v
   }
 }
 
-// ---------------------------------------------------------------- forward
-// One block: one KV head of one batch entry, ROWS rows of the (query head in
-// the group, query) plane, and the key tiles of one split.  ROWS = 64: every
-// warp has 16 rows of its own and all 64 keys of a tile.  ROWS = 16 (few
-// rows): the warps share the rows and take 16 keys of each tile each; their
-// running (max, sum, row) are joined at the end through shared memory.
-template <typename T, int DP, int ROWS>
+// ------------------------------------------------- forward, many query rows
+// One block: one KV head of one batch entry, 64 rows of the (query head in the
+// group, query) plane - every warp has 16 of its own - and the key tiles of one
+// split.
+template <typename T, int DP>
 __global__ void __launch_bounds__(kT) attn_mma_fwd_kernel(const __grid_constant__ AttnArgs a, int vec_q, int vec_kv) {
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr int P = pitch<T, DP>();
-  constexpr bool SHARED = ROWS == 16;
-  constexpr int NT = SHARED ? 2 : 8;  // key groups of 8 per warp
+  constexpr int NT = kBN / 8;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int G = a.Hq / a.Hkv;
   const long long rows = (long long)G * a.Lq;
-  const unsigned ntile = (unsigned)((rows + ROWS - 1) / ROWS);
+  const unsigned ntile = (unsigned)((rows + kBM - 1) / kBM);
   const int b = blockIdx.x / ntile / a.Hkv, kh = blockIdx.x / ntile % a.Hkv;
-  const long long r0 = (long long)(blockIdx.x % ntile) * ROWS;
+  const long long r0 = (long long)(blockIdx.x % ntile) * kBM;
   const uint32_t sm = ptx::smem_u32(smem);
-  const uint32_t sQ = sm, sK = sQ + ROWS * P, sV = sK + 2 * kBN * P;
+  const uint32_t sQ = sm, sK = sQ + kBM * P, sV = sK + 2 * kBN * P;
   const int len = kv_len(a, b);
 
   // the furthest key that a row of this block may meet
   long long kend = len;
   if (a.causal) {
-    const long long last = min(rows, r0 + ROWS) - 1;
+    const long long last = min(rows, r0 + kBM) - 1;
     const long long imax = (r0 / a.Lq != last / a.Lq) ? a.Lq - 1 : last % a.Lq;
     kend = max(0ll, min(kend, imax + a.q_off + 1));
   }
@@ -234,7 +255,7 @@ __global__ void __launch_bounds__(kT) attn_mma_fwd_kernel(const __grid_constant_
   const T* kb = static_cast<const T*>(a.k) + (int64_t)b * a.ks[0] + (int64_t)kh * a.ks[2];
   const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.vs[0] + (int64_t)kh * a.vs[2];
   const uint8_t* mb = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
-  stage_rows<T, DP>(sQ, ROWS, a.D, vec_q, tid, [&](int r) -> const T* {
+  stage_rows<T, DP>(sQ, kBM, a.D, vec_q, tid, [&](int r) -> const T* {
     const long long x = r0 + r;
     return x < rows ? qb + (x % a.Lq) * a.qs[1] + (kh * G + x / a.Lq) * a.qs[2] : nullptr;
   });
@@ -250,7 +271,7 @@ __global__ void __launch_bounds__(kT) attn_mma_fwd_kernel(const __grid_constant_
   if (t0 < t1) load(t0, 0);
 
   // the two rows of this thread
-  const int wr = SHARED ? 0 : warp * 16;
+  const int wr = warp * 16;
   long long qi[2];
   const float* bias[2];
 #pragma unroll
@@ -275,15 +296,14 @@ __global__ void __launch_bounds__(kT) attn_mma_fwd_kernel(const __grid_constant_
       cp_wait<0>();
     }
     __syncthreads();
-    const int key0 = SHARED ? warp * 16 : 0;
     float s[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int x = 0; x < 4; ++x) s[n][x] = 0.f;
-    mma_abt<T, DP, NT>(s, sQ + wr * P, sK + (st * kBN + key0) * P, lane);
-    const int j0 = tile * kBN + key0;
-    const bool whole = !mb && j0 + NT * 8 <= len && (!a.causal || j0 + NT * 8 <= min(qi[0], qi[1]) + a.q_off + 1);
+    mma_abt<T, DP, NT>(s, sQ + wr * P, sK + st * kBN * P, lane);
+    const int j0 = tile * kBN;
+    const bool whole = !mb && j0 + kBN <= len && (!a.causal || j0 + kBN <= min(qi[0], qi[1]) + a.q_off + 1);
     float mx[2] = {m[0], m[1]};
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -321,7 +341,7 @@ __global__ void __launch_bounds__(kT) attn_mma_fwd_kernel(const __grid_constant_
       for (int x = 0; x < 4; ++x) o[d][x] *= f[x >> 1];
     m[0] = mx[0];
     m[1] = mx[1];
-    mma_pb<T, DP, NT>(o, s, sV + (st * kBN + key0) * P, lane);
+    mma_pb<T, DP, NT>(o, s, sV + st * kBN * P, lane);
     __syncthreads();
   }
 #pragma unroll
@@ -329,81 +349,308 @@ __global__ void __launch_bounds__(kT) attn_mma_fwd_kernel(const __grid_constant_
     l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
     l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
   }
-  if constexpr (SHARED) {  // join the four warps: rows of warp w at [w][16][DP + 4] floats, (m, l) behind
-    cp_wait<0>();
-    __syncthreads();
-    float* part = reinterpret_cast<float*>(smem);
-    constexpr int LD = DP + 4;
-    float* ml = part + 4 * 16 * LD;
 #pragma unroll
-    for (int d = 0; d < DP / 8; ++d)
+  for (int y = 0; y < 2; ++y) {
+    const long long x = r0 + wr + g + 8 * y;
+    if (x >= rows) continue;
+    const long long i = x % a.Lq, h = kh * G + x / a.Lq;
+    const long long row = ((long long)b * a.Hq + h) * a.Lq + i;
+    if (a.nsplit > 1) {
+      const long long pr = (long long)blockIdx.y * a.B * a.Hq * a.Lq + row;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) part[(warp * 16 + g + 8 * (x >> 1)) * LD + d * 8 + 2 * t + (x & 1)] = o[d][x];
-    if (t == 0)
+      for (int d = 0; d < DP / 8; ++d)
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        ml[2 * (warp * 16 + g + 8 * y)] = m[y];
-        ml[2 * (warp * 16 + g + 8 * y) + 1] = l[y];
+        for (int z = 0; z < 2; ++z)
+          if (d * 8 + 2 * t + z < a.D) a.po[pr * a.D + d * 8 + 2 * t + z] = o[d][2 * y + z];
+      if (t == 0) {
+        a.pml[2 * pr] = m[y];
+        a.pml[2 * pr + 1] = l[y];
       }
-    __syncthreads();
-    for (int e = tid; e < 16 * DP; e += kT) {
-      const int r = e / DP, d = e % DP;
-      const long long x = r0 + r;
-      if (x >= rows || d >= a.D) continue;
-      float M = -INFINITY;
+    } else {
+      const float inv = l[y] > 0.f ? 1.f / l[y] : 0.f;
+      T* dst = static_cast<T*>(a.out) + (((long long)b * a.Lq + i) * a.Hq + h) * a.D;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[2 * (w * 16 + r)]);
-      float L = 0.f, v = 0.f;
+      for (int d = 0; d < DP / 8; ++d)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float f = ml[2 * (w * 16 + r)] == -INFINITY ? 0.f : exp2_approx(ml[2 * (w * 16 + r)] - M);
-        L = fmaf(f, ml[2 * (w * 16 + r) + 1], L);
-        v = fmaf(f, part[(w * 16 + r) * LD + d], v);
-      }
-      const long long i = x % a.Lq, h = kh * G + x / a.Lq;
-      const long long row = ((long long)b * a.Hq + h) * a.Lq + i;
-      if (a.nsplit > 1) {
-        const long long pr = (long long)blockIdx.y * a.B * a.Hq * a.Lq + row;
-        a.po[pr * a.D + d] = v;
-        if (d == 0) {
-          a.pml[2 * pr] = M;
-          a.pml[2 * pr + 1] = L;
-        }
-      } else {
-        static_cast<T*>(a.out)[(((long long)b * a.Lq + i) * a.Hq + h) * a.D + d] = from_f<T>(L > 0.f ? v / L : 0.f);
-        if (d == 0) a.lse[row] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      const long long x = r0 + wr + g + 8 * y;
-      if (x >= rows) continue;
-      const long long i = x % a.Lq, h = kh * G + x / a.Lq;
-      const long long row = ((long long)b * a.Hq + h) * a.Lq + i;
-      if (a.nsplit > 1) {
-        const long long pr = (long long)blockIdx.y * a.B * a.Hq * a.Lq + row;
-#pragma unroll
-        for (int d = 0; d < DP / 8; ++d)
-#pragma unroll
-          for (int z = 0; z < 2; ++z)
-            if (d * 8 + 2 * t + z < a.D) a.po[pr * a.D + d * 8 + 2 * t + z] = o[d][2 * y + z];
-        if (t == 0) {
-          a.pml[2 * pr] = m[y];
-          a.pml[2 * pr + 1] = l[y];
-        }
-      } else {
-        const float inv = l[y] > 0.f ? 1.f / l[y] : 0.f;
-        T* dst = static_cast<T*>(a.out) + (((long long)b * a.Lq + i) * a.Hq + h) * a.D;
-#pragma unroll
-        for (int d = 0; d < DP / 8; ++d)
-#pragma unroll
-          for (int z = 0; z < 2; ++z)
-            if (d * 8 + 2 * t + z < a.D) dst[d * 8 + 2 * t + z] = from_f<T>(o[d][2 * y + z] * inv);
-        if (t == 0) a.lse[row] = l[y] > 0.f ? (m[y] + log2f(l[y])) * kLn2 : -INFINITY;
-      }
+        for (int z = 0; z < 2; ++z)
+          if (d * 8 + 2 * t + z < a.D) dst[d * 8 + 2 * t + z] = from_f<T>(o[d][2 * y + z] * inv);
+      if (t == 0) a.lse[row] = l[y] > 0.f ? (m[y] + log2f(l[y])) * kLn2 : -INFINITY;
     }
   }
+}
+
+// -------------------------------------------------- forward, few query rows
+// At most 16 rows to a KV head (one or a few new tokens): bound by reading the
+// keys and values once.  Every warp streams 16 keys at a time through a ring of
+// its own in shared memory (cp.async, no barrier between warps) with all rows in
+// one fragment; the running maximum is raised, and the output rescaled, only
+// when it grows by more than 2^8.  The warps join through shared memory, and
+// the splits of a row through the shared memory of their cluster (nsplit <=
+// kCluster), so that one launch does it; more splits go through the workspace.
+constexpr int kCluster = 8;
+
+// Three stages of 128 16-bit values leave room for two blocks to an SM.
+template <typename T, int DP> constexpr int few_stages() { return DP * sizeof(T) > 256 ? 2 : DP * sizeof(T) > 192 ? 3 : 4; }
+template <typename T, int DP> constexpr size_t few_smem() {
+  return std::max((size_t)4 * few_stages<T, DP>() * 2 * 16 * pitch<T, DP>() + (size_t)16 * pitch<T, DP>(),
+                  (size_t)(5 * 16 * (DP + 4) + 5 * 32) * 4);
+}
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+  float v;
+  asm volatile(
+      "{\n\t.reg .b32 r;\n\t"
+      "mapa.shared::cluster.u32 r, %1, %2;\n\t"
+      "ld.shared::cluster.f32 %0, [r];\n\t}"
+      : "=f"(v)
+      : "r"(addr), "r"(rank)
+      : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <typename T, int DP, bool CLUSTER>
+__global__ void __launch_bounds__(kT) attn_mma_few_kernel(const __grid_constant__ AttnArgs a, int vec_q, int vec_kv) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int P = pitch<T, DP>(), S = few_stages<T, DP>();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int G = a.Hq / a.Hkv, rows = G * a.Lq;  // <= 16
+  const int b = blockIdx.x / a.Hkv, kh = blockIdx.x % a.Hkv;
+  const uint32_t sm = ptx::smem_u32(smem);
+  const uint32_t sQ = sm, ring = sm + 16 * P + warp * S * 2 * 16 * P;
+  const int len = kv_len(a, b);
+  long long kend = len;
+  if (a.causal) kend = max(0ll, min(kend, (long long)a.Lq + a.q_off));
+  // steps of 16 keys of this split, dealt to the warps in turn
+  const int steps = (int)((kend + 15) / 16);
+  const int s0 = (int)((long long)steps * blockIdx.y / a.nsplit), s1 = (int)((long long)steps * (blockIdx.y + 1) / a.nsplit);
+  const int n = max(0, s1 - s0 - warp + 3) / 4;  // of this warp: s0 + warp + 4 x
+
+  const T* qb = static_cast<const T*>(a.q) + (int64_t)b * a.qs[0];
+  const T* kb = static_cast<const T*>(a.k) + (int64_t)b * a.ks[0] + (int64_t)kh * a.ks[2];
+  const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.vs[0] + (int64_t)kh * a.vs[2];
+  const uint8_t* mb = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
+  constexpr int E = 16 / (int)sizeof(T), CH = DP / E;
+  constexpr bool POW2 = (CH & (CH - 1)) == 0;
+  // a lane's chunk of a row and its rows: lane / CH, then every 32 / CH
+  const int lr = lane / CH, lc = lane % CH;
+  const T* kp = kb + (int64_t)((s0 + warp) * 16 + lr) * a.ks[1] + lc * E;
+  const T* vp = vb + (int64_t)((s0 + warp) * 16 + lr) * a.vs[1] + lc * E;
+  const uint32_t cols = lc * E < a.D ? 16u : 0u;
+  auto load = [&](int x) {  // the warp's x-th step; always one group, so that counts agree
+    if (x < n) {
+      const int j0 = (s0 + warp + 4 * x) * 16;
+      const uint32_t dk = ring + (x % S) * 2 * 16 * P, dv = dk + 16 * P;
+      if (vec_kv && POW2) {
+        const T *k = kp + (int64_t)(64 * x) * a.ks[1], *v = vp + (int64_t)(64 * x) * a.vs[1];
+        const bool whole = !mb && j0 + 16 <= len;
+        const uint32_t at = dk + lr * P + lc * 16;
+#pragma unroll
+        for (int i = 0; i < CH / 2; ++i) {
+          const int r = i * (32 / CH);
+          uint32_t on = cols;
+          if (!whole && !(j0 + lr + r < len && (!mb || mb[(int64_t)(j0 + lr + r) * a.mask_k]))) on = 0;
+          cp16(at + r * P, on ? k : kb, on);
+          cp16(at + 16 * P + r * P, on ? v : vb, on);
+          k += (32 / CH) * a.ks[1];
+          v += (32 / CH) * a.vs[1];
+        }
+      } else if (vec_kv) {
+#pragma unroll
+        for (int e = lane; e < 16 * CH; e += 32) {
+          const int r = e / CH, c = e % CH, j = j0 + r;
+          const bool on = c * E < a.D && j < len && (!mb || mb[(int64_t)j * a.mask_k]);
+          cp16(dk + r * P + c * 16, on ? kb + (int64_t)j * a.ks[1] + c * E : kb, on ? 16u : 0u);
+          cp16(dv + r * P + c * 16, on ? vb + (int64_t)j * a.vs[1] + c * E : vb, on ? 16u : 0u);
+        }
+      } else {
+        for (int e = lane; e < 16 * DP; e += 32) {
+          const int r = e / DP, c = e % DP, j = j0 + r;
+          const bool on = c < a.D && j < len && (!mb || mb[(int64_t)j * a.mask_k]);
+          T* pk = reinterpret_cast<T*>(smem + (dk - sm) + r * P) + c;
+          T* pv = reinterpret_cast<T*>(smem + (dv - sm) + r * P) + c;
+          *pk = on ? kb[(int64_t)j * a.ks[1] + c] : from_f<T>(0.f);
+          *pv = on ? vb[(int64_t)j * a.vs[1] + c] : from_f<T>(0.f);
+        }
+      }
+    }
+    cp_commit();
+  };
+  stage_rows<T, DP>(sQ, 16, a.D, vec_q, tid, [&](int r) -> const T* {
+    return r < rows ? qb + (int64_t)(r % a.Lq) * a.qs[1] + (int64_t)(kh * G + r / a.Lq) * a.qs[2] : nullptr;
+  });
+  cp_commit();
+#pragma unroll
+  for (int x = 0; x < S - 1; ++x) load(x);
+  cp_wait<S - 1>();
+  __syncthreads();  // Q is there for every warp
+  FragA<T, sizeof(T) == 2 ? DP : 16> fq;
+  if constexpr (sizeof(T) == 2) fq.load(sQ, lane);
+
+  int qi[2];
+  const float* bias[2];
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    const int r = min(g + 8 * y, rows - 1);
+    qi[y] = r % a.Lq;
+    bias[y] = a.diag ? a.diag + (kh * G + r / a.Lq) * a.diag_ld + a.diag0 - qi[y] : nullptr;
+  }
+  const float sc = a.scale * kLog2e;
+  float o[DP / 8][4];
+#pragma unroll
+  for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) o[d][x] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  for (int x = 0; x < n; ++x) {
+    load(x + S - 1);
+    cp_wait<S - 1>();
+    __syncwarp();
+    const uint32_t sK = ring + (x % S) * 2 * 16 * P, sV = sK + 16 * P;
+    float s[2][4];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int z = 0; z < 4; ++z) s[c][z] = 0.f;
+    if constexpr (sizeof(T) == 2) fq.abt(s, sK, lane);
+    else mma_abt<T, DP, 2>(s, sQ, sK, lane);
+    const int j0 = (s0 + warp + 4 * x) * 16;
+    const bool whole = !mb && j0 + 16 <= len && (!a.causal || j0 + 16 <= min(qi[0], qi[1]) + a.q_off + 1);
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        const int j = j0 + c * 8 + 2 * t + (z & 1), y = z >> 1;
+        float v = s[c][z] * sc;
+        if (a.diag && j < a.Lk) v += __ldg(bias[y] + j);
+        if (!whole) {
+          const bool on = j < len && (!mb || mb[(int64_t)j * a.mask_k]) && (!a.causal || j <= qi[y] + a.q_off);
+          v = on ? v : -INFINITY;
+        }
+        s[c][z] = v;
+        mx[y] = fmaxf(mx[y], v);
+      }
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      mx[y] = fmaxf(mx[y], __shfl_xor_sync(0xffffffffu, mx[y], 1));
+      mx[y] = fmaxf(mx[y], __shfl_xor_sync(0xffffffffu, mx[y], 2));
+    }
+    const bool up[2] = {mx[0] > m[0] + 8.f, mx[1] > m[1] + 8.f};
+    if (__any_sync(0xffffffffu, up[0] || up[1])) {
+      float f[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        f[y] = up[y] ? (m[y] == -INFINITY ? 0.f : exp2_approx(m[y] - mx[y])) : 1.f;
+        m[y] = up[y] ? mx[y] : m[y];
+        l[y] *= f[y];
+      }
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+        for (int z = 0; z < 4; ++z) o[d][z] *= f[z >> 1];
+    }
+    const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        s[c][z] = exp2_approx(s[c][z] - base[z >> 1]);
+        l[z >> 1] += s[c][z];
+      }
+    mma_pb<T, DP, 2>(o, s, sV, lane);
+    __syncwarp();  // the ring's place is read before it is written again
+  }
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
+    l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
+  }
+  cp_wait<0>();
+  __syncthreads();
+  // parts of the four warps [4][16][DP + 4], this block's [16][DP + 4] behind, then (max, sum) of each
+  constexpr int LD = DP + 4;
+  float* part = reinterpret_cast<float*>(smem);
+  float* mine = part + 4 * 16 * LD;
+  float* ml = mine + 16 * LD;   // [4][16][2]
+  float* bml = ml + 4 * 32;     // [16][2]
+#pragma unroll
+  for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+    for (int z = 0; z < 4; ++z) part[(warp * 16 + g + 8 * (z >> 1)) * LD + d * 8 + 2 * t + (z & 1)] = o[d][z];
+  if (t == 0)
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      ml[2 * (warp * 16 + g + 8 * y)] = m[y];
+      ml[2 * (warp * 16 + g + 8 * y) + 1] = l[y];
+    }
+  __syncthreads();
+  for (int e = tid; e < rows * DP; e += kT) {
+    const int r = e / DP, d = e % DP;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[2 * (w * 16 + r)]);
+    float L = 0.f, v = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = ml[2 * (w * 16 + r)] == -INFINITY ? 0.f : exp2_approx(ml[2 * (w * 16 + r)] - M);
+      L = fmaf(f, ml[2 * (w * 16 + r) + 1], L);
+      v = fmaf(f, part[(w * 16 + r) * LD + d], v);
+    }
+    mine[r * LD + d] = v;
+    if (d == 0) {
+      bml[2 * r] = M;
+      bml[2 * r + 1] = L;
+    }
+  }
+  if (!CLUSTER && a.nsplit > 1) {
+    __syncthreads();
+    for (int e = tid; e < rows * a.D; e += kT) {
+      const int r = e / a.D, d = e % a.D;
+      const long long row = ((long long)b * a.Hq + kh * G + r / a.Lq) * a.Lq + r % a.Lq;
+      const long long pr = (long long)blockIdx.y * a.B * a.Hq * a.Lq + row;
+      a.po[pr * a.D + d] = mine[r * LD + d];
+      if (d == 0) {
+        a.pml[2 * pr] = bml[2 * r];
+        a.pml[2 * pr + 1] = bml[2 * r + 1];
+      }
+    }
+    return;
+  }
+  if (CLUSTER) cluster_sync();
+  else __syncthreads();
+  // the blocks of the cluster take the values in turn
+  const int ranks = CLUSTER ? a.nsplit : 1, rank = CLUSTER ? (int)blockIdx.y : 0;
+  const uint32_t at_o = ptx::smem_u32(mine), at_ml = ptx::smem_u32(bml);
+  for (int e = rank * kT + tid; e < rows * a.D; e += ranks * kT) {
+    const int r = e / a.D, d = e % a.D;
+    float M, L, v;
+    if (CLUSTER) {
+      float ms[kCluster];
+      M = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < kCluster; ++c) {
+        ms[c] = c < ranks ? ld_cluster(at_ml + 8 * r, c) : -INFINITY;
+        M = fmaxf(M, ms[c]);
+      }
+      L = v = 0.f;
+#pragma unroll
+      for (int c = 0; c < kCluster; ++c)
+        if (c < ranks) {
+          const float f = ms[c] == -INFINITY ? 0.f : exp2_approx(ms[c] - M);
+          L = fmaf(f, ld_cluster(at_ml + 8 * r + 4, c), L);
+          v = fmaf(f, ld_cluster(at_o + 4 * (r * LD + d), c), v);
+        }
+    } else {
+      M = bml[2 * r], L = bml[2 * r + 1], v = mine[r * LD + d];
+    }
+    const int i = r % a.Lq, h = kh * G + r / a.Lq;
+    static_cast<T*>(a.out)[(((long long)b * a.Lq + i) * a.Hq + h) * a.D + d] = from_f<T>(L > 0.f ? v / L : 0.f);
+    if (d == 0) a.lse[((long long)b * a.Hq + h) * a.Lq + i] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+  }
+  if (CLUSTER) cluster_sync();  // no block leaves while another reads its memory
 }
 
 // Joins the splits of a row: one warp per row, lanes over the head dimension.
@@ -714,31 +961,63 @@ __global__ void __launch_bounds__(kT) attn_mma_dkv_kernel(const __grid_constant_
   }
 }
 
-void allow_smem(const void* f, size_t smem) {
-  if (smem > 48 * 1024)
-    RVC_CUDA_TRY(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+// Lifts a kernel's limit of dynamic shared memory once per device.
+template <auto K>
+void allow_smem(size_t smem) {
+  static std::atomic<uint64_t> done{0};
+  if (smem <= 48 * 1024) return;
+  int dev = 0;
+  RVC_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & (1ull << dev))) return;
+  RVC_CUDA_TRY(cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+  if (dev < 64) done.fetch_or(1ull << dev);
+}
+
+bool few_rows(const AttnArgs& a) { return (long long)(a.Hq / a.Hkv) * a.Lq <= 16; }
+
+template <typename T, int DP>
+void few_dp(const AttnArgs& a, cudaStream_t st) {
+  const int vq = aligned16(a, a.q, a.qs), vkv = aligned16(a, a.k, a.ks) && aligned16(a, a.v, a.vs);
+  constexpr size_t smem = few_smem<T, DP>();
+  const dim3 grid((unsigned)(a.B * a.Hkv), a.nsplit);
+  if (a.nsplit > 1 && a.nsplit <= kCluster) {
+    allow_smem<attn_mma_few_kernel<T, DP, true>>(smem);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kT);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 1;
+    at[0].val.clusterDim.y = a.nsplit;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    RVC_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn_mma_few_kernel<T, DP, true>, a, vq, vkv));
+  } else {
+    allow_smem<attn_mma_few_kernel<T, DP, false>>(smem);
+    attn_mma_few_kernel<T, DP, false><<<grid, kT, smem, st>>>(a, vq, vkv);
+  }
+  note_launch();
+  RVC_CUDA_TRY(cudaGetLastError());
 }
 
 template <typename T, int DP>
 void fwd_dp(const AttnArgs& a, cudaStream_t st) {
-  const int vq = aligned16(a, a.q, a.qs), vkv = aligned16(a, a.k, a.ks) && aligned16(a, a.v, a.vs);
-  const long long rows = (long long)(a.Hq / a.Hkv) * a.Lq;
-  constexpr int P = pitch<T, DP>();
-  const bool few = rows <= 16;
-  const int R = few ? 16 : kBM;
-  size_t smem = (size_t)(R + 4 * kBN) * P;
-  if (few) smem = std::max(smem, (size_t)(4 * 16 * (DP + 4) + 128) * 4);
-  const dim3 grid((unsigned)((rows + R - 1) / R * a.B * a.Hkv), a.nsplit);
-  if (few) {
-    allow_smem((const void*)attn_mma_fwd_kernel<T, DP, 16>, smem);
-    attn_mma_fwd_kernel<T, DP, 16><<<grid, kT, smem, st>>>(a, vq, vkv);
+  if (few_rows(a)) {
+    few_dp<T, DP>(a, st);
   } else {
-    allow_smem((const void*)attn_mma_fwd_kernel<T, DP, kBM>, smem);
-    attn_mma_fwd_kernel<T, DP, kBM><<<grid, kT, smem, st>>>(a, vq, vkv);
+    const int vq = aligned16(a, a.q, a.qs), vkv = aligned16(a, a.k, a.ks) && aligned16(a, a.v, a.vs);
+    const long long rows = (long long)(a.Hq / a.Hkv) * a.Lq;
+    const size_t smem = (size_t)(kBM + 4 * kBN) * pitch<T, DP>();
+    const dim3 grid((unsigned)((rows + kBM - 1) / kBM * a.B * a.Hkv), a.nsplit);
+    allow_smem<attn_mma_fwd_kernel<T, DP>>(smem);
+    attn_mma_fwd_kernel<T, DP><<<grid, kT, smem, st>>>(a, vq, vkv);
+    note_launch();
+    RVC_CUDA_TRY(cudaGetLastError());
   }
-  note_launch();
-  RVC_CUDA_TRY(cudaGetLastError());
-  if (a.nsplit > 1) {
+  if (a.po) {
     const long long n = (long long)a.B * a.Hq * a.Lq;
     attn_join_kernel<T><<<(unsigned)((n + 7) / 8), 256, 0, st>>>(a, n);
     note_launch();
@@ -758,13 +1037,13 @@ void bwd_dp(const AttnArgs& a, cudaStream_t st) {
     if constexpr (sizeof(T) == 4) {
       attn_delta_kernel<<<(unsigned)((n + 7) / 8), 256, 0, st>>>(a, n);
     } else {
-      allow_smem((const void*)attn_mma_dq_kernel<T, DP, BN, true>, smem);
+      allow_smem<attn_mma_dq_kernel<T, DP, BN, true>>(smem);
       attn_mma_dq_kernel<T, DP, BN, true>
           <<<(unsigned)((a.Lq + kBM - 1ll) / kBM * a.B * a.Hq), kT, smem, st>>>(a, vq, vkv, vdo);
     }
     note_launch();
     RVC_CUDA_TRY(cudaGetLastError());
-    allow_smem((const void*)attn_mma_dq_kernel<T, DP, BN, false>, smem);
+    allow_smem<attn_mma_dq_kernel<T, DP, BN, false>>(smem);
     attn_mma_dq_kernel<T, DP, BN, false>
         <<<(unsigned)((a.Lq + kBM - 1ll) / kBM * a.B * a.Hq), kT, smem, st>>>(a, vq, vkv, vdo);
     note_launch();
@@ -772,7 +1051,7 @@ void bwd_dp(const AttnArgs& a, cudaStream_t st) {
   }
   if (a.Lk > 0) {
     const size_t smem = (size_t)(2 * kBN + 4 * BN) * P + 4 * BN * 4;
-    allow_smem((const void*)attn_mma_dkv_kernel<T, DP, BN>, smem);
+    allow_smem<attn_mma_dkv_kernel<T, DP, BN>>(smem);
     attn_mma_dkv_kernel<T, DP, BN>
         <<<(unsigned)((a.Lk + kBN - 1ll) / kBN * a.B * a.Hkv), kT, smem, st>>>(a, vq, vkv, vdo);
     note_launch();
@@ -797,16 +1076,32 @@ void bwd_t(const AttnArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-// Splits of the keys: enough blocks for every SM to hold a few, at least two
-// key tiles each.
-int attn_mma_splits(const AttnArgs& a, int sms) {
+// Splits of the keys.  Many rows: enough blocks for two to an SM, at least two
+// key tiles each.  Few rows: 64 keys at least (a step for each warp), no more
+// than four blocks to an SM, a power of two up to kCluster (a GPU cluster's
+// blocks share a group of 16 to 18 SMs); where that leaves SMs without work (a
+// single long sequence), as many as fill the GPU, through the workspace.
+int attn_mma_splits(const AttnArgs& a, int sms, bool* workspace) {
   const long long rows = (long long)(a.Hq / a.Hkv) * a.Lq;
-  const int R = rows <= 16 ? 16 : kBM;
-  const long long blocks = (rows + R - 1) / R * a.B * a.Hkv;
+  *workspace = false;
+  if (rows == 0 || a.B == 0) return 1;
+  if (few_rows(a)) {
+    const long long blocks = (long long)a.B * a.Hkv;
+    const long long n = std::min((a.Lk + 63ll) / 64, (4ll * sms + blocks - 1) / blocks);
+    if (n > kCluster && blocks * kCluster < sms) {
+      *workspace = true;
+      return (int)std::min<long long>({n, (sms + blocks - 1) / blocks, 128ll});
+    }
+    int p = 1;
+    while (p < n && p < kCluster) p *= 2;
+    return p;
+  }
+  const long long blocks = (rows + kBM - 1) / kBM * a.B * a.Hkv;
   const int tiles = (a.Lk + kBN - 1) / kBN;
-  if (blocks == 0 || tiles < 2) return 1;
   const long long want = (2ll * sms + blocks - 1) / blocks;
-  return (int)std::max(1ll, std::min({want, (long long)(tiles / 2), 64ll}));
+  const int n = (int)std::max(1ll, std::min({want, (long long)(tiles / 2), 64ll}));
+  *workspace = n > 1;
+  return n;
 }
 
 void attn_mma_forward(const AttnArgs& a, cudaStream_t st) {

@@ -147,16 +147,16 @@ _SIGS = {
     "rvc_cuda_index_set_ivf": ([_i64, _fp, _i32, _ip64], _i32),
     "rvc_cuda_index_ivf_search": ([_i64, _fp, _i64, _i32, _i32, _i32, _fp, _ip64], _i32),
     "rvc_cuda_index_ivf_blend": ([_i64, _fp, _i64, _i32, _i32, _i32, _f64, _fp, _fp], _i32),
-    "rvc_cuda_attention_workspace": ([_i64, _ip64, _i32, _i32, _ip64], _i32),
-    "rvc_cuda_attention_device": ([_i64, _p, _ip64, _i32, _f64] + [_p] * 7 + [_i32, _p, _p, _p, _i64], _i32),
-    "rvc_cuda_attention_backward_device": ([_i64, _p, _ip64, _i32, _f64] + [_p] * 10 + [_i32] + [_p] * 5 + [_i64],
-                                           _i32),
-    "rvc_cuda_relative_bias_device": ([_i64, _p, _ip64, _i32, _p, _p, _i32, _p], _i32),
-    "rvc_cuda_relative_bias_workspace": ([_i64, _ip64, _i32, _ip64], _i32),
-    "rvc_cuda_relative_bias_backward_device": ([_i64, _p, _ip64, _i32, _p, _p, _i32, _p, _p, _i64], _i32),
-    "rvc_cuda_qk_norm_rope_device": ([_i64, _p, _ip64, _i32, _f64] + [_p] * 9, _i32),
-    "rvc_cuda_qk_norm_rope_workspace": ([_i64, _ip64, _i32, _ip64], _i32),
-    "rvc_cuda_qk_norm_rope_backward_device": ([_i64, _p, _ip64, _i32, _f64] + [_p] * 14 + [_i64], _i32),
+    # descriptors (packed int64 values) go in as bytes
+    "rvc_cuda_attention_workspace": ([_i64, _p, _i32, _i32, _ip64], _i32),
+    "rvc_cuda_attention_device": ([_i64, _p, _p, _i32, _f64] + [_p] * 7 + [_i32, _p, _p, _p, _i64], _i32),
+    "rvc_cuda_attention_backward_device": ([_i64, _p, _p, _i32, _f64] + [_p] * 10 + [_i32] + [_p] * 5 + [_i64], _i32),
+    "rvc_cuda_relative_bias_device": ([_i64, _p, _p, _i32, _p, _p, _i32, _p], _i32),
+    "rvc_cuda_relative_bias_workspace": ([_i64, _p, _i32, _ip64], _i32),
+    "rvc_cuda_relative_bias_backward_device": ([_i64, _p, _p, _i32, _p, _p, _i32, _p, _p, _i64], _i32),
+    "rvc_cuda_qk_norm_rope_device": ([_i64, _p, _p, _i32, _f64] + [_p] * 9, _i32),
+    "rvc_cuda_qk_norm_rope_workspace": ([_i64, _p, _i32, _ip64], _i32),
+    "rvc_cuda_qk_norm_rope_backward_device": ([_i64, _p, _p, _i32, _f64] + [_p] * 14 + [_i64], _i32),
 }
 for _name, (_args, _ret) in _SIGS.items():
     _fn = getattr(lib, _name)

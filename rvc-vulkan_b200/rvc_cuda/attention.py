@@ -25,6 +25,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import struct
 from typing import Optional
 
 import numpy as np
@@ -37,12 +38,15 @@ __all__ = ["BucketBias", "attention", "attention_backward", "relative_bias", "re
            "qk_norm_rope", "qk_norm_rope_backward", "rope_table"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+# torch's own short way to the current stream's handle, a microsecond less than the public one
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda i: torch.cuda.current_stream(i).cuda_stream)
 MAX_HEAD_DIM = 128
 MAX_BUCKETS = 1024
 
-_Desc29 = C.c_int64 * 29
-_Desc25 = C.c_int64 * 25
-_Desc11 = C.c_int64 * 11
+_pack29 = struct.Struct("=29q").pack
+_pack25 = struct.Struct("=25q").pack
+_pack11 = struct.Struct("=11q").pack
 
 
 @functools.lru_cache(maxsize=64)
@@ -105,6 +109,7 @@ class BucketBias:
 
 
 def _tensor(x, name: str, ndim: int, like=None):
+    """``x`` with its last dimension contiguous, checked against ``like``."""
     if not isinstance(x, torch.Tensor):
         raise ValueError(f"{name}: a tensor is expected")
     if x.dim() != ndim:
@@ -112,24 +117,27 @@ def _tensor(x, name: str, ndim: int, like=None):
     if like is None:
         if x.dtype not in _TYPES:
             raise ValueError(f"{name}: float32, bfloat16 or float16 expected, got {x.dtype}")
-    else:
-        if x.dtype != like.dtype:
-            raise ValueError(f"{name}: {like.dtype} expected, got {x.dtype}")
-        if x.device != like.device:
-            raise ValueError(f"{name}: on {x.device}, expected {like.device}")
+    elif x.dtype is not like.dtype:
+        raise ValueError(f"{name}: {like.dtype} expected, got {x.dtype}")
+    elif x.get_device() != like.get_device():
+        raise ValueError(f"{name}: on {x.device}, expected {like.device}")
     return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
 
 
 def _where(x):
-    """(context handle, stream of the tensor's device)."""
-    if not x.is_cuda:
+    """(context handle, raw stream of the tensor's device)."""
+    i = x.get_device()
+    if i < 0:
         raise ValueError(f"CUDA tensors are expected, got one on {x.device}")
-    i = x.device.index
-    return _lib.get_context(i).handle, torch.cuda.current_stream(i).cuda_stream
+    return _lib.get_context(i).handle, _raw_stream(i)
 
 
-def _scratch(nbytes: int, like):
-    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+def _scratch(fn, ctx, desc, n, like, *how):
+    """Workspace that ``fn`` (a ``*_workspace`` entry) asks for: (tensor or None, bytes)."""
+    need = C.c_int64(0)
+    check(fn(ctx, desc, n, *how, need))
+    nbytes = need.value
+    return (torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None), nbytes
 
 
 def _ptr(x):
@@ -140,8 +148,8 @@ def _qkv(q, k, v):
     q = _tensor(q, "q", 4)
     k, v = _tensor(k, "k", 4, q), _tensor(v, "v", 4, q)
     B, Lq, Hq, D = q.shape
-    Lk, Hkv = k.shape[1], k.shape[2]
-    if k.shape[0] != B or k.shape[3] != D or v.shape != k.shape:
+    Bk, Lk, Hkv, Dk = k.shape
+    if Bk != B or Dk != D or v.shape != k.shape:
         raise ValueError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match "
                          "[B, Lq, Hq, D] and [B, Lk, Hkv, D]")
     if not 1 <= D <= MAX_HEAD_DIM:
@@ -214,16 +222,15 @@ def attention(q, k, v, *, kv_lens=None, key_mask=None, scale: Optional[float] = 
     mask, mb, mk = _mask(key_mask, B, Lk, q)
     table, nb, both, borders, nborders = _table(bias, Hq, q)
     ctx, stream = _where(q)
-    desc = _Desc29(_TYPES[q.dtype], B, Hq, Hkv, Lq, Lk, D, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], bits, mb,
-                   mk, int(bool(causal)), int(q_offset), nb, both)
-    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    desc = _pack29(_TYPES[q.dtype], B, Hq, Hkv, Lq, Lk, D, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1],
+                   vs[2], bits, mb, mk, bool(causal), q_offset, nb, both, 0, 0, 0, 0, 0, 0)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device)
-    need = C.c_int64(0)
-    check(lib.rvc_cuda_attention_workspace(ctx, desc, 29, 0, need))
-    ws = _scratch(need.value, q)
+    ws, nbytes = _scratch(lib.rvc_cuda_attention_workspace, ctx, desc, 29, q, 0)
     check(lib.rvc_cuda_attention_device(ctx, stream, desc, 29, _scale(scale, D), q.data_ptr(), k.data_ptr(),
                                         v.data_ptr(), _ptr(lens), _ptr(mask), _ptr(table), borders, nborders,
-                                        out.data_ptr(), lse.data_ptr(), _ptr(ws), need.value))
+                                        out.data_ptr(), lse.data_ptr(), _ptr(ws), nbytes))
     return out, lse
 
 
@@ -251,19 +258,15 @@ def attention_backward(dout, q, k, v, out, lse, *, kv_lens=None, key_mask=None, 
     mask, mb, mk = _mask(key_mask, B, Lk, q)
     table, nb, both, borders, nborders = _table(bias, Hq, q)
     ctx, stream = _where(q)
-    desc = _Desc29(_TYPES[q.dtype], B, Hq, Hkv, Lq, Lk, D, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], bits, mb,
-                   mk, int(bool(causal)), int(q_offset), nb, both, *dout.stride()[:3], *out.stride()[:3])
-    dq = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
-    dk = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=q.device)
-    dv = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=q.device)
+    desc = _pack29(_TYPES[q.dtype], B, Hq, Hkv, Lq, Lk, D, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], bits, mb,
+                   mk, bool(causal), q_offset, nb, both, *dout.stride()[:3], *out.stride()[:3])
+    dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
     dtable = torch.empty((nb, Hq), dtype=q.dtype, device=q.device) if nb else None
-    need = C.c_int64(0)
-    check(lib.rvc_cuda_attention_workspace(ctx, desc, 29, 1, need))
-    ws = _scratch(need.value, q)
+    ws, nbytes = _scratch(lib.rvc_cuda_attention_workspace, ctx, desc, 29, q, 1)
     check(lib.rvc_cuda_attention_backward_device(
         ctx, stream, desc, 29, _scale(scale, D), dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
         out.data_ptr(), lse.data_ptr(), _ptr(lens), _ptr(mask), _ptr(table), borders, nborders, dq.data_ptr(),
-        dk.data_ptr(), dv.data_ptr(), _ptr(dtable), _ptr(ws), need.value))
+        dk.data_ptr(), dv.data_ptr(), _ptr(dtable), _ptr(ws), nbytes))
     return (dq, dk, dv) if dtable is None else (dq, dk, dv, dtable)
 
 
@@ -281,7 +284,7 @@ def relative_bias(bias: BucketBias, Lq: int, Lk: int, *, q_offset: int = 0):
         raise ValueError(f"relative_bias: lengths {Lq} and {Lk}")
     ctx, stream = _where(t)
     out = torch.empty((H, Lq, Lk), dtype=t.dtype, device=t.device)
-    desc = _Desc11(_TYPES[t.dtype], 1, H, Lq, Lk, int(q_offset), bias.num_buckets, int(bias.bidirectional))
+    desc = _pack11(_TYPES[t.dtype], 1, H, Lq, Lk, q_offset, bias.num_buckets, bias.bidirectional, 0, 0, 0)
     check(lib.rvc_cuda_relative_bias_device(ctx, stream, desc, 11, t.data_ptr(), bias._borders, bias._nborders,
                                             out.data_ptr()))
     return out
@@ -303,14 +306,11 @@ def relative_bias_backward(bias: BucketBias, dbias, *, q_offset: int = 0):
     if H != bias.table.shape[1]:
         raise ValueError(f"relative_bias_backward: {H} heads, the table has {bias.table.shape[1]}")
     ctx, stream = _where(d)
-    desc = _Desc11(_TYPES[d.dtype], B, H, Lq, Lk, int(q_offset), bias.num_buckets, int(bias.bidirectional),
-                   *d.stride()[:3])
+    desc = _pack11(_TYPES[d.dtype], B, H, Lq, Lk, q_offset, bias.num_buckets, bias.bidirectional, *d.stride()[:3])
     dtable = torch.empty((bias.num_buckets, H), dtype=d.dtype, device=d.device)
-    need = C.c_int64(0)
-    check(lib.rvc_cuda_relative_bias_workspace(ctx, desc, 11, need))
-    ws = _scratch(need.value, d)
+    ws, nbytes = _scratch(lib.rvc_cuda_relative_bias_workspace, ctx, desc, 11, d)
     check(lib.rvc_cuda_relative_bias_backward_device(ctx, stream, desc, 11, d.data_ptr(), bias._borders,
-                                                     bias._nborders, dtable.data_ptr(), _ptr(ws), need.value))
+                                                     bias._nborders, dtable.data_ptr(), _ptr(ws), nbytes))
     return dtable
 
 
@@ -338,33 +338,41 @@ def _rope(q, k, q_weight, k_weight, cos, sin, positions, interleaved, name):
         raise ValueError(f"{name}: q {tuple(q.shape)} and k {tuple(k.shape)} do not match [B, L, heads, D]")
     if D < 2 or D > 256 or D % 2:
         raise ValueError(f"{name}: head dimension {D}; even ones from 2 to 256 are supported")
+    dev = q.get_device()
     for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if not isinstance(w, torch.Tensor) or w.shape != (D,) or w.device != q.device:
+        if not isinstance(w, torch.Tensor) or w.shape != (D,) or w.get_device() != dev:
             raise ValueError(f"{name}: {n} [{D}] on {q.device} expected")
         if w.dtype not in (torch.float32, q.dtype) or w.dtype != q_weight.dtype:
             raise ValueError(f"{name}: the weights are both float32 or both {q.dtype}")
     for t, n in ((cos, "cos"), (sin, "sin")):
-        if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.dtype != torch.float32 or t.device != q.device:
+        if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.dtype is not torch.float32 or t.get_device() != dev:
             raise ValueError(f"{name}: {n} must be a float32 [positions, rotary_dim / 2] on {q.device}")
     if cos.shape != sin.shape or 2 * cos.shape[1] > D:
         raise ValueError(f"{name}: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} do not fit head dimension {D}")
     bits = pb = pl = 0
     if positions is not None:
-        if not isinstance(positions, torch.Tensor) or positions.device != q.device:
+        if not isinstance(positions, torch.Tensor) or positions.get_device() != dev:
             raise ValueError(f"{name}: positions must be a tensor on {q.device}")
-        if positions.dtype not in (torch.int32, torch.int64) or positions.shape not in ((B, L), (L,)):
-            raise ValueError(f"{name}: positions int32 or int64 [{B}, {L}] or [{L}] expected, got {positions.dtype} "
-                             f"{tuple(positions.shape)}")
-        bits = 32 if positions.dtype == torch.int32 else 64
-        positions = positions.expand(B, L)
-        pb, pl = positions.stride()
+        if positions.shape == (B, L):
+            pb, pl = positions.stride()
+        elif positions.shape == (L,):
+            pl = positions.stride(0)
+        else:
+            raise ValueError(f"{name}: positions [{B}, {L}] or [{L}] expected, got {tuple(positions.shape)}")
+        if positions.dtype is torch.int64:
+            bits = 64
+        elif positions.dtype is torch.int32:
+            bits = 32
+        else:
+            raise ValueError(f"{name}: positions are int32 or int64, got {positions.dtype}")
     elif L > cos.shape[0] and cos.shape[1]:
         raise ValueError(f"{name}: the tables hold {cos.shape[0]} positions, fewer than the {L} rows")
     if B * L == 0:
         positions = None
         bits = 0
-    head = (_TYPES[q.dtype], _TYPES[q_weight.dtype], B, L, Hq, Hk, D, 2 * cos.shape[1], cos.shape[0],
-            int(bool(interleaved)), bits, pb, pl)
+    qs, ks = q.stride(), k.stride()
+    head = (_TYPES[q.dtype], _TYPES[q_weight.dtype], B, L, Hq, Hk, D, 2 * cos.shape[1], cos.shape[0], bool(interleaved),
+            bits, pb, pl, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2])
     return q, k, q_weight.contiguous(), k_weight.contiguous(), cos.contiguous(), sin.contiguous(), positions, head
 
 
@@ -382,9 +390,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps: flo
     q, k, wq, wk, cos, sin, pos, head = _rope(q, k, q_weight, k_weight, cos, sin, positions, interleaved,
                                               "qk_norm_rope")
     ctx, stream = _where(q)
-    desc = _Desc25(*head, *q.stride()[:3], *k.stride()[:3])
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    desc = _pack25(*head, 0, 0, 0, 0, 0, 0)
+    qo, ko = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k))
     check(lib.rvc_cuda_qk_norm_rope_device(ctx, stream, desc, 25, float(eps), q.data_ptr(), k.data_ptr(),
                                            wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ptr(pos),
                                            qo.data_ptr(), ko.data_ptr()))
@@ -403,17 +410,14 @@ def qk_norm_rope_backward(dqo, dko, q, k, q_weight, k_weight, cos, sin, *, posit
         raise ValueError(f"qk_norm_rope_backward: dqo {tuple(gq.shape)}, dko {tuple(gk.shape)} for q {tuple(q.shape)}, "
                          f"k {tuple(k.shape)}")
     ctx, stream = _where(q)
-    desc = _Desc25(*head, *q.stride()[:3], *k.stride()[:3], *gq.stride()[:3], *gk.stride()[:3])
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    desc = _pack25(*head, *gq.stride()[:3], *gk.stride()[:3])
+    dq, dk = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k))
     dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
     if k.shape[2] == 0:
         dwk.zero_()
-    need = C.c_int64(0)
-    check(lib.rvc_cuda_qk_norm_rope_workspace(ctx, desc, 25, need))
-    ws = _scratch(need.value, q)
+    ws, nbytes = _scratch(lib.rvc_cuda_qk_norm_rope_workspace, ctx, desc, 25, q)
     check(lib.rvc_cuda_qk_norm_rope_backward_device(
         ctx, stream, desc, 25, float(eps), gq.data_ptr(), gk.data_ptr(), q.data_ptr(), k.data_ptr(), wq.data_ptr(),
         wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ptr(pos), dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(),
-        dwk.data_ptr(), _ptr(ws), need.value))
+        dwk.data_ptr(), _ptr(ws), nbytes))
     return dq, dk, dwq, dwk

@@ -560,13 +560,13 @@ def test_numpy_forms():
 
 def test_workspace_is_checked():
     """The C entry point refuses a workspace that is too small before any launch."""
-    c = Case("bf16", 1, 4, 4, 64, 1, 4096)
-    desc = (A.C.c_int64 * 29)(1, 1, 4, 4, 1, 4096, 64, *c.q.stride()[:3], *c.k.stride()[:3], *c.v.stride()[:3])
+    c = Case("bf16", 1, 1, 1, 64, 1, 32768)  # one row on long states: split through the workspace
+    desc = (A.C.c_int64 * 29)(1, 1, 1, 1, 1, 32768, 64, *c.q.stride()[:3], *c.k.stride()[:3], *c.v.stride()[:3])
     ctx = _lib.get_context().handle
     need = A.C.c_int64(0)
     _lib.check(_lib.lib.rvc_cuda_attention_workspace(ctx, desc, 29, 0, need))
     assert need.value > 0
-    out, lse, ws = torch.empty_like(c.q), torch.empty(4, device="cuda"), torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    out, lse, ws = torch.empty_like(c.q), torch.empty(1, device="cuda"), torch.empty(need.value, dtype=torch.uint8, device="cuda")
     n0 = _lib.launch_count()
 
     def call(ws_ptr, nbytes, n=29, lse_ptr=lse.data_ptr()):
