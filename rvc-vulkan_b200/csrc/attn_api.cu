@@ -25,27 +25,31 @@ __global__ void expand_bias_kernel(const T* __restrict__ table, int H, long long
 // Tiles of BM queries (by_key = 0) hold it at x - (Lq - 1) + BM - 1 + t BM, tiles
 // of BM keys at (Lq - 1) - x + BM - 1 + t BM; there the last two entries of a
 // tile are sums that lie whole in the last bucket behind / ahead.
-__global__ void diag_sums_kernel(const float* __restrict__ ws, int B, int H, int nt, int BM, int by_key, long long ld,
-                                 long long Lq, long long Lk, double* __restrict__ sums, double* __restrict__ far) {
-  const long long x = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+// Block: 32 diagonals x 8 shares of the (tile, batch) list, joined in order.
+__global__ void __launch_bounds__(256) diag_sums_kernel(const float* __restrict__ ws, int B, int H, int nt, int BM,
+                                                        int by_key, long long ld, long long Lq, long long Lk,
+                                                        double* __restrict__ sums, double* __restrict__ far) {
+  __shared__ double red[8][32];
+  const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const long long x = (long long)blockIdx.x * 32 + lane;
   const int h = blockIdx.y;
   const long long n = Lq + Lk - 1;
-  if (x >= n + 2) return;
+  const long long d = x - (Lq - 1), top = by_key ? ld - 2 : ld;
   double s = 0.0;
-  if (x < n) {
-    const long long d = x - (Lq - 1), top = by_key ? ld - 2 : ld;
-    for (int t = 0; t < nt; ++t) {
-      const long long e = (by_key ? -d : d) + BM - 1 + (long long)t * BM;
-      if (e < 0 || e >= top) continue;
-      for (int b = 0; b < B; ++b) s += ws[(((long long)b * H + h) * nt + t) * ld + e];
+  if (x < n || (x < n + 2 && by_key))
+#pragma unroll 4
+    for (long long k = y; k < (long long)B * nt; k += 8) {
+      const long long t = k / B, b = k % B;
+      const long long e = x < n ? (by_key ? -d : d) + BM - 1 + t * BM : top + (x - n);
+      if (e >= 0 && (e < top || x >= n)) s += ws[((b * H + h) * nt + t) * ld + e];
     }
-    sums[h * n + x] = s;
-  } else {
-    if (by_key)
-      for (long long e = 0; e < (long long)B * nt; ++e)
-        s += ws[(((e / nt) * H + h) * nt + e % nt) * ld + ld - 2 + (x - n)];
-    far[h * 2 + (x - n)] = s;
-  }
+  red[y][lane] = s;
+  __syncthreads();
+  if (y) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) s += red[k][lane];
+  if (x < n) sums[h * n + x] = s;
+  else if (x < n + 2) far[h * 2 + (x - n)] = s;
 }
 
 // One block per (bucket, head): its diagonals are a run, found with the borders.
@@ -218,7 +222,7 @@ void attn_backward(AttnArgs a, const void* table, const BucketRule* rule, void* 
   if (rule) {
     double *sums = at<double>(ws, l.sums), *far = at<double>(ws, l.far);
     const int64_t n = (int64_t)a.Lq + a.Lk + 1;
-    diag_sums_kernel<<<dim3((unsigned)((n + 127) / 128), a.Hq), 128, 0, st>>>(
+    diag_sums_kernel<<<dim3((unsigned)((n + 31) / 32), a.Hq), 256, 0, st>>>(
         a.dws, a.B, a.Hq, l.nt, l.BM, l.tc ? 1 : 0, l.dws_ld, a.Lq, a.Lk, sums, far);
     note_launch();
     RVC_CUDA_TRY(cudaGetLastError());

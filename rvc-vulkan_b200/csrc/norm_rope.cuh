@@ -20,8 +20,9 @@ struct RopeArgs {
   int64_t pos_b = 0, pos_l = 0;
   void *oq = nullptr, *ok = nullptr;           // contiguous outputs / input gradients
   void *dwq = nullptr, *dwk = nullptr;
-  float* part = nullptr;                       // [blocks][2][D] partial weight gradients
+  float* part = nullptr;                       // [blocks][D] partial weight gradients
   int head_block = 0;                          // heads of one item
+  int q_blocks = 0;                            // blocks of the queries, the others take the keys
 };
 
 int64_t rope_backward_workspace(const RopeArgs& a, int sms);
