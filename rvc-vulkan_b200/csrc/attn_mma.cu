@@ -56,14 +56,14 @@ __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t tf32_rn(float x) {
-  uint32_t r;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-  return r;
-}
+// x = hi + lo: hi rounded to TF32's 11 bits on the integer form (half away from
+// zero; a carry runs into the exponent as it should, infinities and NaN stay
+// themselves or become NaN), the rest exact, and cut to 11 bits by the tensor
+// core, which reads no more.  The conversion instruction runs at a fraction of
+// this rate.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-  hi = tf32_rn(x);
-  lo = tf32_rn(x - __uint_as_float(hi));
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
 }
 struct Split4 {
   uint32_t hi[4], lo[4];
