@@ -199,7 +199,11 @@ int64_t attn_workspace(const AttnArgs& a, bool bias, bool backward, int sms) {
 void attn_forward(AttnArgs a, const void* table, const BucketRule* rule, void* ws, int sms, cudaStream_t st) {
   const Layout l = plan(a, rule != nullptr, false, sms, use_tc(a, false));
   apply(a, l, ws);
-  if (rule) attn_expand_bias(a, table, *rule, const_cast<float*>(a.diag), st);
+  if (rule) {
+    a.far = rule->nb ? rule->border[rule->nb - 1] : 1;
+    a.far_both = rule->both;
+    attn_expand_bias(a, table, *rule, const_cast<float*>(a.diag), st);
+  }
   if (l.tc)
     attn_tc_forward(a, st);
   else

@@ -75,29 +75,40 @@ namespace {
 
 using namespace atc;
 
-constexpr int kFwdThreads = 320;
+constexpr int kFwdThreads = 384;  // three warpgroups: two of softmax, one of loader and issuer
 constexpr float kGrow = 8.f;  // log2 of the growth of a maximum that is taken without rescaling
 
 struct FwdMaps {
   CUtensorMap q, k, v;
 };
 
-// shared memory: Q [2 tiles][NS], K [2 stages][NS], V [2][NS] slabs, bias [2][384], barriers
-template <int NS> constexpr uint32_t fwd_smem() { return 6 * NS * kSlab + 2 * 384 * 4 + 256 + 1024; }
+// Key tiles under way: a load takes about as long as a tile of 128 values does,
+// two tiles of 64 and more.
+template <int NS> constexpr int kRing = NS == 1 ? 4 : 2;
+// shared memory: Q [2 tiles][NS], K [stages][NS], V [stages][NS] slabs, bias [stages][384], barriers
+template <int NS> constexpr uint32_t fwd_smem() {
+  return (2 + 2 * kRing<NS>) * NS * kSlab + kRing<NS> * 384 * 4 + 512 + 1024;
+}
 
-template <typename T, int NS>
+// FULL: the head dimension is 64 NS, its steps are known to the compiler.
+template <typename T, int NS, bool FULL>
 __global__ void __launch_bounds__(kFwdThreads, 1)
     attn_tc_fwd_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ FwdMaps maps) {
+  // Heads of 64 leave columns of tensor memory for P beside S, so that the next
+  // product into S starts as soon as the softmax has read this one.
+  constexpr bool APART = false;
+  constexpr int R = kRing<NS>;
   extern __shared__ uint8_t raw[];
   const uint32_t base = (ptx::smem_u32(raw) + 1023) & ~1023u;
   uint8_t* gen = raw + (base - ptx::smem_u32(raw));
-  const uint32_t sQ = base, sK = sQ + 2 * NS * kSlab, sV = sK + 2 * NS * kSlab;
-  const uint32_t oB = 6 * NS * kSlab, oBar = oB + 2 * 384 * 4;
+  const uint32_t sQ = base, sK = sQ + 2 * NS * kSlab, sV = sK + R * NS * kSlab;
+  const uint32_t oB = (2 + 2 * R) * NS * kSlab, oBar = oB + R * 384 * 4;
   const float* bias_s = reinterpret_cast<const float*>(gen + oB);
   const uint32_t bar = base + oBar;
-  const uint32_t Q_FULL = bar, K_FULL = bar + 8, V_FULL = bar + 24, K_EMPTY = bar + 40, V_EMPTY = bar + 56,
-                 S_FULL = bar + 72, P_FULL = bar + 88, O_DONE = bar + 104, DRAIN = bar + 120;
-  uint32_t* slot = reinterpret_cast<uint32_t*>(gen + oBar + 128);
+  const uint32_t Q_FULL = bar, K_FULL = bar + 8, V_FULL = K_FULL + 8 * R, K_EMPTY = V_FULL + 8 * R,
+                 V_EMPTY = K_EMPTY + 8 * R, S_FULL = V_EMPTY + 8 * R, P_FULL = S_FULL + 16 /* [2 tiles][2 halves] */,
+                 O_DONE = P_FULL + 32, S_FREE = O_DONE + 16, DRAIN = S_FREE + 16;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(gen + oBar + 248);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   const int npair = (a.Lq + 255) / 256;
@@ -111,14 +122,18 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 
   if (threadIdx.x == 0) {
     ptx::mbar_init(Q_FULL, 1);
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < R; ++s) {
       ptx::mbar_init(K_FULL + 8 * s, 1);
       ptx::mbar_init(V_FULL + 8 * s, 1);
       ptx::mbar_init(K_EMPTY + 8 * s, a.diag ? 9 : 1);  // the softmax warps read the bias of the stage
       ptx::mbar_init(V_EMPTY + 8 * s, 1);
+    }
+    for (int s = 0; s < 2; ++s) {
       ptx::mbar_init(S_FULL + 8 * s, 1);
-      ptx::mbar_init(P_FULL + 8 * s, 4);
+      ptx::mbar_init(P_FULL + 16 * s, 4);
+      ptx::mbar_init(P_FULL + 16 * s + 8, 4);
       ptx::mbar_init(O_DONE + 8 * s, 1);
+      ptx::mbar_init(S_FREE + 8 * s, 4);
     }
     ptx::mbar_init(DRAIN, 1);
     ptx::fence_mbar_init();
@@ -131,98 +146,117 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *slot;
-  const uint32_t tS = tmem, tO = tmem + 256;  // S0 S1 (128 columns each), O0 O1 (64 NS each)
+  // S0 S1 (128 columns each), O0 O1 (64 NS each), P0 P1 (64 each; over S where there is no room)
+  const uint32_t tS = tmem, tO = tmem + 256, tP = APART ? tmem + 384 : tS;
+  constexpr uint32_t P_LD = APART ? 64 : 128;
 
-  if (warp == 8) {
-    if (lane == 0 && tiles > 0) {
-      ptx::mbar_expect_tx(Q_FULL, 2 * NS * kSlab);
-      for (int w = 0; w < 2; ++w)
-        for (int s = 0; s < NS; ++s)
-          ptx::tma_load_4d(sQ + (w * NS + s) * kSlab, &maps.q, 64 * s, h, q0 + 128 * w, b, Q_FULL);
-      bool ok = true;
-      int nk = 0, nv = 0;  // tiles asked for
-      for (int t = 0; t < tiles && ok; ++t) {
-        const int st = t & 1;
-        const uint32_t ph = ((t >> 1) & 1) ^ 1;
-        if (!ptx::mbar_wait(K_EMPTY + 8 * st, ph, kWaitNs)) {
-          ok = false;
-          break;
+  // 3 x 168 registers a thread at the launch: 216 + 216 + 72 (the issuer must not spill)
+  if (warp >= 8) {
+    regs_down<72>();
+    if (warp == 8) {
+      if (lane == 0 && tiles > 0) {
+        ptx::mbar_expect_tx(Q_FULL, 2 * NS * kSlab);
+        for (int w = 0; w < 2; ++w)
+          for (int s = 0; s < NS; ++s)
+            ptx::tma_load_4d(sQ + (w * NS + s) * kSlab, &maps.q, 64 * s, h, q0 + 128 * w, b, Q_FULL);
+        bool ok = true;
+        int nk = 0, nv = 0;  // tiles asked for
+        for (int t = 0; t < tiles && ok; ++t) {
+          const int st = t % R;
+          const uint32_t ph = ((t / R) & 1) ^ 1;
+          if (!bar_wait(K_EMPTY + 8 * st, ph)) {
+            ok = false;
+            break;
+          }
+          ptx::mbar_expect_tx(K_FULL + 8 * st, NS * kSlab + (a.diag ? 384 * 4 : 0));
+          for (int s = 0; s < NS; ++s)
+            ptx::tma_load_4d(sK + (st * NS + s) * kSlab, &maps.k, 64 * s, kh, t * 128, b, K_FULL + 8 * st);
+          nk = t + 1;
+          if (a.diag)
+            ptx::bulk_g2s(base + oB + st * 384 * 4, a.diag + h * a.diag_ld + (t * 128 - q0 - 256 + a.diag0), 384 * 4,
+                          K_FULL + 8 * st);
+          if (!bar_wait(V_EMPTY + 8 * st, ph)) {
+            ok = false;
+            break;
+          }
+          ptx::mbar_expect_tx(V_FULL + 8 * st, NS * kSlab);
+          for (int s = 0; s < NS; ++s)
+            ptx::tma_load_4d(sV + (st * NS + s) * kSlab, &maps.v, 64 * s, kh, t * 128, b, V_FULL + 8 * st);
+          nv = t + 1;
         }
-        ptx::mbar_expect_tx(K_FULL + 8 * st, NS * kSlab + (a.diag ? 384 * 4 : 0));
-        for (int s = 0; s < NS; ++s)
-          ptx::tma_load_4d(sK + (st * NS + s) * kSlab, &maps.k, 64 * s, kh, t * 128, b, K_FULL + 8 * st);
-        nk = t + 1;
-        if (a.diag)
-          ptx::bulk_g2s(base + oB + st * 384 * 4, a.diag + h * a.diag_ld + (t * 128 - q0 - 256 + a.diag0), 384 * 4,
-                        K_FULL + 8 * st);
-        if (!ptx::mbar_wait(V_EMPTY + 8 * st, ph, kWaitNs)) {
-          ok = false;
-          break;
-        }
-        ptx::mbar_expect_tx(V_FULL + 8 * st, NS * kSlab);
-        for (int s = 0; s < NS; ++s)
-          ptx::tma_load_4d(sV + (st * NS + s) * kSlab, &maps.v, 64 * s, kh, t * 128, b, V_FULL + 8 * st);
-        nv = t + 1;
+        if (!ok) atomicExch(a.err, 41);
+        // no copy left in flight when the block ends
+        bar_wait(Q_FULL, 0);
+        for (int x = max(0, nk - R); x < nk; ++x) bar_wait(K_FULL + 8 * (x % R), (x / R) & 1);
+        for (int x = max(0, nv - R); x < nv; ++x) bar_wait(V_FULL + 8 * (x % R), (x / R) & 1);
       }
-      if (!ok) atomicExch(a.err, 41);
-      // no copy left in flight when the block ends
-      ptx::mbar_wait(Q_FULL, 0, kWaitNs);
-      for (int x = max(0, nk - 2); x < nk; ++x) ptx::mbar_wait(K_FULL + 8 * (x & 1), (x >> 1) & 1, kWaitNs);
-      for (int x = max(0, nv - 2); x < nv; ++x) ptx::mbar_wait(V_FULL + 8 * (x & 1), (x >> 1) & 1, kWaitNs);
-    }
-    __syncwarp();
-  } else if (warp == 9) {
-    if (lane == 0 && tiles > 0) {
-      const uint32_t id_s = idesc<T>(128, false, false);
-      const int DK = (a.D + 15) / 16;
-      const uint32_t id_o = idesc<T>(16 * DK, false, true);
-      bool ok = ptx::mbar_wait(Q_FULL, 0, kWaitNs);
-      auto issue_s = [&](int w, int t) {
-        const int st = t & 1;
-        if (ok) ok = ptx::mbar_wait(K_FULL + 8 * st, (t >> 1) & 1, kWaitNs);
-        if (!ok) return;
-        ptx::tc_fence_after();
-        const uint64_t dq = desc_k(sQ + w * NS * kSlab), dk = desc_k(sK + st * NS * kSlab);
+      __syncwarp();
+    } else if (warp == 9) {
+      if (lane == 0 && tiles > 0) {
+        const uint32_t id_s = idesc<T>(128, false, false);
+        const int DK = FULL ? 4 * NS : (a.D + 15) / 16;
+        const uint32_t id_o = idesc<T>(16 * DK, false, true);
+        bool ok = bar_wait(Q_FULL, 0);
+        auto issue_s = [&](int w, int t) {
+          const int st = t % R;
+          if (ok) ok = bar_wait(K_FULL + 8 * st, (t / R) & 1);
+          if (!ok) return;
+          ptx::tc_fence_after();
+          const uint64_t dq = desc_k(sQ + w * NS * kSlab), dk = desc_k(sK + st * NS * kSlab);
 #pragma unroll
-        for (int kk = 0; kk < 4 * NS; ++kk) {
-          if (kk >= DK) break;
-          const uint64_t off = (uint64_t)(((kk >> 2) * kSlab + (kk & 3) * 32) >> 4);
-          mma_ss(tS + 128 * w, dq + off, dk + off, id_s, kk > 0);
+          for (int kk = 0; kk < 4 * NS; ++kk) {
+            if (kk >= DK) break;
+            const uint64_t off = (uint64_t)(((kk >> 2) * kSlab + (kk & 3) * 32) >> 4);
+            mma_ss(tS + 128 * w, dq + off, dk + off, id_s, kk > 0);
+          }
+          ptx::mma_commit(S_FULL + 8 * w);
+          if (w == 1) ptx::mma_commit(K_EMPTY + 8 * st);
+        };
+        auto issue_o = [&](int w, int t) {
+          const int st = t % R;
+          if (ok) ok = bar_wait(V_FULL + 8 * st, (t / R) & 1);
+          const uint64_t dv = desc_mn(sV + st * NS * kSlab);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (ok) ok = bar_wait(P_FULL + 16 * w + 8 * x, t & 1);
+            if (!ok) return;
+            ptx::tc_fence_after();
+#pragma unroll
+            for (int kk = 4 * x; kk < 4 * x + 4; ++kk)
+              mma_ts(tO + 64 * NS * w, tP + P_LD * w + 8 * kk, dv + (uint64_t)(kk * 2048 >> 4), id_o, t > 0 || kk > 0);
+          }
+          ptx::mma_commit(O_DONE + 8 * w);
+          if (w == 1) ptx::mma_commit(V_EMPTY + 8 * st);
+        };
+        issue_s(0, 0);
+        issue_s(1, 0);
+        for (int t = 0; t < tiles && ok; ++t) {
+          if (APART) {
+            for (int w = 0; w < 2 && t + 1 < tiles; ++w) {
+              if (ok) ok = bar_wait(S_FREE + 8 * w, t & 1);
+              issue_s(w, t + 1);
+            }
+            issue_o(0, t);
+            issue_o(1, t);
+          } else {
+            issue_o(0, t);
+            if (t + 1 < tiles) issue_s(0, t + 1);
+            issue_o(1, t);
+            if (t + 1 < tiles) issue_s(1, t + 1);
+          }
         }
-        ptx::mma_commit(S_FULL + 8 * w);
-        if (w == 1) ptx::mma_commit(K_EMPTY + 8 * st);
-      };
-      auto issue_o = [&](int w, int t) {
-        const int st = t & 1;
-        if (ok) ok = ptx::mbar_wait(V_FULL + 8 * st, (t >> 1) & 1, kWaitNs);
-        if (ok) ok = ptx::mbar_wait(P_FULL + 8 * w, t & 1, kWaitNs);
-        if (!ok) return;
-        ptx::tc_fence_after();
-        const uint64_t dv = desc_mn(sV + st * NS * kSlab);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          mma_ts(tO + 64 * NS * w, tS + 128 * w + 8 * kk, dv + (uint64_t)(kk * 2048 >> 4), id_o, t > 0 || kk > 0);
-        ptx::mma_commit(O_DONE + 8 * w);
-        if (w == 1) ptx::mma_commit(V_EMPTY + 8 * st);
-      };
-      issue_s(0, 0);
-      issue_s(1, 0);
-      for (int t = 0; t < tiles && ok; ++t) {
-        issue_o(0, t);
-        if (t + 1 < tiles) issue_s(0, t + 1);
-        issue_o(1, t);
-        if (t + 1 < tiles) issue_s(1, t + 1);
+        if (!ok) atomicExch(a.err, 42);
+        ptx::mma_commit(DRAIN);
+        bar_wait(DRAIN, 0);  // every product done before tensor memory is freed
       }
-      if (!ok) atomicExch(a.err, 42);
-      ptx::mma_commit(DRAIN);
-      ptx::mbar_wait(DRAIN, 0, kWaitNs);  // every product done before tensor memory is freed
+      __syncwarp();
     }
-    __syncwarp();
   } else {
+    regs_up<216>();
     const int w = warp >> 2;  // query tile
     const int row = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_col = tS + 128 * w + lanes, o_col = tO + 64 * NS * w + lanes;
+    const uint32_t s_col = tS + 128 * w + lanes, p_col = tP + P_LD * w + lanes, o_col = tO + 64 * NS * w + lanes;
     const long long i = (long long)q0 + 128 * w + row;
     const float sc = a.scale * kLog2e;
     // keys that this row may meet: [0, lim)
@@ -234,7 +268,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int t = 0; t < tiles && ok; ++t) {
-      const int st = t & 1, j0 = t * 128;
+      const int st = t % R, j0 = t * 128;
       uint32_t alive[4] = {~0u, ~0u, ~0u, ~0u};
       if (mb) {
 #pragma unroll
@@ -244,13 +278,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         }
       }
       if (mb || j0 + 128 > len) {  // zero the dead rows of V (both query tiles do, with the same result)
-        const bool dead = j0 + row >= len || !((alive[row >> 5] >> (row & 31)) & 1);
-        if (!warp_wait(V_FULL + 8 * st, (t >> 1) & 1)) {
+        const uint32_t word = (warp & 3) == 0 ? alive[0] : (warp & 3) == 1 ? alive[1] : (warp & 3) == 2 ? alive[2] : alive[3];
+        const bool dead = j0 + row >= len || !((word >> lane) & 1);
+        if (!warp_wait(V_FULL + 8 * st, (t / R) & 1)) {
           ok = false;
           break;
         }
         if (dead) {
-          uint4* z = reinterpret_cast<uint4*>(gen + 4 * NS * kSlab + st * NS * kSlab + row * 128);
+          uint4* z = reinterpret_cast<uint4*>(gen + (2 + R + st) * NS * kSlab + row * 128);
 #pragma unroll
           for (int s = 0; s < NS; ++s)
 #pragma unroll
@@ -258,7 +293,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         }
         ptx::fence_proxy_async_smem();
       }
-      if (a.diag && !warp_wait(K_FULL + 8 * st, (t >> 1) & 1)) {
+      // relative positions of this query tile and the key tile: [hi - 254, hi].  Where
+      // they lie whole in the last bucket the bias is one value.
+      const long long hi = (long long)j0 + 127 - (q0 + 128 * w) - a.q_off;
+      const bool flat = !a.diag || hi <= -(long long)a.far || hi - 254 >= (a.far_both ? (long long)a.far : 0ll);
+      if (a.diag && !warp_wait(K_FULL + 8 * st, (t / R) & 1)) {
         ok = false;
         break;
       }
@@ -272,22 +311,35 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       for (int x = 0; x < 4; ++x) ptx::tmem_ld32_async(s_col + 32 * x, s[x]);
 #pragma unroll
       for (int x = 0; x < 4; ++x) ptx::tmem_wait_ld(s[x]);
-      float mx = -INFINITY;
+      if (APART) {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(S_FREE + 8 * w);
+      }
+      // exponents are s x + c - m; without a bias by pair the products stay as they are
+      float mul = 1.f, add = 0.f;
+      const bool plain = flat && sc > 0.f;
       if (a.diag) {
         const float* bb = bias_s + st * 384 + 256 - 128 * w - row;
+        if (plain) {
+          add = bb[0];
+        } else {
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+          for (int x = 0; x < 4; ++x)
 #pragma unroll
-          for (int c = 0; c < 32; ++c) s[x][c] = __float_as_uint(fmaf(__uint_as_float(s[x][c]), sc, bb[32 * x + c]));
+            for (int c = 0; c < 32; ++c) s[x][c] = __float_as_uint(fmaf(__uint_as_float(s[x][c]), sc, bb[32 * x + c]));
+        }
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(K_EMPTY + 8 * st);
-      } else {
+      } else if (!plain) {
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
           for (int c = 0; c < 32; ++c) s[x][c] = __float_as_uint(__uint_as_float(s[x][c]) * sc);
       }
-      if (mb || j0 + 128 > wlim) {
+      if (plain) mul = sc;
+      const bool cut = mb || j0 + 128 > wlim;
+      if (cut) {
         const int n = (int)max(0ll, min(128ll, lim - j0));
 #pragma unroll
         for (int x = 0; x < 4; ++x)
@@ -295,10 +347,15 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           for (int c = 0; c < 32; ++c)
             if (32 * x + c >= n || !((alive[x] >> c) & 1)) s[x][c] = 0xff800000u;
       }
+      float mx = -INFINITY, my = -INFINITY;
 #pragma unroll
       for (int x = 0; x < 4; ++x)
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) mx = fmaxf(fmaxf(mx, __uint_as_float(s[x][c])), __uint_as_float(s[x][c + 1]));
+        for (int c = 0; c < 32; c += 4) {
+          mx = fmaxf(fmaxf(mx, __uint_as_float(s[x][c])), __uint_as_float(s[x][c + 1]));
+          my = fmaxf(fmaxf(my, __uint_as_float(s[x][c + 2])), __uint_as_float(s[x][c + 3]));
+        }
+      mx = fmaf(fmaxf(mx, my), mul, add);
       const bool up = mx > m + kGrow;  // always on a row's first live key
       if (__any_sync(0xffffffffu, up)) {
         const float m_new = up ? mx : m;
@@ -322,26 +379,40 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         if (up) l *= f;
         m = m_new;
       }
-      const float mb2 = m == -INFINITY ? 0.f : m;
-      float l0 = 0.f, l1 = 0.f;
+      if (APART && t > 0) {  // the last P has been read
+        ok = warp_wait(O_DONE + 8 * w, (t - 1) & 1);
+        if (!ok) break;
+        ptx::tc_fence_after();
+      }
+      const float off = m == -INFINITY ? 0.f : add - m;
+      const uint64_t mul2 = f32x2(mul, mul), off2 = f32x2(off, off);
+      uint64_t l2 = f32x2(0.f, 0.f), l3 = l2;
+      // in two halves of 64 keys, so that the product of the first starts early
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         uint32_t p[32];
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
-          const float e0 = exp2_approx(__uint_as_float(s[2 * x + (c >> 4)][(2 * c) & 31]) - mb2);
-          const float e1 = exp2_approx(__uint_as_float(s[2 * x + (c >> 4)][(2 * c + 1) & 31]) - mb2);
-          l0 += e0;
-          l1 += e1;
+          const uint32_t(&v)[32] = s[2 * x + (c >> 4)];
+          const uint64_t y =
+              fma2(f32x2(__uint_as_float(v[(2 * c) & 31]), __uint_as_float(v[(2 * c + 1) & 31])), mul2, off2);
+          float e0, e1;
+          split2(y, e0, e1);
+          e0 = exp2_approx(e0);
+          e1 = exp2_approx(e1);
+          if (c & 1) l2 = add2(l2, f32x2(e0, e1));
+          else l3 = add2(l3, f32x2(e0, e1));
           p[c] = pack2<T>(e0, e1);
         }
-        tmem_st32(s_col + 32 * x, p);
+        tmem_st32(p_col + 32 * x, p);
+        tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(P_FULL + 16 * w + 8 * x);
       }
-      l += l0 + l1;
-      tmem_wait_st();
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(P_FULL + 8 * w);
+      float la, lb;
+      split2(add2(l2, l3), la, lb);
+      l += la + lb;
     }
     if (ok && tiles > 0) {
       ok = warp_wait(O_DONE + 8 * w, (tiles - 1) & 1);
@@ -380,7 +451,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   if (warp == 9) ptx::tmem_dealloc(tmem, 512);
 }
 
-template <typename T, int NS>
+template <typename T, int NS, bool FULL>
 void fwd(const AttnArgs& a, cudaStream_t st) {
   FwdMaps maps;
   make_map(&maps.q, a.type, a.q, a.qs, a.B, a.Lq, a.Hq, a.D, 128);
@@ -390,14 +461,22 @@ void fwd(const AttnArgs& a, cudaStream_t st) {
   int dev = 0;
   RVC_CUDA_TRY(cudaGetDevice(&dev));
   if (dev >= 64 || !(done.load() & (1ull << dev))) {
-    RVC_CUDA_TRY(cudaFuncSetAttribute(attn_tc_fwd_kernel<T, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    RVC_CUDA_TRY(cudaFuncSetAttribute(attn_tc_fwd_kernel<T, NS, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)fwd_smem<NS>()));
     if (dev < 64) done.fetch_or(1ull << dev);
   }
   const unsigned grid = (unsigned)((a.Lq + 255ll) / 256 * a.B * a.Hq);
-  attn_tc_fwd_kernel<T, NS><<<grid, kFwdThreads, fwd_smem<NS>(), st>>>(a, maps);
+  attn_tc_fwd_kernel<T, NS, FULL><<<grid, kFwdThreads, fwd_smem<NS>(), st>>>(a, maps);
   note_launch();
   RVC_CUDA_TRY(cudaGetLastError());
+}
+
+template <typename T>
+void fwd_t(const AttnArgs& a, cudaStream_t st) {
+  if (a.D == 64) fwd<T, 1, true>(a, st);
+  else if (a.D < 64) fwd<T, 1, false>(a, st);
+  else if (a.D == 128) fwd<T, 2, true>(a, st);
+  else fwd<T, 2, false>(a, st);
 }
 
 }  // namespace
@@ -411,13 +490,8 @@ bool attn_tc_fits(const AttnArgs& a) {
 }
 
 void attn_tc_forward(const AttnArgs& a, cudaStream_t st) {
-  if (a.type == kBf16) {
-    if (a.D <= 64) fwd<__nv_bfloat16, 1>(a, st);
-    else fwd<__nv_bfloat16, 2>(a, st);
-  } else {
-    if (a.D <= 64) fwd<__half, 1>(a, st);
-    else fwd<__half, 2>(a, st);
-  }
+  if (a.type == kBf16) fwd_t<__nv_bfloat16>(a, st);
+  else fwd_t<__half>(a, st);
 }
 
 }  // namespace rvc

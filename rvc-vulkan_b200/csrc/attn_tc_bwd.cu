@@ -44,29 +44,34 @@ struct BwdMaps {
   CUtensorMap x1, x2, y1, y2;
 };
 
-// X1 X2 [NS], Y1 Y2 [2 stages][NS] slabs; per stage bias [256], lse [128],
+// Tiles that pass by under way: as in the forward pass.
+template <int NS> constexpr int kRing = NS == 1 ? 4 : 2;
+
+// X1 X2 [NS], Y1 Y2 [stages][NS] slabs; per stage bias [256], lse [128],
 // delta [128]; diagonals [8][96], carry [128]; row exchange [2][128]; barriers
 template <int NS> constexpr uint32_t bwd_smem() {
-  return 6 * NS * kSlab + 2 * 512 * 4 + 8 * kDiagLd * 4 + 128 * 4 + 256 * 4 + 256 + 1024;
+  return (2 + 2 * kRing<NS>) * NS * kSlab + kRing<NS> * 512 * 4 + 8 * kDiagLd * 4 + 128 * 4 + 256 * 4 + 256 + 1024;
 }
 
 template <typename T, int NS, bool KV>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attn_tc_bwd_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ BwdMaps maps) {
+  constexpr int R = kRing<NS>;
   extern __shared__ uint8_t raw[];
   const uint32_t base = (ptx::smem_u32(raw) + 1023) & ~1023u;
   uint8_t* gen = raw + (base - ptx::smem_u32(raw));
-  const uint32_t sX1 = base, sX2 = sX1 + NS * kSlab, sY1 = sX2 + NS * kSlab, sY2 = sY1 + 2 * NS * kSlab;
-  const uint32_t oE = 6 * NS * kSlab;  // extras of the stages
+  const uint32_t sX1 = base, sX2 = sX1 + NS * kSlab, sY1 = sX2 + NS * kSlab, sY2 = sY1 + R * NS * kSlab;
+  const uint32_t oE = (2 + 2 * R) * NS * kSlab;  // extras of the stages
   float* ext = reinterpret_cast<float*>(gen + oE);
-  float* diag_s = ext + 2 * 512;
+  float* diag_s = ext + R * 512;
   float* carry = diag_s + 8 * kDiagLd;
   float* red = carry + 128;
-  const uint32_t oBar = oE + (2 * 512 + 8 * kDiagLd + 128 + 256) * 4;
+  const uint32_t oBar = oE + (R * 512 + 8 * kDiagLd + 128 + 256) * 4;
   const uint32_t bar = base + oBar;
-  const uint32_t X_FULL = bar, Y1_FULL = bar + 8, Y2_FULL = bar + 24, Y1_EMPTY = bar + 40, Y2_EMPTY = bar + 56,
-                 S_FULL = bar + 72, DP_FULL = bar + 80, P_READY = bar + 88, DS_READY = bar + 96, DONE = bar + 104;
-  uint32_t* slot = reinterpret_cast<uint32_t*>(gen + oBar + 112);
+  const uint32_t X_FULL = bar, Y1_FULL = bar + 8, Y2_FULL = Y1_FULL + 8 * R, Y1_EMPTY = Y2_FULL + 8 * R,
+                 Y2_EMPTY = Y1_EMPTY + 8 * R, S_FULL = Y2_EMPTY + 8 * R, DP_FULL = S_FULL + 8, P_READY = S_FULL + 16,
+                 DS_READY = S_FULL + 24, DONE = S_FULL + 32;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(gen + oBar + 192);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   const int G = a.Hq / a.Hkv;
@@ -94,7 +99,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
   if (threadIdx.x == 0) {
     ptx::mbar_init(X_FULL, 1);
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < R; ++s) {
       ptx::mbar_init(Y1_FULL + 8 * s, 1);
       ptx::mbar_init(Y2_FULL + 8 * s, 1);
       ptx::mbar_init(Y1_EMPTY + 8 * s, extras ? 9 : 1);
@@ -128,11 +133,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       int n1 = 0, n2 = 0;  // tiles asked for
       bool ok = true;
       for (int t = 0; t < tiles; ++t) {
-        const int st = t & 1;
-        const uint32_t ph = ((t >> 1) & 1) ^ 1;
+        const int st = t % R;
+        const uint32_t ph = ((t / R) & 1) ^ 1;
         const int hy = KV ? kh * G + t / per : kh;
         const int y0 = KV ? (first + t % per) * 128 : t * 128;
-        ok = ptx::mbar_wait(Y1_EMPTY + 8 * st, ph, kWaitNs);
+        ok = bar_wait(Y1_EMPTY + 8 * st, ph);
         if (!ok) break;
         ptx::mbar_expect_tx(Y1_FULL + 8 * st, NS * kSlab + (a.diag ? 1024 : 0) + (KV ? 1024 : 0));
         for (int s = 0; s < NS; ++s)
@@ -149,7 +154,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           ptx::bulk_g2s(e + 1536, a.delta + r, 512, Y1_FULL + 8 * st);
         }
         n1 = t + 1;
-        ok = ptx::mbar_wait(Y2_EMPTY + 8 * st, ph, kWaitNs);
+        ok = bar_wait(Y2_EMPTY + 8 * st, ph);
         if (!ok) break;
         ptx::mbar_expect_tx(Y2_FULL + 8 * st, NS * kSlab);
         for (int s = 0; s < NS; ++s)
@@ -157,16 +162,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         n2 = t + 1;
       }
       if (!ok) atomicExch(a.err, 51);
-      ptx::mbar_wait(X_FULL, 0, kWaitNs);  // no copy left in flight when the block ends
-      for (int x = max(0, n1 - 2); x < n1; ++x) ptx::mbar_wait(Y1_FULL + 8 * (x & 1), (x >> 1) & 1, kWaitNs);
-      for (int x = max(0, n2 - 2); x < n2; ++x) ptx::mbar_wait(Y2_FULL + 8 * (x & 1), (x >> 1) & 1, kWaitNs);
+      bar_wait(X_FULL, 0);  // no copy left in flight when the block ends
+      for (int x = max(0, n1 - R); x < n1; ++x) bar_wait(Y1_FULL + 8 * (x % R), (x / R) & 1);
+      for (int x = max(0, n2 - R); x < n2; ++x) bar_wait(Y2_FULL + 8 * (x % R), (x / R) & 1);
     }
     __syncwarp();
   } else if (warp == 9) {
     if (lane == 0 && tiles > 0) {
       const int DK = (a.D + 15) / 16;
       const uint32_t id_s = idesc<T>(128, false, false), id_a = idesc<T>(16 * DK, false, true);
-      bool ok = ptx::mbar_wait(X_FULL, 0, kWaitNs);
+      bool ok = bar_wait(X_FULL, 0);
       auto abt = [&](uint32_t d, uint32_t x, uint32_t y) {
         const uint64_t dx = desc_k(x), dy = desc_k(y);
 #pragma unroll
@@ -183,16 +188,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           mma_ts(d, p + 64 * (kk >> 2) + 8 * (kk & 3), dy + (uint64_t)(kk * 2048 >> 4), id_a, acc || kk > 0);
       };
       auto issue_s = [&](int t) {
-        const int st = t & 1;
-        if (ok) ok = ptx::mbar_wait(Y1_FULL + 8 * st, (t >> 1) & 1, kWaitNs);
+        const int st = t % R;
+        if (ok) ok = bar_wait(Y1_FULL + 8 * st, (t / R) & 1);
         if (!ok) return;
         ptx::tc_fence_after();
         abt(tS, sX1, sY1 + st * NS * kSlab);
         ptx::mma_commit(S_FULL);
       };
       auto issue_dp = [&](int t) {
-        const int st = t & 1;
-        if (ok) ok = ptx::mbar_wait(Y2_FULL + 8 * st, (t >> 1) & 1, kWaitNs);
+        const int st = t % R;
+        if (ok) ok = bar_wait(Y2_FULL + 8 * st, (t / R) & 1);
         if (!ok) return;
         ptx::tc_fence_after();
         abt(tD, sX2, sY2 + st * NS * kSlab);
@@ -202,14 +207,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       issue_s(0);
       issue_dp(0);
       for (int t = 0; t < tiles && ok; ++t) {
-        const int st = t & 1;
-        if (ok) ok = ptx::mbar_wait(P_READY, t & 1, kWaitNs);
+        const int st = t % R;
+        if (ok) ok = bar_wait(P_READY, t & 1);
         if (!ok) break;
         ptx::tc_fence_after();
         pb(tA2, tS, (KV ? sY2 : sY1) + st * NS * kSlab, t > 0);
         if (KV) ptx::mma_commit(Y2_EMPTY + 8 * st);
         if (t + 1 < tiles) issue_s(t + 1);
-        if (ok) ok = ptx::mbar_wait(DS_READY, t & 1, kWaitNs);
+        if (ok) ok = bar_wait(DS_READY, t & 1);
         if (!ok) break;
         ptx::tc_fence_after();
         pb(tA1, tD, sY1 + st * NS * kSlab, t > 0);
@@ -218,7 +223,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       if (!ok) atomicExch(a.err, 52);
       ptx::mma_commit(DONE);
-      ptx::mbar_wait(DONE, 0, kWaitNs);  // every product done before tensor memory is freed
+      bar_wait(DONE, 0);  // every product done before tensor memory is freed
     }
     __syncwarp();
   } else {
@@ -256,7 +261,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     float far_behind = 0.f, far_ahead = 0.f;
     for (int t = 0; t < tiles; ++t) {
-      const int st = t & 1;
+      const int st = t % R;
       const int y0 = KV ? (first + t % per) * 128 : t * 128;
       const float* e = ext + st * 512;
       uint32_t alive[2] = {~0u, ~0u};  // first: keys of this half
@@ -269,7 +274,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       float p[64];
       do {  // a wait that gives up leaves the tile; the warps meet again below
-        if (extras && !(ok = warp_wait(Y1_FULL + 8 * st, (t >> 1) & 1))) break;
+        if (extras && !(ok = warp_wait(Y1_FULL + 8 * st, (t / R) & 1))) break;
         if (!(ok = warp_wait(S_FULL, t & 1))) break;
         ptx::tc_fence_after();
 #pragma unroll
