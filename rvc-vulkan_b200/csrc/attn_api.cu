@@ -23,8 +23,8 @@ __global__ void expand_bias_kernel(const T* __restrict__ table, int H, long long
 
 // sums[h][x] = sum over batch entries and tiles of the diagonal j - i = x - (Lq - 1).
 // Tiles of BM queries (by_key = 0) hold it at x - (Lq - 1) + BM - 1 + t BM, tiles
-// of BM keys at (Lq - 1) - x + BM - 1 + t BM; there the last two entries of a
-// tile are sums that lie whole in the last bucket behind / ahead.
+// of BM keys (by_key arrays each) at (Lq - 1) - x + BM - 1 + t BM; there the last
+// two entries of an array are sums that lie whole in the last bucket behind / ahead.
 // Block: 32 diagonals x 8 shares of the (tile, batch) list, joined in order.
 __global__ void __launch_bounds__(256) diag_sums_kernel(const float* __restrict__ ws, int B, int H, int nt, int BM,
                                                         int by_key, long long ld, long long Lq, long long Lk,
@@ -35,13 +35,14 @@ __global__ void __launch_bounds__(256) diag_sums_kernel(const float* __restrict_
   const int h = blockIdx.y;
   const long long n = Lq + Lk - 1;
   const long long d = x - (Lq - 1), top = by_key ? ld - 2 : ld;
+  const int na = by_key ? by_key : 1;
   double s = 0.0;
   if (x < n || (x < n + 2 && by_key))
 #pragma unroll 4
-    for (long long k = y; k < (long long)B * nt; k += 8) {
-      const long long t = k / B, b = k % B;
+    for (long long k = y; k < (long long)B * nt * na; k += 8) {
+      const long long u = k / B, b = k % B, t = u / na;
       const long long e = x < n ? (by_key ? -d : d) + BM - 1 + t * BM : top + (x - n);
-      if (e >= 0 && (e < top || x >= n)) s += ws[((b * H + h) * nt + t) * ld + e];
+      if (e >= 0 && (e < top || x >= n)) s += ws[((b * H + h) * nt * na + u) * ld + e];
     }
   red[y][lane] = s;
   __syncthreads();
@@ -130,7 +131,7 @@ Layout plan(const AttnArgs& a, bool bias, bool backward, int sms, bool tc) {
     const int64_t tiled = tc ? a.Lk : a.Lq, along = tc ? a.Lq : a.Lk;
     l.nt = (int)((tiled + l.BM - 1) / l.BM);
     l.dws_ld = up(along, l.BM) + l.BM + (tc ? 2 : 0);
-    l.dws = take(4 * l.dws_ld * l.nt * a.B * a.Hq);
+    l.dws = take(4 * l.dws_ld * l.nt * (tc ? attn_tc_bwd_arrays(a) : 1) * a.B * a.Hq);
     l.sums = take(8 * ((int64_t)a.Lq + a.Lk - 1) * a.Hq);
     l.far = take(16 * a.Hq);
   }
@@ -227,7 +228,7 @@ void attn_backward(AttnArgs a, const void* table, const BucketRule* rule, void* 
     double *sums = at<double>(ws, l.sums), *far = at<double>(ws, l.far);
     const int64_t n = (int64_t)a.Lq + a.Lk + 1;
     diag_sums_kernel<<<dim3((unsigned)((n + 31) / 32), a.Hq), 256, 0, st>>>(
-        a.dws, a.B, a.Hq, l.nt, l.BM, l.tc ? 1 : 0, l.dws_ld, a.Lq, a.Lk, sums, far);
+        a.dws, a.B, a.Hq, l.nt, l.BM, l.tc ? attn_tc_bwd_arrays(a) : 0, l.dws_ld, a.Lq, a.Lk, sums, far);
     note_launch();
     RVC_CUDA_TRY(cudaGetLastError());
     relbias_bucket_sums(a.type, a.Hq, a.Lq, a.Lk, a.q_off, sums, far, *rule, dtable, st);

@@ -70,8 +70,8 @@ struct AttnArgs {
   // backward
   const void *dout = nullptr, *fout = nullptr;
   int64_t dos[3] = {0, 0, 0}, os[3] = {0, 0, 0};
-  float* delta = nullptr;        // [B, Hq, row_ld] sum_j P dP of every query
-  float* lse2 = nullptr;         // [B, Hq, row_ld] log2 sums, +inf for a row without a key (attn_tc_bwd.cu)
+  float* delta = nullptr;        // [B, Hq, row_ld] sum_j P dP of every query (attn_tc_bwd.cu: its negative)
+  float* lse2 = nullptr;         // [B, Hq, row_ld] -log2 sums, -inf for a row without a key (attn_tc_bwd.cu)
   int64_t row_ld = 0;
   void *dq = nullptr, *dk = nullptr, *dv = nullptr;  // contiguous [B, L, H, D]
   float* dws = nullptr;          // diagonal sums of dS: [B][Hq][tiles][dws_ld], see attn_api.cu
@@ -137,6 +137,7 @@ int attn_mma_splits(const AttnArgs& a, int sms, bool* workspace);
 bool attn_tc_fits(const AttnArgs& a);
 void attn_tc_forward(const AttnArgs& a, cudaStream_t st);
 bool attn_tc_bwd_fits(const AttnArgs& a);
+int attn_tc_bwd_arrays(const AttnArgs& a);  // arrays of diagonal sums to a tile of keys
 void attn_tc_backward(const AttnArgs& a, cudaStream_t st);
 
 void relbias_forward(int type, int H, int64_t Lq, int64_t Lk, int64_t q_off, const void* table, const BucketRule& rule,

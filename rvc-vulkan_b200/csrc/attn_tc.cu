@@ -94,9 +94,6 @@ template <int NS> constexpr uint32_t fwd_smem() {
 template <typename T, int NS, bool FULL>
 __global__ void __launch_bounds__(kFwdThreads, 1)
     attn_tc_fwd_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ FwdMaps maps) {
-  // Heads of 64 leave columns of tensor memory for P beside S, so that the next
-  // product into S starts as soon as the softmax has read this one.
-  constexpr bool APART = false;
   constexpr int R = kRing<NS>;
   extern __shared__ uint8_t raw[];
   const uint32_t base = (ptx::smem_u32(raw) + 1023) & ~1023u;
@@ -107,7 +104,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   const uint32_t bar = base + oBar;
   const uint32_t Q_FULL = bar, K_FULL = bar + 8, V_FULL = K_FULL + 8 * R, K_EMPTY = V_FULL + 8 * R,
                  V_EMPTY = K_EMPTY + 8 * R, S_FULL = V_EMPTY + 8 * R, P_FULL = S_FULL + 16 /* [2 tiles][2 halves] */,
-                 O_DONE = P_FULL + 32, S_FREE = O_DONE + 16, DRAIN = S_FREE + 16;
+                 O_DONE = P_FULL + 32, DRAIN = O_DONE + 16;
   uint32_t* slot = reinterpret_cast<uint32_t*>(gen + oBar + 248);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -133,7 +130,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       ptx::mbar_init(P_FULL + 16 * s, 4);
       ptx::mbar_init(P_FULL + 16 * s + 8, 4);
       ptx::mbar_init(O_DONE + 8 * s, 1);
-      ptx::mbar_init(S_FREE + 8 * s, 4);
     }
     ptx::mbar_init(DRAIN, 1);
     ptx::fence_mbar_init();
@@ -146,9 +142,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *slot;
-  // S0 S1 (128 columns each), O0 O1 (64 NS each), P0 P1 (64 each; over S where there is no room)
-  const uint32_t tS = tmem, tO = tmem + 256, tP = APART ? tmem + 384 : tS;
-  constexpr uint32_t P_LD = APART ? 64 : 128;
+  // S0 S1 (128 columns each, P over them), O0 O1 (64 NS each)
+  const uint32_t tS = tmem, tO = tmem + 256;
 
   // 3 x 168 registers a thread at the launch: 216 + 216 + 72 (the issuer must not spill)
   if (warp >= 8) {
@@ -223,7 +218,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             ptx::tc_fence_after();
 #pragma unroll
             for (int kk = 4 * x; kk < 4 * x + 4; ++kk)
-              mma_ts(tO + 64 * NS * w, tP + P_LD * w + 8 * kk, dv + (uint64_t)(kk * 2048 >> 4), id_o, t > 0 || kk > 0);
+              mma_ts(tO + 64 * NS * w, tS + 128 * w + 8 * kk, dv + (uint64_t)(kk * 2048 >> 4), id_o, t > 0 || kk > 0);
           }
           ptx::mma_commit(O_DONE + 8 * w);
           if (w == 1) ptx::mma_commit(V_EMPTY + 8 * st);
@@ -231,19 +226,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         issue_s(0, 0);
         issue_s(1, 0);
         for (int t = 0; t < tiles && ok; ++t) {
-          if (APART) {
-            for (int w = 0; w < 2 && t + 1 < tiles; ++w) {
-              if (ok) ok = bar_wait(S_FREE + 8 * w, t & 1);
-              issue_s(w, t + 1);
-            }
-            issue_o(0, t);
-            issue_o(1, t);
-          } else {
-            issue_o(0, t);
-            if (t + 1 < tiles) issue_s(0, t + 1);
-            issue_o(1, t);
-            if (t + 1 < tiles) issue_s(1, t + 1);
-          }
+          issue_o(0, t);
+          if (t + 1 < tiles) issue_s(0, t + 1);
+          issue_o(1, t);
+          if (t + 1 < tiles) issue_s(1, t + 1);
         }
         if (!ok) atomicExch(a.err, 42);
         ptx::mma_commit(DRAIN);
@@ -256,7 +242,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     const int w = warp >> 2;  // query tile
     const int row = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_col = tS + 128 * w + lanes, p_col = tP + P_LD * w + lanes, o_col = tO + 64 * NS * w + lanes;
+    const uint32_t s_col = tS + 128 * w + lanes, o_col = tO + 64 * NS * w + lanes;
     const long long i = (long long)q0 + 128 * w + row;
     const float sc = a.scale * kLog2e;
     // keys that this row may meet: [0, lim)
@@ -267,15 +253,22 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     const uint8_t* mb = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
+    uint8_t bytes[4] = {0, 0, 0, 0};  // mask of keys `lane`, 32 + `lane`, ... of the next tile
+    auto fetch = [&](int j0) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int j = j0 + 32 * x + lane;
+        bytes[x] = j < len ? mb[(int64_t)j * a.mask_k] : 0;
+      }
+    };
+    if (mb) fetch(0);
     for (int t = 0; t < tiles && ok; ++t) {
       const int st = t % R, j0 = t * 128;
-      uint32_t alive[4] = {~0u, ~0u, ~0u, ~0u};
+      uint32_t alive[4] = {~0u, ~0u, ~0u, ~0u};  // the mask's bytes came with the last tile
       if (mb) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int j = j0 + 32 * x + lane;
-          alive[x] = __ballot_sync(0xffffffffu, j < len && mb[(int64_t)j * a.mask_k] != 0);
-        }
+        for (int x = 0; x < 4; ++x) alive[x] = __ballot_sync(0xffffffffu, bytes[x] != 0);
+        fetch(j0 + 128);
       }
       if (mb || j0 + 128 > len) {  // zero the dead rows of V (both query tiles do, with the same result)
         const uint32_t word = (warp & 3) == 0 ? alive[0] : (warp & 3) == 1 ? alive[1] : (warp & 3) == 2 ? alive[2] : alive[3];
@@ -311,11 +304,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       for (int x = 0; x < 4; ++x) ptx::tmem_ld32_async(s_col + 32 * x, s[x]);
 #pragma unroll
       for (int x = 0; x < 4; ++x) ptx::tmem_wait_ld(s[x]);
-      if (APART) {
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(S_FREE + 8 * w);
-      }
       // exponents are s x + c - m; without a bias by pair the products stay as they are
       float mul = 1.f, add = 0.f;
       const bool plain = flat && sc > 0.f;
@@ -342,10 +330,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       if (cut) {
         const int n = (int)max(0ll, min(128ll, lim - j0));
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < 4; ++x) {
+          alive[x] &= low_bits(n - 32 * x);
 #pragma unroll
           for (int c = 0; c < 32; ++c)
-            if (32 * x + c >= n || !((alive[x] >> c) & 1)) s[x][c] = 0xff800000u;
+            if (!(alive[x] & (1u << c))) s[x][c] = 0xff800000u;
+        }
       }
       float mx = -INFINITY, my = -INFINITY;
 #pragma unroll
@@ -379,11 +369,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         if (up) l *= f;
         m = m_new;
       }
-      if (APART && t > 0) {  // the last P has been read
-        ok = warp_wait(O_DONE + 8 * w, (t - 1) & 1);
-        if (!ok) break;
-        ptx::tc_fence_after();
-      }
       const float off = m == -INFINITY ? 0.f : add - m;
       const uint64_t mul2 = f32x2(mul, mul), off2 = f32x2(off, off);
       uint64_t l2 = f32x2(0.f, 0.f), l3 = l2;
@@ -404,7 +389,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           else l3 = add2(l3, f32x2(e0, e1));
           p[c] = pack2<T>(e0, e1);
         }
-        tmem_st32(p_col + 32 * x, p);
+        tmem_st32(s_col + 32 * x, p);
         tmem_wait_st();
         ptx::tc_fence_before();
         __syncwarp();

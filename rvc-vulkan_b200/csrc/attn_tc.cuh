@@ -24,9 +24,9 @@ __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
          ((uint64_t)2 << 61);
 }
 // Contraction along the rows (MN-major): eight rows are 1024 bytes, the next
-// 64 values lie one slab further; 16 rows further is 2048 bytes further.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(kSlab >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+// 64 values lie one slab (`slab` bytes) further; 16 rows further is 2048 bytes further.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t slab = kSlab) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(slab >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
@@ -72,6 +72,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// The lowest n bits (none for n <= 0, all from 32 on).
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+
 // Two fp32 operations to an instruction, each rounded on its own.
 __device__ __forceinline__ uint64_t f32x2(float a, float b) {
   uint64_t r;
@@ -84,6 +87,11 @@ __device__ __forceinline__ void split2(uint64_t p, float& a, float& b) {
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {

@@ -4,15 +4,21 @@
 //   first   dQ of 128 queries, keys passing by;
 //   second  dK, dV of 128 keys of one KV head, queries of its group passing by.
 // Both hold a resident pair X1, X2 and stream pairs Y1, Y2 (first: X = Q, dO and
-// Y = K, V; second: X = K, V and Y = Q, dO) and form, per tile of 128 x 128,
+// Y = K, V; second: X = K, V and Y = Q, dO) and form, per tile of 128 rows of X
+// and 64 of Y,
 //   S = X1 Y1^T, dP = X2 Y2^T           (fp32 in tensor memory)
-//   P = 2^(scale S + bias - lse), dS = P (dP - delta)   (eight warps)
+//   P = 2^(scale S + bias - lse), dS = P (dP - delta)
 //   first:  A1 += dS K, A2 += P K       second: A1 += dS^T Q, A2 += P^T dO
 // with P and dS read from tensor memory as 16-bit pairs over the columns of S
-// and dP.  The tensor pipe runs in the order S dP | A2 S' | A1 dP' ..., so the
-// products of the next tile run while the warps work on this one.  Seven
-// products instead of the five of a single kernel, against no atomics and no
-// fp32 copy of dQ in memory.
+// and dP, one row to a thread of a group of four warps.  The tensor pipe runs in
+// the order
+//   A2(t) S(t + GR) | A1(t - GR + 1) dP(t + 1)
+// where GR = 1 or 2 groups take the tiles in turn, each with its own S and dP.
+// Heads of up to 64 values have one group and half of the tensor memory, so that
+// two blocks share an SM: one's start and end (5 to 8 us, as long as four tiles)
+// and its exponentials go on beside the other's products.  Longer heads fill the
+// tensor memory and have two groups.  Seven products instead of the five of a
+// single kernel, against no atomics and no fp32 copy of dQ in memory.
 //
 // delta = sum_j P dP is wanted to more than the 16 bits that dO . out gives
 // (where the softmax is narrow, or summed over a wide bucket of the bias, dP -
@@ -37,46 +43,48 @@ namespace {
 
 using namespace atc;
 
-constexpr int kBwdThreads = 320;
-constexpr int kDiagLd = 96;  // diagonals of one warp's 32 x 64 part: 95
+template <int NS> constexpr int kGroups = NS == 1 ? 1 : 2;
+template <int NS> constexpr int kBwdThreads = 128 * kGroups<NS> + 64;
+constexpr int kDiagLd = 96;          // diagonals of one warp's 32 x 64 part: 95
+constexpr uint32_t kHalf = kSlab / 2;  // a slab of 64 rows
+constexpr int R = 4;                 // Y tiles under way
 
 struct BwdMaps {
   CUtensorMap x1, x2, y1, y2;
 };
 
-// Tiles that pass by under way: as in the forward pass.
-template <int NS> constexpr int kRing = NS == 1 ? 4 : 2;
-
-// X1 X2 [NS], Y1 Y2 [stages][NS] slabs; per stage bias [256], lse [128],
-// delta [128]; diagonals [8][96], carry [128]; row exchange [2][128]; barriers
+// X1 X2 [NS] slabs, Y1 Y2 [R][NS] slabs of 64 rows; per stage bias [192], -lse
+// [64], -delta [64]; diagonals [4 GR warps][96], open diagonals [128]; barriers
+constexpr uint32_t kExt = 320;
 template <int NS> constexpr uint32_t bwd_smem() {
-  return (2 + 2 * kRing<NS>) * NS * kSlab + kRing<NS> * 512 * 4 + 8 * kDiagLd * 4 + 128 * 4 + 256 * 4 + 256 + 1024;
+  return 2 * NS * kSlab + 2 * R * NS * kHalf + (R * kExt + 4 * kGroups<NS> * kDiagLd + 128) * 4 + 512 + 1024;
 }
 
-template <typename T, int NS, bool KV>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+template <typename T, int NS, bool KV, bool FULL>
+__global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
     attn_tc_bwd_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ BwdMaps maps) {
-  constexpr int R = kRing<NS>;
+  constexpr int GR = kGroups<NS>;
+  constexpr int kLoad = 4 * GR, kIssue = 4 * GR + 1;  // warps
+  constexpr int kStep = 64 * GR, kOpen = 192 - kStep;  // diagonals that a group's tile closes, and leaves open
   extern __shared__ uint8_t raw[];
   const uint32_t base = (ptx::smem_u32(raw) + 1023) & ~1023u;
   uint8_t* gen = raw + (base - ptx::smem_u32(raw));
-  const uint32_t sX1 = base, sX2 = sX1 + NS * kSlab, sY1 = sX2 + NS * kSlab, sY2 = sY1 + R * NS * kSlab;
-  const uint32_t oE = (2 + 2 * R) * NS * kSlab;  // extras of the stages
+  constexpr uint32_t oY1 = 2 * NS * kSlab, oY2 = oY1 + R * NS * kHalf, oE = oY2 + R * NS * kHalf;
+  constexpr uint32_t oBar = oE + (R * kExt + 4 * kGroups<NS> * kDiagLd + 128) * 4;
+  const uint32_t sX1 = base, sX2 = sX1 + NS * kSlab, sY1 = base + oY1, sY2 = base + oY2;
   float* ext = reinterpret_cast<float*>(gen + oE);
-  float* diag_s = ext + R * 512;
-  float* carry = diag_s + 8 * kDiagLd;
-  float* red = carry + 128;
-  const uint32_t oBar = oE + (R * 512 + 8 * kDiagLd + 128 + 256) * 4;
+  float* diag_s = ext + R * kExt;
+  float* carry = diag_s + 4 * GR * kDiagLd;
   const uint32_t bar = base + oBar;
   const uint32_t X_FULL = bar, Y1_FULL = bar + 8, Y2_FULL = Y1_FULL + 8 * R, Y1_EMPTY = Y2_FULL + 8 * R,
-                 Y2_EMPTY = Y1_EMPTY + 8 * R, S_FULL = Y2_EMPTY + 8 * R, DP_FULL = S_FULL + 8, P_READY = S_FULL + 16,
-                 DS_READY = S_FULL + 24, DONE = S_FULL + 32;
-  uint32_t* slot = reinterpret_cast<uint32_t*>(gen + oBar + 192);
+                 Y2_EMPTY = Y1_EMPTY + 8 * R, S_FULL = Y2_EMPTY + 8 * R /* [2 groups] each from here */,
+                 DP_FULL = S_FULL + 16, P_READY = S_FULL + 32, DS_READY = S_FULL + 48, DONE = S_FULL + 64;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(gen + oBar + 504);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   const int G = a.Hq / a.Hkv;
-  const int nq = (a.Lq + 127) / 128;
-  const int ntile = KV ? (a.Lk + 127) / 128 : nq;
+  const int ny = KV ? (a.Lq + 63) / 64 : 0;  // second: query tiles of a head
+  const int ntile = KV ? (a.Lk + 127) / 128 : (a.Lq + 127) / 128;
   const int heads = KV ? a.Hkv : a.Hq;
   // with a causal limit the longest walks come first: late queries, early keys
   const int xt = a.causal && !KV ? ntile - 1 - (int)(blockIdx.x % ntile) : (int)(blockIdx.x % ntile);
@@ -87,13 +95,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   // tiles that pass by: first: keys [0, kend); second: queries from `first` on, head by head
   int first = 0, per = 0, tiles = 0;
   if (KV) {
-    if (a.causal) first = (int)(max(0ll, min((long long)a.Lq, (long long)x0 - a.q_off)) / 128);
-    per = x0 < len ? max(0, nq - first) : 0;
+    if (a.causal) first = (int)(max(0ll, min((long long)a.Lq, (long long)x0 - a.q_off)) / 64);
+    per = x0 < len ? max(0, ny - first) : 0;
     tiles = per * G;
   } else {
     long long kend = len;
     if (a.causal) kend = max(0ll, min(kend, (long long)min(a.Lq, x0 + 128) + a.q_off));
-    tiles = (int)((kend + 127) / 128);
+    tiles = (int)((kend + 63) / 64);
   }
   const bool extras = KV || a.diag;
 
@@ -102,28 +110,31 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     for (int s = 0; s < R; ++s) {
       ptx::mbar_init(Y1_FULL + 8 * s, 1);
       ptx::mbar_init(Y2_FULL + 8 * s, 1);
-      ptx::mbar_init(Y1_EMPTY + 8 * s, extras ? 9 : 1);
+      ptx::mbar_init(Y1_EMPTY + 8 * s, extras ? 5 : 1);
       ptx::mbar_init(Y2_EMPTY + 8 * s, 1);
     }
-    ptx::mbar_init(S_FULL, 1);
-    ptx::mbar_init(DP_FULL, 1);
-    ptx::mbar_init(P_READY, 8);
-    ptx::mbar_init(DS_READY, 8);
+    for (int w = 0; w < GR; ++w) {
+      ptx::mbar_init(S_FULL + 8 * w, 1);
+      ptx::mbar_init(DP_FULL + 8 * w, 1);
+      ptx::mbar_init(P_READY + 8 * w, 4);
+      ptx::mbar_init(DS_READY + 8 * w, 4);
+    }
     ptx::mbar_init(DONE, 1);
     ptx::fence_mbar_init();
   }
-  if (warp == 9) {
-    ptx::tmem_alloc(ptx::smem_u32(slot), 512);
+  if (warp == kIssue) {
+    ptx::tmem_alloc(ptx::smem_u32(slot), 256 * GR);
     ptx::tmem_relinquish();
   }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *slot;
-  const uint32_t tS = tmem, tD = tmem + 128, tA1 = tmem + 256, tA2 = tA1 + 64 * NS;
-  const int Lp = nq * 128;  // padded rows of lse and delta
+  // S and dP of a group: 64 columns each at 128 w; A1, A2: 64 NS columns each
+  const uint32_t tS = tmem, tD = tmem + 64, tA1 = tmem + 128 * GR, tA2 = tA1 + 64 * NS;
+  const int Lp = (a.Lq + 127) / 128 * 128;  // padded rows of lse and delta
 
-  if (warp == 8) {
+  if (warp == kLoad) {
     if (lane == 0 && tiles > 0) {
       ptx::mbar_expect_tx(X_FULL, 2 * NS * kSlab);
       for (int s = 0; s < NS; ++s) {
@@ -136,29 +147,29 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const int st = t % R;
         const uint32_t ph = ((t / R) & 1) ^ 1;
         const int hy = KV ? kh * G + t / per : kh;
-        const int y0 = KV ? (first + t % per) * 128 : t * 128;
+        const int y0 = KV ? (first + t % per) * 64 : t * 64;
         ok = bar_wait(Y1_EMPTY + 8 * st, ph);
         if (!ok) break;
-        ptx::mbar_expect_tx(Y1_FULL + 8 * st, NS * kSlab + (a.diag ? 1024 : 0) + (KV ? 1024 : 0));
+        ptx::mbar_expect_tx(Y1_FULL + 8 * st, NS * kHalf + (a.diag ? 768 : 0) + (KV ? 512 : 0));
         for (int s = 0; s < NS; ++s)
-          ptx::tma_load_4d(sY1 + (st * NS + s) * kSlab, &maps.y1, 64 * s, hy, y0, b, Y1_FULL + 8 * st);
-        const uint32_t e = base + oE + st * 2048;
+          ptx::tma_load_4d(sY1 + (st * NS + s) * kHalf, &maps.y1, 64 * s, hy, y0, b, Y1_FULL + 8 * st);
+        const uint32_t e = base + oE + st * kExt * 4;
         if (a.diag) {
           const int h = KV ? hy : hx;
-          const int d = KV ? x0 - y0 - 128 : y0 - x0 - 128;
-          ptx::bulk_g2s(e, a.diag + h * a.diag_ld + (d + a.diag0), 1024, Y1_FULL + 8 * st);
+          const int d = KV ? x0 - y0 - 64 : y0 - x0 - 128;
+          ptx::bulk_g2s(e, a.diag + h * a.diag_ld + (d + a.diag0), 768, Y1_FULL + 8 * st);
         }
         if (KV) {
           const int64_t r = ((int64_t)b * a.Hq + hy) * Lp + y0;
-          ptx::bulk_g2s(e + 1024, a.lse2 + r, 512, Y1_FULL + 8 * st);
-          ptx::bulk_g2s(e + 1536, a.delta + r, 512, Y1_FULL + 8 * st);
+          ptx::bulk_g2s(e + 768, a.lse2 + r, 256, Y1_FULL + 8 * st);
+          ptx::bulk_g2s(e + 1024, a.delta + r, 256, Y1_FULL + 8 * st);
         }
         n1 = t + 1;
         ok = bar_wait(Y2_EMPTY + 8 * st, ph);
         if (!ok) break;
-        ptx::mbar_expect_tx(Y2_FULL + 8 * st, NS * kSlab);
+        ptx::mbar_expect_tx(Y2_FULL + 8 * st, NS * kHalf);
         for (int s = 0; s < NS; ++s)
-          ptx::tma_load_4d(sY2 + (st * NS + s) * kSlab, &maps.y2, 64 * s, hy, y0, b, Y2_FULL + 8 * st);
+          ptx::tma_load_4d(sY2 + (st * NS + s) * kHalf, &maps.y2, 64 * s, hy, y0, b, Y2_FULL + 8 * st);
         n2 = t + 1;
       }
       if (!ok) atomicExch(a.err, 51);
@@ -167,58 +178,63 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int x = max(0, n2 - R); x < n2; ++x) bar_wait(Y2_FULL + 8 * (x % R), (x / R) & 1);
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == kIssue) {
     if (lane == 0 && tiles > 0) {
-      const int DK = (a.D + 15) / 16;
-      const uint32_t id_s = idesc<T>(128, false, false), id_a = idesc<T>(16 * DK, false, true);
+      const int DK = FULL ? 4 * NS : (a.D + 15) / 16;
+      const uint32_t id_s = idesc<T>(64, false, false), id_a = idesc<T>(16 * DK, false, true);
       bool ok = bar_wait(X_FULL, 0);
       auto abt = [&](uint32_t d, uint32_t x, uint32_t y) {
         const uint64_t dx = desc_k(x), dy = desc_k(y);
 #pragma unroll
         for (int kk = 0; kk < 4 * NS; ++kk) {
           if (kk >= DK) break;
-          const uint64_t off = (uint64_t)(((kk >> 2) * kSlab + (kk & 3) * 32) >> 4);
-          mma_ss(d, dx + off, dy + off, id_s, kk > 0);
+          mma_ss(d, dx + (uint64_t)(((kk >> 2) * kSlab + (kk & 3) * 32) >> 4),
+                 dy + (uint64_t)(((kk >> 2) * kHalf + (kk & 3) * 32) >> 4), id_s, kk > 0);
         }
       };
       auto pb = [&](uint32_t d, uint32_t p, uint32_t y, bool acc) {
-        const uint64_t dy = desc_mn(y);
+        const uint64_t dy = desc_mn(y, kHalf);
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          mma_ts(d, p + 64 * (kk >> 2) + 8 * (kk & 3), dy + (uint64_t)(kk * 2048 >> 4), id_a, acc || kk > 0);
+        for (int kk = 0; kk < 4; ++kk) mma_ts(d, p + 8 * kk, dy + (uint64_t)(kk * 2048 >> 4), id_a, acc || kk > 0);
       };
       auto issue_s = [&](int t) {
         const int st = t % R;
         if (ok) ok = bar_wait(Y1_FULL + 8 * st, (t / R) & 1);
         if (!ok) return;
         ptx::tc_fence_after();
-        abt(tS, sX1, sY1 + st * NS * kSlab);
-        ptx::mma_commit(S_FULL);
+        abt(tS + 128 * (t % GR), sX1, sY1 + st * NS * kHalf);
+        ptx::mma_commit(S_FULL + 8 * (t % GR));
       };
       auto issue_dp = [&](int t) {
         const int st = t % R;
         if (ok) ok = bar_wait(Y2_FULL + 8 * st, (t / R) & 1);
         if (!ok) return;
         ptx::tc_fence_after();
-        abt(tD, sX2, sY2 + st * NS * kSlab);
-        ptx::mma_commit(DP_FULL);
+        abt(tD + 128 * (t % GR), sX2, sY2 + st * NS * kHalf);
+        ptx::mma_commit(DP_FULL + 8 * (t % GR));
         if (!KV) ptx::mma_commit(Y2_EMPTY + 8 * st);
       };
-      issue_s(0);
+      for (int t = 0; t < GR && t < tiles; ++t) issue_s(t);
       issue_dp(0);
-      for (int t = 0; t < tiles && ok; ++t) {
-        const int st = t % R;
-        if (ok) ok = bar_wait(P_READY, t & 1);
-        if (!ok) break;
-        ptx::tc_fence_after();
-        pb(tA2, tS, (KV ? sY2 : sY1) + st * NS * kSlab, t > 0);
-        if (KV) ptx::mma_commit(Y2_EMPTY + 8 * st);
-        if (t + 1 < tiles) issue_s(t + 1);
-        if (ok) ok = bar_wait(DS_READY, t & 1);
-        if (!ok) break;
-        ptx::tc_fence_after();
-        pb(tA1, tD, sY1 + st * NS * kSlab, t > 0);
-        ptx::mma_commit(Y1_EMPTY + 8 * st);
+      for (int t = 0; t < tiles + GR - 1 && ok; ++t) {
+        if (t < tiles) {
+          const int st = t % R;
+          ok = bar_wait(P_READY + 8 * (t % GR), (t / GR) & 1);
+          if (!ok) break;
+          ptx::tc_fence_after();
+          pb(tA2, tS + 128 * (t % GR), (KV ? sY2 : sY1) + st * NS * kHalf, t > 0);
+          if (KV) ptx::mma_commit(Y2_EMPTY + 8 * st);
+          if (t + GR < tiles) issue_s(t + GR);
+        }
+        const int u = t - (GR - 1);
+        if (u >= 0) {
+          const int st = u % R;
+          if (ok) ok = bar_wait(DS_READY + 8 * (u % GR), (u / GR) & 1);
+          if (!ok) break;
+          ptx::tc_fence_after();
+          pb(tA1, tD + 128 * (u % GR), sY1 + st * NS * kHalf, u > 0);
+          ptx::mma_commit(Y1_EMPTY + 8 * st);
+        }
         if (t + 1 < tiles) issue_dp(t + 1);
       }
       if (!ok) atomicExch(a.err, 52);
@@ -227,174 +243,231 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     __syncwarp();
   } else {
-    const int hf = warp >> 2, row = threadIdx.x & 127;  // columns 64 hf .. 64 hf + 63 of row `row`
+    const int w = warp >> 2, row = threadIdx.x & 127;  // group, row of X
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_col = tS + 64 * hf + lanes, d_col = tD + 64 * hf + lanes;
+    const uint32_t s_col = tS + 128 * w + lanes, d_col = tD + 128 * w + lanes;
     const float sc = a.scale * kLog2e;
+    const uint64_t sc2 = f32x2(sc, sc);
     const uint8_t* mb = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
     const long long x = (long long)x0 + row;  // this row's query (first) or key (second)
     bool ok = true;
-    // first: this row's lse and t = dO . out, each half sums half of the values
-    float lse2 = INFINITY, t0 = 0.f, r = 0.f;
+    // first: this row's -lse and -t, t = dO . out (both groups form them)
+    float nl = -INFINITY, nt = 0.f, r = 0.f;
     bool dead = false;  // second: this row's key
     if (!KV) {
-      const bool in = x < a.Lq;
       const T* go = static_cast<const T*>(a.dout) + (int64_t)b * a.dos[0] + x * a.dos[1] + (int64_t)hx * a.dos[2];
       const T* fo = static_cast<const T*>(a.fout) + (int64_t)b * a.os[0] + x * a.os[1] + (int64_t)hx * a.os[2];
-      if (in) {
+      if (x < a.Lq) {
         const float z = a.lse[((int64_t)b * a.Hq + hx) * a.Lq + x];
-        lse2 = z == -INFINITY ? INFINITY : z * kLog2e;
-        for (int d = 8 * hf; d < a.D; d += 16) {
+        nl = z == -INFINITY ? -INFINITY : -z * kLog2e;  // a row without a key: P = 0
+#pragma unroll 4
+        for (int d = 0; d < a.D; d += 8) {
           const uint4 u = *reinterpret_cast<const uint4*>(go + d), v = *reinterpret_cast<const uint4*>(fo + d);
           const T *pu = reinterpret_cast<const T*>(&u), *pv = reinterpret_cast<const T*>(&v);
 #pragma unroll
-          for (int c = 0; c < 8; ++c) t0 = fmaf(to_f(pu[c]), to_f(pv[c]), t0);
+          for (int c = 0; c < 8; ++c) nt = fmaf(-to_f(pu[c]), to_f(pv[c]), nt);
         }
       }
-      red[128 * hf + row] = t0;
-      ptx::named_bar(1, 256);
-      t0 = red[row] + red[128 + row];
-      ptx::named_bar(1, 256);
     } else {
       dead = x >= len || (mb && !mb[x * a.mask_k]);
-      if (a.dws && threadIdx.x < 128) carry[threadIdx.x] = 0.f;
+      if (a.dws && row < kOpen) carry[64 * w + row] = 0.f;
     }
     float far_behind = 0.f, far_ahead = 0.f;
-    for (int t = 0; t < tiles; ++t) {
-      const int st = t % R;
-      const int y0 = KV ? (first + t % per) * 128 : t * 128;
-      const float* e = ext + st * 512;
-      uint32_t alive[2] = {~0u, ~0u};  // first: keys of this half
-      if (!KV && mb) {
+    int64_t at = 0;  // second: first diagonal of this group's array that is not written yet
+    // second: writes the end of a head's diagonals (the array of this group)
+    auto end_head = [&](int hy) {
+      float* dws = a.dws + ((((int64_t)b * a.Hq + hy) * ntile + xt) * GR + w) * a.dws_ld;
+      ptx::named_bar(1 + w, 128);  // the last open diagonals are there
+      for (int64_t z = at + row; z < a.dws_ld - 2; z += 128) dws[z] = z - at < kOpen ? carry[64 * w + (z - at)] : 0.f;
+      // sums of the tiles whole in a last bucket: lanes, then the four warps in order
+      float fb = far_behind, fa = far_ahead;
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const int j = y0 + 64 * hf + 32 * z + lane;
-          alive[z] = __ballot_sync(0xffffffffu, j < len && mb[(int64_t)j * a.mask_k] != 0);
-        }
+      for (int z = 16; z; z >>= 1) {
+        fb += __shfl_xor_sync(0xffffffffu, fb, z);
+        fa += __shfl_xor_sync(0xffffffffu, fa, z);
       }
+      ptx::named_bar(1 + w, 128);
+      if (lane == 0) {
+        diag_s[warp * kDiagLd] = fb;
+        diag_s[warp * kDiagLd + 1] = fa;
+      }
+      if (row < kOpen) carry[64 * w + row] = 0.f;
+      ptx::named_bar(1 + w, 128);
+      if (row < 2) {
+        const float* f = diag_s + 4 * w * kDiagLd + row;
+        dws[a.dws_ld - 2 + row] = ((f[0] + f[kDiagLd]) + f[2 * kDiagLd]) + f[3 * kDiagLd];
+      }
+      ptx::named_bar(1 + w, 128);
+      far_behind = far_ahead = 0.f;
+      at = 0;
+    };
+    int head = 0;  // second: heads of the group whose diagonals are written
+    uint8_t byte0 = 0, byte1 = 0;  // first: mask of keys `lane` and 32 + `lane` of this group's next tile
+    auto fetch = [&](int y0) {
+      byte0 = y0 + lane < len ? mb[(int64_t)(y0 + lane) * a.mask_k] : 0;
+      byte1 = y0 + 32 + lane < len ? mb[(int64_t)(y0 + 32 + lane) * a.mask_k] : 0;
+    };
+    if (!KV && mb) fetch(64 * w);
+    for (int t = w; t < tiles; t += GR) {
+      const int st = t % R;
+      const uint32_t turn = (t / GR) & 1;
+      const int y0 = KV ? (first + t % per) * 64 : t * 64;
+      const float* e = ext + st * kExt;
+      if (KV && a.dws)
+        for (; head < t / per; ++head) end_head(kh * G + head);
+      uint32_t alive[2] = {~0u, ~0u};  // first: keys of the tile; the mask's bytes came with the last one
+      if (!KV && mb) {
+        alive[0] = __ballot_sync(0xffffffffu, byte0 != 0);
+        alive[1] = __ballot_sync(0xffffffffu, byte1 != 0);
+        fetch(y0 + 64 * GR);
+      }
+      // relative positions of the tile: [hi - 190, hi]; where they lie whole in the
+      // last bucket the bias is one value, and so is the gradient's bucket
+      const long long hi = (KV ? (long long)x0 + 127 - y0 : (long long)y0 + 63 - x0) - a.q_off;
+      const bool behind = hi <= -(long long)a.far, ahead = hi - 190 >= (a.far_both ? (long long)a.far : 0ll);
+      const bool flat = behind || ahead;
       float p[64];
-      do {  // a wait that gives up leaves the tile; the warps meet again below
+      do {  // a wait that gives up leaves the tile; the warps of a group meet again below
         if (extras && !(ok = warp_wait(Y1_FULL + 8 * st, (t / R) & 1))) break;
-        if (!(ok = warp_wait(S_FULL, t & 1))) break;
+        if (!(ok = warp_wait(S_FULL + 8 * w, turn))) break;
         ptx::tc_fence_after();
+        const float* bb = KV ? e + 64 + row : e + 128 - row;
+        const float whole = KV ? (a.diag && flat ? bb[0] : 0.f) : nl + (a.diag && flat ? bb[0] : 0.f);
+        const bool each = a.diag && !flat;
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
           uint32_t s[32];
           ptx::tmem_ld32_async(s_col + 32 * z, s);
           ptx::tmem_wait_ld(s);
-          if (KV) {
 #pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              const float4 l4 = *reinterpret_cast<const float4*>(e + 256 + 64 * hf + 32 * z + c);
-              p[32 * z + c] = -l4.x, p[32 * z + c + 1] = -l4.y, p[32 * z + c + 2] = -l4.z, p[32 * z + c + 3] = -l4.w;
+          for (int c = 0; c < 32; c += 4) {
+            uint64_t o0 = f32x2(whole, whole), o1 = o0;
+            if (KV) {
+              const float4 l4 = *reinterpret_cast<const float4*>(e + 192 + 32 * z + c);
+              o0 = add2(o0, f32x2(l4.x, l4.y));
+              o1 = add2(o1, f32x2(l4.z, l4.w));
             }
-            if (a.diag) {
-              const float* bb = e + 128 + row - 64 * hf - 32 * z;
-#pragma unroll
-              for (int c = 0; c < 32; ++c) p[32 * z + c] += bb[-c];
+            if (each) {
+              const int k = 32 * z + c;
+              o0 = add2(o0, KV ? f32x2(bb[-k], bb[-k - 1]) : f32x2(bb[k], bb[k + 1]));
+              o1 = add2(o1, KV ? f32x2(bb[-k - 2], bb[-k - 3]) : f32x2(bb[k + 2], bb[k + 3]));
             }
-          } else if (a.diag) {
-            const float* bb = e + 128 - row + 64 * hf + 32 * z;
-#pragma unroll
-            for (int c = 0; c < 32; ++c) p[32 * z + c] = bb[c] - lse2;
-          } else {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) p[32 * z + c] = -lse2;
+            float v0, v1, v2, v3;
+            split2(fma2(f32x2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, o0), v0, v1);
+            split2(fma2(f32x2(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])), sc2, o1), v2, v3);
+            p[32 * z + c] = exp2_approx(v0);
+            p[32 * z + c + 1] = exp2_approx(v1);
+            p[32 * z + c + 2] = exp2_approx(v2);
+            p[32 * z + c + 3] = exp2_approx(v3);
           }
-#pragma unroll
-          for (int c = 0; c < 32; ++c) p[32 * z + c] = exp2_approx(fmaf(__uint_as_float(s[c]), sc, p[32 * z + c]));
         }
+        bool cut = false;  // pairs that do not take part: their P is 0, whatever dP is
         if (KV) {
-          // causal: queries c of this half with y0 + 64 hf + c + q_off < key are out
-          const long long lo = a.causal ? x - a.q_off - y0 - 64 * hf : 0;
-          if (dead || lo > 0) {
+          // causal: queries c with y0 + c + q_off < key are out
+          const long long lo = a.causal ? x - a.q_off - y0 : 0;
+          cut = dead || lo > 0;
+          if (cut) {
             const int n = dead ? 64 : (int)min(64ll, lo);
-#pragma unroll
-            for (int c = 0; c < 64; ++c) p[c] = c < n ? 0.f : p[c];
+            alive[0] = ~low_bits(n), alive[1] = ~low_bits(n - 32);
           }
         } else {
-          const long long lim = (a.causal ? min((long long)len, x + a.q_off + 1) : (long long)len) - y0 - 64 * hf;
-          if (mb || lim < 64) {
-            const int n = (int)max(0ll, min(64ll, lim));
-#pragma unroll
-            for (int c = 0; c < 64; ++c) p[c] = c < n && ((alive[c >> 5] >> (c & 31)) & 1) ? p[c] : 0.f;
-          }
-          if (mb || y0 + 128 > len) {  // zero the dead rows of K: both halves' threads take half of the slabs
-            const int j = y0 + row;
-            if (j >= len || (mb && !mb[(int64_t)j * a.mask_k])) {
-              uint4* zr = reinterpret_cast<uint4*>(gen + 2 * NS * kSlab + st * NS * kSlab + row * 128);
+          const long long lim = (a.causal ? min((long long)len, x + a.q_off + 1) : (long long)len) - y0;
+          if (mb || y0 + 64 > len) {  // zero the dead rows of K: two threads to a key, half of its bytes each
+            const int k = row >> 1;
+            if (y0 + k >= len || !(((warp & 2 ? alive[1] : alive[0]) >> (k & 31)) & 1)) {
+              uint4* zr = reinterpret_cast<uint4*>(gen + oY1 + st * NS * kHalf + k * 128) + 4 * (row & 1);
 #pragma unroll
               for (int s = 0; s < NS; ++s)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) zr[s * (kSlab / 16) + 4 * hf + c] = make_uint4(0, 0, 0, 0);
+                for (int c = 0; c < 4; ++c) zr[s * (kHalf / 16) + c] = make_uint4(0, 0, 0, 0);
             }
             ptx::fence_proxy_async_smem();
           }
+          cut = mb || lim < 64;
+          if (cut) {
+            const int n = (int)max(0ll, min(64ll, lim));
+            alive[0] &= low_bits(n), alive[1] &= low_bits(n - 32);
+          }
+        }
+        if (cut) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (!(alive[c >> 5] & (1u << (c & 31)))) p[c] = 0.f;
         }
         {
-          uint32_t w[32];
+          uint32_t q[32];
 #pragma unroll
-          for (int c = 0; c < 32; ++c) w[c] = pack2<T>(p[2 * c], p[2 * c + 1]);
-          tmem_st32(s_col, w);
+          for (int c = 0; c < 32; ++c) q[c] = pack2<T>(p[2 * c], p[2 * c + 1]);
+          tmem_st32(s_col, q);
         }
         tmem_wait_st();
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(P_READY);
+        if (lane == 0) ptx::mbar_arrive(P_READY + 8 * w);
 
-        if (!(ok = warp_wait(DP_FULL, t & 1))) break;
+        if (!(ok = warp_wait(DP_FULL + 8 * w, turn))) break;
         ptx::tc_fence_after();
+        uint64_t sum = f32x2(0.f, 0.f);
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
           uint32_t s[32];
           ptx::tmem_ld32_async(d_col + 32 * z, s);
           ptx::tmem_wait_ld(s);
-          if (KV) {
 #pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              const float4 d4 = *reinterpret_cast<const float4*>(e + 384 + 64 * hf + 32 * z + c);
-              const float dd[4] = {d4.x, d4.y, d4.z, d4.w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                float& q = p[32 * z + c + k];
-                q = q != 0.f ? q * (__uint_as_float(s[c + k]) - dd[k]) : 0.f;
-              }
+          for (int c = 0; c < 32; c += 4) {
+            uint64_t n0 = f32x2(nt, nt), n1 = n0;
+            if (KV) {
+              const float4 d4 = *reinterpret_cast<const float4*>(e + 256 + 32 * z + c);
+              n0 = f32x2(d4.x, d4.y), n1 = f32x2(d4.z, d4.w);
             }
-          } else {
+            float* q = p + 32 * z + c;
+            const uint64_t u0 = mul2(f32x2(q[0], q[1]), add2(f32x2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), n0));
+            const uint64_t u1 =
+                mul2(f32x2(q[2], q[3]), add2(f32x2(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])), n1));
+            float v[4];
+            split2(u0, v[0], v[1]);
+            split2(u1, v[2], v[3]);
+            if (cut) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              float& q = p[32 * z + c];
-              q = q != 0.f ? q * (__uint_as_float(s[c]) - t0) : 0.f;
-              r += q;
+              for (int k = 0; k < 4; ++k) q[k] = alive[z] & (1u << (c + k)) ? v[k] : 0.f;
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) q[k] = v[k];
             }
+            if (!KV) sum = add2(sum, add2(f32x2(q[0], q[1]), f32x2(q[2], q[3])));
           }
         }
+        if (!KV) {
+          float u, v;
+          split2(sum, u, v);
+          r += u + v;
+        }
         {
-          uint32_t w[32];
+          uint32_t q[32];
 #pragma unroll
-          for (int c = 0; c < 32; ++c) w[c] = pack2<T>(p[2 * c], p[2 * c + 1]);
-          tmem_st32(d_col, w);
+          for (int c = 0; c < 32; ++c) q[c] = pack2<T>(p[2 * c], p[2 * c + 1]);
+          tmem_st32(d_col, q);
         }
         tmem_wait_st();
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          ptx::mbar_arrive(DS_READY);
+          ptx::mbar_arrive(DS_READY + 8 * w);
           if (extras) ptx::mbar_arrive(Y1_EMPTY + 8 * st);
         }
       } while (false);
-      // the named barriers below are taken by all warps or by none
-      if (KV && a.dws) ok = ptx::named_bar_and(1, 256, ok);
+      // the named barriers below are taken by all warps of a group or by none
+      if (KV && a.dws) ok = ptx::named_bar_and(1 + w, 128, ok);
       if (!ok) break;
       if (KV && a.dws) {
-        const int hy = kh * G + t / per, tq = t % per;
-        float* dws = a.dws + (((int64_t)b * a.Hq + hy) * ntile + xt) * a.dws_ld;
-        // relative positions of the tile: [hi - 254, hi]
-        const long long hi = (long long)x0 + 127 - y0 - a.q_off;
-        const bool behind = hi <= -(long long)a.far, ahead = hi - 254 >= (a.far_both ? (long long)a.far : 0ll);
-        const int u = threadIdx.x;  // diagonal key - query = 127 - u within the tile, u < 255
-        float v = 0.f;
-        if (behind || ahead) {
+        float* dws = a.dws + ((((int64_t)b * a.Hq + kh * G + head) * ntile + xt) * GR + w) * a.dws_ld;
+        // Diagonal u < 191 of the tile: key - query = 127 - u; it is entry y0 + u of
+        // the array.  The first kStep are whole with this tile (the group's next is
+        // kStep queries on), the others stay open.
+        for (int64_t z = at + row; z < y0; z += 128) dws[z] = z - at < kOpen ? carry[64 * w + (z - at)] : 0.f;
+        const bool joins = at == y0;  // the open diagonals are the first of this tile
+        float v0 = 0.f, v1 = 0.f;     // diagonals row and 128 + row
+        if (flat) {
           float s = 0.f;
 #pragma unroll
           for (int c = 0; c < 64; ++c) s += p[c];
@@ -411,53 +484,27 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             if (c < 63) acc = lane == 0 ? 0.f : up;
           }
           if (lane < 31) mine[94 - lane] = acc;  // lane - 63
-          ptx::named_bar(1, 256);
-          if (u < 255) {
+          ptx::named_bar(1 + w, 128);
 #pragma unroll
-            for (int w = 0; w < 8; ++w) {
-              // rows 32 (w & 3) + lane, columns 64 (w >> 2) + c: entry 31 - (lane - c)
-              const int k = 31 - ((127 - u) - 32 * (w & 3) + 64 * (w >> 2));
-              if (k >= 0 && k < 95) v += diag_s[w * kDiagLd + k];
-            }
+          for (int y = 0; y < 4; ++y) {
+            // rows 32 y + lane, columns c: entry 31 - (lane - c) = 31 - (127 - u - 32 y)
+            const float* part = diag_s + (4 * w + y) * kDiagLd;
+            const int k = 31 - (127 - row - 32 * y);
+            if (k >= 0 && k < 95) v0 += part[k];
+            if (row < 63 && k + 128 < 95) v1 += part[k + 128];
           }
         }
-        // u <= 127 (key - query >= 0) is whole with this tile, the others go on in the next
-        if (u < 128) dws[(int64_t)(first + tq) * 128 + u] = v + carry[u];
-        ptx::named_bar(1, 256);
-        if (u >= 128 && u < 256) carry[u - 128] = u < 255 ? v : 0.f;
-        ptx::named_bar(1, 256);
-        if (tq + 1 == per) {  // a head ends: its open diagonals, and zeros where no tile was
-          const int64_t end = (int64_t)(first + per) * 128;
-          for (int64_t z = u; z < a.dws_ld - 2; z += 256)
-            if (z < (int64_t)first * 128 || z >= end) dws[z] = z >= end && z < end + 128 ? carry[z - end] : 0.f;
-          const float fb = far_behind, fa = far_ahead;
-          red[u] = fb;
-          ptx::named_bar(1, 256);
-          if (u == 0) {
-            float s = 0.f;
-            for (int z = 0; z < 256; ++z) s += red[z];
-            dws[a.dws_ld - 2] = s;
-          }
-          ptx::named_bar(1, 256);
-          red[u] = fa;
-          ptx::named_bar(1, 256);
-          if (u == 0) {
-            float s = 0.f;
-            for (int z = 0; z < 256; ++z) s += red[z];
-            dws[a.dws_ld - 1] = s;
-          }
-          far_behind = far_ahead = 0.f;
-          if (u < 128) carry[u] = 0.f;
-          ptx::named_bar(1, 256);
-        }
+        if (joins && row < kOpen) v0 += carry[64 * w + row];
+        if (row < kStep) dws[(int64_t)y0 + row] = v0;
+        ptx::named_bar(1 + w, 128);
+        if (row >= kStep) carry[64 * w + row - kStep] = v0;
+        if (row < 64) carry[64 * w + 128 - kStep + row] = row < 63 ? v1 : 0.f;
+        at = (int64_t)y0 + kStep;
+        ptx::named_bar(1 + w, 128);
       }
     }
-    if (KV && a.dws && tiles == 0) {
-      for (int g = 0; g < G; ++g) {
-        float* dws = a.dws + (((int64_t)b * a.Hq + kh * G + g) * ntile + xt) * a.dws_ld;
-        for (int64_t z = threadIdx.x; z < a.dws_ld; z += 256) dws[z] = 0.f;
-      }
-    }
+    if (KV && a.dws && ok)
+      for (; head < G; ++head) end_head(kh * G + head);
     if (ok && tiles > 0) ok = warp_wait(DONE, 0);
     ptx::tc_fence_after();
     if (!ok) {
@@ -465,23 +512,26 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     float rr = 0.f;
     if (!KV) {
-      // every warp comes here, also after a wait that gave up
-      red[128 * hf + row] = r;
-      ptx::named_bar(1, 256);
-      rr = red[row] + red[128 + row];
-      if (hf == 0) {
-        const int64_t at = ((int64_t)b * a.Hq + hx) * Lp + x;
-        a.lse2[at] = lse2;
-        a.delta[at] = lse2 == INFINITY ? 0.f : t0 + rr;
+      // the groups' sums of a row (every warp comes here, also after a wait that gave up)
+      rr = r;
+      if (GR == 2) {
+        ext[128 * w + row] = r;
+        ptx::named_bar(3, 256);
+        rr = ext[row] + ext[128 + row];
+      }
+      if (w == 0) {
+        const int64_t to = ((int64_t)b * a.Hq + hx) * Lp + x;
+        a.lse2[to] = nl;
+        a.delta[to] = nl == -INFINITY ? 0.f : nt - rr;
       }
     }
     if (ok) {
       const int L = KV ? a.Lk : a.Lq;
-      const int64_t at = (((int64_t)b * L + x) * heads + hx) * a.D;
-      T* d1 = static_cast<T*>(KV ? a.dk : a.dq) + at;
-      T* d2 = static_cast<T*>(a.dv) + at;
+      const int64_t to = (((int64_t)b * L + x) * heads + hx) * a.D;
+      T* d1 = static_cast<T*>(KV ? a.dk : a.dq) + to;
+      T* d2 = static_cast<T*>(a.dv) + to;
 #pragma unroll 1
-      for (int c0 = 32 * NS * hf; c0 < 32 * NS * (hf + 1); c0 += 16) {
+      for (int c0 = 64 * NS / GR * w; c0 < 64 * NS / GR * (w + 1); c0 += 16) {  // each group its share of the values
         if (c0 >= a.D) break;
         float u[16], v[16];
         if (tiles > 0) {
@@ -509,39 +559,51 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  if (warp == 9) ptx::tmem_dealloc(tmem, 512);
+  if (warp == kIssue) ptx::tmem_dealloc(tmem, 256 * GR);
 }
 
-template <typename T, int NS, bool KV>
+template <typename T, int NS, bool KV, bool FULL>
 void launch(const AttnArgs& a, const BwdMaps& maps, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};  // one bit per device
   int dev = 0;
   RVC_CUDA_TRY(cudaGetDevice(&dev));
   if (dev >= 64 || !(done.load() & (1ull << dev))) {
-    RVC_CUDA_TRY(cudaFuncSetAttribute(attn_tc_bwd_kernel<T, NS, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    RVC_CUDA_TRY(cudaFuncSetAttribute(attn_tc_bwd_kernel<T, NS, KV, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)bwd_smem<NS>()));
     if (dev < 64) done.fetch_or(1ull << dev);
   }
   const unsigned grid = KV ? (unsigned)((a.Lk + 127ll) / 128 * a.B * a.Hkv) : (unsigned)((a.Lq + 127ll) / 128 * a.B * a.Hq);
-  attn_tc_bwd_kernel<T, NS, KV><<<grid, kBwdThreads, bwd_smem<NS>(), st>>>(a, maps);
+  attn_tc_bwd_kernel<T, NS, KV, FULL><<<grid, kBwdThreads<NS>, bwd_smem<NS>(), st>>>(a, maps);
   note_launch();
   RVC_CUDA_TRY(cudaGetLastError());
 }
 
-template <typename T, int NS>
+template <typename T, int NS, bool FULL>
 void bwd(const AttnArgs& a, cudaStream_t st) {
   BwdMaps m;
   make_map(&m.x1, a.type, a.q, a.qs, a.B, a.Lq, a.Hq, a.D, 128);
   make_map(&m.x2, a.type, a.dout, a.dos, a.B, a.Lq, a.Hq, a.D, 128);
-  make_map(&m.y1, a.type, a.k, a.ks, a.B, a.Lk, a.Hkv, a.D, 128);
-  make_map(&m.y2, a.type, a.v, a.vs, a.B, a.Lk, a.Hkv, a.D, 128);
-  launch<T, NS, false>(a, m, st);
-  std::swap(m.x1, m.y1);
-  std::swap(m.x2, m.y2);
-  launch<T, NS, true>(a, m, st);
+  make_map(&m.y1, a.type, a.k, a.ks, a.B, a.Lk, a.Hkv, a.D, 64);
+  make_map(&m.y2, a.type, a.v, a.vs, a.B, a.Lk, a.Hkv, a.D, 64);
+  launch<T, NS, false, FULL>(a, m, st);
+  make_map(&m.x1, a.type, a.k, a.ks, a.B, a.Lk, a.Hkv, a.D, 128);
+  make_map(&m.x2, a.type, a.v, a.vs, a.B, a.Lk, a.Hkv, a.D, 128);
+  make_map(&m.y1, a.type, a.q, a.qs, a.B, a.Lq, a.Hq, a.D, 64);
+  make_map(&m.y2, a.type, a.dout, a.dos, a.B, a.Lq, a.Hq, a.D, 64);
+  launch<T, NS, true, FULL>(a, m, st);
+}
+
+template <typename T>
+void bwd_t(const AttnArgs& a, cudaStream_t st) {
+  if (a.D == 64) bwd<T, 1, true>(a, st);
+  else if (a.D < 64) bwd<T, 1, false>(a, st);
+  else if (a.D == 128) bwd<T, 2, true>(a, st);
+  else bwd<T, 2, false>(a, st);
 }
 
 }  // namespace
+
+int attn_tc_bwd_arrays(const AttnArgs& a) { return a.D <= 64 ? kGroups<1> : kGroups<2>; }
 
 bool attn_tc_bwd_fits(const AttnArgs& a) {
   const auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
@@ -551,13 +613,8 @@ bool attn_tc_bwd_fits(const AttnArgs& a) {
 }
 
 void attn_tc_backward(const AttnArgs& a, cudaStream_t st) {
-  if (a.type == kBf16) {
-    if (a.D <= 64) bwd<__nv_bfloat16, 1>(a, st);
-    else bwd<__nv_bfloat16, 2>(a, st);
-  } else {
-    if (a.D <= 64) bwd<__half, 1>(a, st);
-    else bwd<__half, 2>(a, st);
-  }
+  if (a.type == kBf16) bwd_t<__nv_bfloat16>(a, st);
+  else bwd_t<__half>(a, st);
 }
 
 }  // namespace rvc
