@@ -3,18 +3,23 @@
 // fast ones where rows are few (one new token against long states) or the
 // type is fp32.
 //
-// 16-bit inputs go through m16n8k16 with fp32 accumulators; fp32 inputs
-// through m16n8k8 TF32 with each operand split as hi + lo (both rounded to
-// TF32's 11 bits) and three products hi.hi + hi.lo + lo.hi, which leaves about
-// 2^-22 of a product: the accuracy of an fp32 sum.  Weights P and dS enter
-// their second product rounded to the inputs' type (16-bit inputs: 2^-9 /
-// 2^-12, the rounding of the output itself) or split the same way (fp32).
+// 16-bit inputs go through m16n8k16 with fp32 accumulators.  fp32 inputs are
+// split into three bf16 parts (24 bits) when they are staged, and a product is
+// the six of their products that are above 2^-24, smallest first; the tensor
+// cores cut their sums off instead of rounding them, so every 16 values' worth
+// is formed in an accumulator of its own and added in fp32 with rounding (a
+// chain in one accumulator was off by 6e-6 over 1500 keys).  Where rows are few
+// and the reading of the states counts, fp32 stays as it is in shared memory and
+// goes through m16n8k8 TF32 as hi + lo with three products (2^-22).  Weights P
+// and dS enter their second product rounded to the inputs' type (16-bit inputs:
+// the rounding of the output itself) or split the same way (fp32).
 //
-// Layout: a block stages a tile of keys and values in shared memory (cp.async,
-// two stages) with 16 bytes of padding per row, so that both the row-wise and
-// the transposed fragment reads are free of bank conflicts.  Dead keys (past
-// the length or masked out) are staged as zeros: whatever the caller's buffer
-// holds there, NaN included, never meets a product.
+// Layout: a block stages a tile of keys and values in shared memory (16-bit
+// types by cp.async in two stages, fp32 through registers) with 16 bytes of
+// padding per row, so that both the row-wise and the transposed fragment reads
+// are free of bank conflicts.  Dead keys (past the length or masked out) are
+// staged as zeros: whatever the caller's buffer holds there, NaN included, never
+// meets a product.
 #include "attn_common.cuh"
 #include "context.cuh"
 #include "tc_ptx.cuh"
@@ -26,8 +31,8 @@ namespace rvc {
 
 namespace {
 
-constexpr int kT = 128;   // threads of a block (4 warps)
-constexpr int kBN = 64;   // keys per tile
+constexpr int kT = 128;   // threads of a forward block (4 warps)
+constexpr int kBN = 64;   // keys per tile (16-bit types)
 constexpr int kBM = 64;   // query rows per block (4 warps x 16) where rows are many
 
 // ------------------------------------------------------------ fragment helpers
@@ -95,60 +100,207 @@ template <int N> __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Bytes of a staged row: D values and 16 bytes, so rows start 4 banks apart.
-template <typename T, int DP> constexpr int pitch() { return DP * (int)sizeof(T) + 16; }
+template <typename T> constexpr int kParts = sizeof(T) == 4 ? 3 : 1;  // bf16 parts of a value
+// Bytes of a staged row (of one part): D 16-bit values and 16 bytes, so rows
+// start 4 banks apart.
+template <int DP> constexpr int pitch() { return DP * 2 + 16; }
+template <typename T, int DP> constexpr int tile_bytes(int rows) { return kParts<T> * rows * pitch<DP>(); }
+// Staged rows: the first row of the first part, and the distance of the parts.
+struct Rows {
+  uint32_t at, part;
+};
+template <typename T> struct MmaType { using type = T; };
+template <> struct MmaType<float> { using type = __nv_bfloat16; };
 
-// C[16][8 NT] (+)= A[16][DP] . B[8 NT][DP]^T; A at `a`, B at `b`, both staged rows.
+// x = hi + mid + lo in bf16 for two values at once, each rounded from what is left.
+__device__ __forceinline__ void split3(float a, float b, uint32_t (&w)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    w[i] = pack2<__nv_bfloat16>(a, b);
+    a -= __uint_as_float(w[i] << 16);
+    b -= __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+// c0, c1 += the six products of three parts each that count, smallest first.
+__device__ __forceinline__ void mma_parts(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[3][4],
+                                          const uint32_t (&b)[3][4]) {
+  constexpr int pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
+  float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) {
+    mma16(t0, a[pa[i]], b[pb[i]][0], b[pb[i]][1], __nv_bfloat16());
+    mma16(t1, a[pa[i]], b[pb[i]][2], b[pb[i]][3], __nv_bfloat16());
+  }
+#pragma unroll
+  for (int x = 0; x < 4; ++x) c0[x] += t0[x], c1[x] += t1[x];
+}
+
+// C[16][8 NT] (+)= A[16][DP] . B[8 NT][DP]^T; A and B staged rows.
 template <typename T, int DP, int NT>
-__device__ __forceinline__ void mma_abt(float (&c)[NT][4], uint32_t a, uint32_t b, int lane) {
-  constexpr int P = pitch<T, DP>();
-  if constexpr (sizeof(T) == 2) {
-    const int mi = lane >> 3, r8 = lane & 7;
+__device__ __forceinline__ void mma_abt(float (&c)[NT][4], Rows a, Rows b, int lane) {
+  constexpr int P = pitch<DP>(), N = kParts<T>;
+  const int mi = lane >> 3, r8 = lane & 7;
+  const uint32_t ra = a.at + ((mi & 1) * 8 + r8) * P + (mi >> 1) * 16, rb = b.at + ((mi >> 1) * 8 + r8) * P + (mi & 1) * 16;
+#pragma unroll(N == 1 ? DP / 16 : 1)
+  for (int kk = 0; kk < DP / 16; ++kk) {
+    uint32_t af[N][4];
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
-      uint32_t af[4];
-      ldsm4(af, a + ((mi & 1) * 8 + r8) * P + (kk * 16 + (mi >> 1) * 8) * 2);
+    for (int i = 0; i < N; ++i) ldsm4(af[i], ra + i * a.part + kk * 32);
 #pragma unroll
-      for (int n = 0; n < NT; n += 2) {
-        uint32_t bf[4];
-        ldsm4(bf, b + (n * 8 + (mi >> 1) * 8 + r8) * P + (kk * 16 + (mi & 1) * 8) * 2);
-        mma16(c[n], af, bf[0], bf[1], T());
-        mma16(c[n + 1], af, bf[2], bf[3], T());
-      }
-    }
-  } else {
-    const int g = lane >> 2, t = lane & 3;
-#pragma unroll 2
-    for (int kk = 0; kk < DP / 8; ++kk) {
-      Split4 af;
-      const uint32_t ar = a + g * P + (kk * 8 + t) * 4;
-      split_tf32(lds_f(ar), af.hi[0], af.lo[0]);
-      split_tf32(lds_f(ar + 8 * P), af.hi[1], af.lo[1]);
-      split_tf32(lds_f(ar + 16), af.hi[2], af.lo[2]);
-      split_tf32(lds_f(ar + 8 * P + 16), af.hi[3], af.lo[3]);
+    for (int n = 0; n < NT; n += 2) {
+      uint32_t bf[N][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const uint32_t br = b + (n * 8 + g) * P + (kk * 8 + t) * 4;
-        mma8x3(c[n], af, lds_f(br), lds_f(br + 16));
+      for (int i = 0; i < N; ++i) ldsm4(bf[i], rb + i * b.part + n * 8 * P + kk * 32);
+      if constexpr (N == 1) {
+        mma16(c[n], af[0], bf[0][0], bf[0][1], T());
+        mma16(c[n + 1], af[0], bf[0][2], bf[0][3], T());
+      } else {
+        mma_parts(c[n], c[n + 1], af, bf);
       }
     }
   }
 }
 
-// The A operand of mma_abt held in registers over many calls (16-bit types).
+// C[16][DP] += A[16][8 NT] . B[8 NT][DP]: A are accumulator fragments (weights),
+// B staged rows.
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void mma_pb(float (&c)[DP / 8][4], const float (&p)[NT][4], Rows b, int lane) {
+  constexpr int P = pitch<DP>(), N = kParts<T>;
+  const int mi = lane >> 3, r8 = lane & 7;
+  const uint32_t rb = b.at + ((mi & 1) * 8 + r8) * P + (mi >> 1) * 16;
+#pragma unroll
+  for (int n = 0; n < NT; n += 2) {
+    uint32_t af[N][4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float u = p[n + (x >> 1)][2 * (x & 1)], v = p[n + (x >> 1)][2 * (x & 1) + 1];
+      if constexpr (N == 1) {
+        af[0][x] = pack2<T>(u, v);
+      } else {
+        uint32_t w[3];
+        split3(u, v, w);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) af[i][x] = w[i];
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 8; d += 2) {
+      uint32_t bf[N][4];
+#pragma unroll
+      for (int i = 0; i < N; ++i) ldsm4t(bf[i], rb + i * b.part + n * 8 * P + d * 16);
+      if constexpr (N == 1) {
+        mma16(c[d], af[0], bf[0][0], bf[0][1], T());
+        mma16(c[d + 1], af[0], bf[0][2], bf[0][3], T());
+      } else {
+        mma_parts(c[d], c[d + 1], af, bf);
+      }
+    }
+  }
+}
+
+// Stages `rows` rows into `dst`; row r comes from src(r), a null source is
+// staged as zeros.  Columns past D are zeros.
+template <typename T, int DP, int THREADS, typename F>
+__device__ __forceinline__ void stage_rows(Rows dst, int rows, int D, bool vec, int tid, F src) {
+  constexpr int P = pitch<DP>();
+  if constexpr (sizeof(T) == 2) {
+    if (vec) {
+      constexpr int CH = DP / 8;
+      for (int e = tid; e < rows * CH; e += THREADS) {
+        const int r = e / CH, c = e % CH;
+        const T* s = src(r);
+        const bool on = s != nullptr && c * 8 < D;
+        cp16(dst.at + r * P + c * 16, on ? s + c * 8 : nullptr, on ? 16u : 0u);
+      }
+    } else {
+      for (int e = tid; e < rows * DP; e += THREADS) {
+        const int r = e / DP, c = e % DP;
+        const T* s = src(r);
+        const T v = (s != nullptr && c < D) ? s[c] : from_f<T>(0.f);
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst.at + r * P + c * 2), "h"(*reinterpret_cast<const uint16_t*>(&v))
+                     : "memory");
+      }
+    }
+  } else {
+    constexpr int CH = DP / 4;
+#pragma unroll 4
+    for (int e = tid; e < rows * CH; e += THREADS) {
+      const int r = e / CH, c = e % CH * 4;
+      const T* s = src(r);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s != nullptr) {
+        if (vec) {
+          if (c < D) v = *reinterpret_cast<const float4*>(s + c);
+        } else {
+          if (c < D) v.x = s[c];
+          if (c + 1 < D) v.y = s[c + 1];
+          if (c + 2 < D) v.z = s[c + 2];
+          if (c + 3 < D) v.w = s[c + 3];
+        }
+      }
+      uint32_t lo[3], hi[3];
+      split3(v.x, v.y, lo);
+      split3(v.z, v.w, hi);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) ptx::sts64(dst.at + i * dst.part + r * P + c * 2, lo[i], hi[i]);
+    }
+  }
+}
+
+// ------------------------------------- fp32 as it is, for few rows (TF32 hi + lo)
+template <typename T, int DP> constexpr int raw_pitch() { return DP * (int)sizeof(T) + 16; }
+
+template <int DP>
+__device__ __forceinline__ void tf32_abt(float (&c)[2][4], uint32_t a, uint32_t b, int lane) {
+  constexpr int P = raw_pitch<float, DP>();
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll 2
+  for (int kk = 0; kk < DP / 8; ++kk) {
+    Split4 af;
+    const uint32_t ar = a + g * P + (kk * 8 + t) * 4;
+    split_tf32(lds_f(ar), af.hi[0], af.lo[0]);
+    split_tf32(lds_f(ar + 8 * P), af.hi[1], af.lo[1]);
+    split_tf32(lds_f(ar + 16), af.hi[2], af.lo[2]);
+    split_tf32(lds_f(ar + 8 * P + 16), af.hi[3], af.lo[3]);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const uint32_t br = b + (n * 8 + g) * P + (kk * 8 + t) * 4;
+      mma8x3(c[n], af, lds_f(br), lds_f(br + 16));
+    }
+  }
+}
+// The contraction runs over the columns in the order 2t, 2t + 1, which is the
+// accumulators' own, so no value changes lanes.
+template <int DP>
+__device__ __forceinline__ void tf32_pb(float (&c)[DP / 8][4], const float (&p)[2][4], uint32_t b, int lane) {
+  constexpr int P = raw_pitch<float, DP>();
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    Split4 af;
+    split_tf32(p[n][0], af.hi[0], af.lo[0]);
+    split_tf32(p[n][2], af.hi[1], af.lo[1]);
+    split_tf32(p[n][1], af.hi[2], af.lo[2]);
+    split_tf32(p[n][3], af.hi[3], af.lo[3]);
+    const uint32_t br = b + (n * 8 + 2 * t) * P + g * 4;
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d) mma8x3(c[d], af, lds_f(br + d * 32), lds_f(br + P + d * 32));
+  }
+}
+
+// The A operand held in registers over many calls (16-bit types).
 template <typename T, int DP>
 struct FragA {
   uint32_t f[DP / 16][4];
   __device__ __forceinline__ void load(uint32_t a, int lane) {
     const int mi = lane >> 3, r8 = lane & 7;
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk)
-      ldsm4(f[kk], a + ((mi & 1) * 8 + r8) * pitch<T, DP>() + (kk * 16 + (mi >> 1) * 8) * 2);
+    for (int kk = 0; kk < DP / 16; ++kk) ldsm4(f[kk], a + ((mi & 1) * 8 + r8) * pitch<DP>() + (kk * 16 + (mi >> 1) * 8) * 2);
   }
   // C[16][16] += A . B[16][DP]^T
   __device__ __forceinline__ void abt(float (&c)[2][4], uint32_t b, int lane) const {
     const int mi = lane >> 3, r8 = lane & 7;
-    const uint32_t at = b + ((mi >> 1) * 8 + r8) * pitch<T, DP>() + (mi & 1) * 16;
+    const uint32_t at = b + ((mi >> 1) * 8 + r8) * pitch<DP>() + (mi & 1) * 16;
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
       uint32_t bf[4];
@@ -159,116 +311,61 @@ struct FragA {
   }
 };
 
-// C[16][DP] += A[16][8 NT] . B[8 NT][DP]: A are accumulator fragments (weights),
-// B staged rows.  fp32: the contraction runs over the columns in the order
-// 2t, 2t + 1, which is the accumulators' own, so no value changes lanes.
-template <typename T, int DP, int NT>
-__device__ __forceinline__ void mma_pb(float (&c)[DP / 8][4], const float (&p)[NT][4], uint32_t b, int lane) {
-  constexpr int P = pitch<T, DP>();
-  if constexpr (sizeof(T) == 2) {
-    const int mi = lane >> 3, r8 = lane & 7;
-#pragma unroll
-    for (int n = 0; n < NT; n += 2) {
-      const uint32_t af[4] = {pack2<T>(p[n][0], p[n][1]), pack2<T>(p[n][2], p[n][3]),
-                              pack2<T>(p[n + 1][0], p[n + 1][1]), pack2<T>(p[n + 1][2], p[n + 1][3])};
-#pragma unroll
-      for (int d = 0; d < DP / 8; d += 2) {
-        uint32_t bf[4];
-        ldsm4t(bf, b + (n * 8 + (mi & 1) * 8 + r8) * P + (d * 8 + (mi >> 1) * 8) * 2);
-        mma16(c[d], af, bf[0], bf[1], T());
-        mma16(c[d + 1], af, bf[2], bf[3], T());
-      }
-    }
-  } else {
-    const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      Split4 af;
-      split_tf32(p[n][0], af.hi[0], af.lo[0]);
-      split_tf32(p[n][2], af.hi[1], af.lo[1]);
-      split_tf32(p[n][1], af.hi[2], af.lo[2]);
-      split_tf32(p[n][3], af.hi[3], af.lo[3]);
-      const uint32_t br = b + (n * 8 + 2 * t) * P + g * 4;
-#pragma unroll
-      for (int d = 0; d < DP / 8; ++d) mma8x3(c[d], af, lds_f(br + d * 32), lds_f(br + P + d * 32));
-    }
-  }
-}
-
-// Stages `rows` rows into `dst`; row r comes from src(r), a null source is
-// staged as zeros.  Columns past D are zeros.
-template <typename T, int DP, typename F>
-__device__ __forceinline__ void stage_rows(uint32_t dst, int rows, int D, bool vec, int tid, F src) {
-  constexpr int P = pitch<T, DP>();
-  constexpr int E = 16 / (int)sizeof(T), CH = DP / E;
-  if (vec) {
-    for (int e = tid; e < rows * CH; e += kT) {
-      const int r = e / CH, c = e % CH;
-      const T* s = src(r);
-      const bool on = s != nullptr && c * E < D;
-      cp16(dst + r * P + c * 16, on ? s + c * E : nullptr, on ? 16u : 0u);
-    }
-  } else {
-    for (int e = tid; e < rows * DP; e += kT) {
-      const int r = e / DP, c = e % DP;
-      const T* s = src(r);
-      const T v = (s != nullptr && c < D) ? s[c] : from_f<T>(0.f);
-      if constexpr (sizeof(T) == 4)
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + r * P + c * 4), "f"(v) : "memory");
-      else
-        asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + r * P + c * 2), "h"(*reinterpret_cast<const uint16_t*>(&v))
-                     : "memory");
-    }
-  }
-}
-
 // ------------------------------------------------- forward, many query rows
-// One block: one KV head of one batch entry, 64 rows of the (query head in the
+// One block: one KV head of one batch entry, 64 (fp32: 128) rows of the (query head in the
 // group, query) plane - every warp has 16 of its own - and the key tiles of one
 // split.
+// fp32: 128 rows share a staged tile of 32 keys (one stage: two blocks to an SM
+// cover each other's loads), as the splitting costs what a warp's products do.
+template <typename T> constexpr int kFwdRows = sizeof(T) == 4 ? 128 : kBM;
+template <typename T> constexpr int kFwdKeys = sizeof(T) == 4 ? 32 : kBN;
+template <typename T> constexpr int kFwdStages = sizeof(T) == 4 ? 1 : 2;
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(kT) attn_mma_fwd_kernel(const __grid_constant__ AttnArgs a, int vec_q, int vec_kv) {
+__global__ void __launch_bounds__(kFwdRows<T> * 2, sizeof(T) == 4 && DP <= 64 ? 2 : 1) attn_mma_fwd_kernel(const __grid_constant__ AttnArgs a, int vec_q, int vec_kv) {
   extern __shared__ __align__(16) uint8_t smem[];
-  constexpr int P = pitch<T, DP>();
-  constexpr int NT = kBN / 8;
+  constexpr int P = pitch<DP>(), BN = kFwdKeys<T>, ST = kFwdStages<T>;
+  constexpr int NT = BN / 8, BM = kFwdRows<T>, TH = 2 * BM;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int G = a.Hq / a.Hkv;
   const long long rows = (long long)G * a.Lq;
-  const unsigned ntile = (unsigned)((rows + kBM - 1) / kBM);
+  const unsigned ntile = (unsigned)((rows + BM - 1) / BM);
   const int b = blockIdx.x / ntile / a.Hkv, kh = blockIdx.x / ntile % a.Hkv;
-  const long long r0 = (long long)(blockIdx.x % ntile) * kBM;
+  const long long r0 = (long long)(blockIdx.x % ntile) * BM;
   const uint32_t sm = ptx::smem_u32(smem);
-  const uint32_t sQ = sm, sK = sQ + kBM * P, sV = sK + 2 * kBN * P;
+  constexpr uint32_t TB = tile_bytes<T, DP>(BN);
+  const Rows sQ = {sm, BM * P};
+  const auto kv = [&](int st, int v) { return Rows{sm + (uint32_t)tile_bytes<T, DP>(BM) + (2 * st + v) * TB, BN * P}; };
   const int len = kv_len(a, b);
 
   // the furthest key that a row of this block may meet
   long long kend = len;
   if (a.causal) {
-    const long long last = min(rows, r0 + kBM) - 1;
+    const long long last = min(rows, r0 + BM) - 1;
     const long long imax = (r0 / a.Lq != last / a.Lq) ? a.Lq - 1 : last % a.Lq;
     kend = max(0ll, min(kend, imax + a.q_off + 1));
   }
-  const int tiles = (int)((kend + kBN - 1) / kBN);
+  const int tiles = (int)((kend + BN - 1) / BN);
   const int t0 = (int)((long long)tiles * blockIdx.y / a.nsplit), t1 = (int)((long long)tiles * (blockIdx.y + 1) / a.nsplit);
 
   const T* qb = static_cast<const T*>(a.q) + (int64_t)b * a.qs[0];
   const T* kb = static_cast<const T*>(a.k) + (int64_t)b * a.ks[0] + (int64_t)kh * a.ks[2];
   const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.vs[0] + (int64_t)kh * a.vs[2];
   const uint8_t* mb = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
-  stage_rows<T, DP>(sQ, kBM, a.D, vec_q, tid, [&](int r) -> const T* {
+  stage_rows<T, DP, TH>(sQ, BM, a.D, vec_q, tid, [&](int r) -> const T* {
     const long long x = r0 + r;
     return x < rows ? qb + (x % a.Lq) * a.qs[1] + (kh * G + x / a.Lq) * a.qs[2] : nullptr;
   });
   auto load = [&](int tile, int st) {
-    const int j0 = tile * kBN;
+    const int j0 = tile * BN;
     auto alive = [&](int r) { return j0 + r < len && (!mb || mb[(int64_t)(j0 + r) * a.mask_k]); };
-    stage_rows<T, DP>(sK + st * kBN * P, kBN, a.D, vec_kv, tid,
+    stage_rows<T, DP, TH>(kv(st, 0), BN, a.D, vec_kv, tid,
                       [&](int r) -> const T* { return alive(r) ? kb + (int64_t)(j0 + r) * a.ks[1] : nullptr; });
-    stage_rows<T, DP>(sV + st * kBN * P, kBN, a.D, vec_kv, tid,
+    stage_rows<T, DP, TH>(kv(st, 1), BN, a.D, vec_kv, tid,
                       [&](int r) -> const T* { return alive(r) ? vb + (int64_t)(j0 + r) * a.vs[1] : nullptr; });
     cp_commit();
   };
-  if (t0 < t1) load(t0, 0);
+  if (ST == 2 && t0 < t1) load(t0, 0);
 
   // the two rows of this thread
   const int wr = warp * 16;
@@ -288,8 +385,10 @@ __global__ void __launch_bounds__(kT) attn_mma_fwd_kernel(const __grid_constant_
     for (int x = 0; x < 4; ++x) o[d][x] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   for (int tile = t0; tile < t1; ++tile) {
-    const int st = (tile - t0) & 1;
-    if (tile + 1 < t1) {
+    const int st = ST == 2 ? (tile - t0) & 1 : 0;
+    if (ST == 1) {
+      load(tile, 0);
+    } else if (tile + 1 < t1) {
       load(tile + 1, st ^ 1);
       cp_wait<1>();
     } else {
@@ -301,9 +400,9 @@ __global__ void __launch_bounds__(kT) attn_mma_fwd_kernel(const __grid_constant_
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int x = 0; x < 4; ++x) s[n][x] = 0.f;
-    mma_abt<T, DP, NT>(s, sQ + wr * P, sK + st * kBN * P, lane);
-    const int j0 = tile * kBN;
-    const bool whole = !mb && j0 + kBN <= len && (!a.causal || j0 + kBN <= min(qi[0], qi[1]) + a.q_off + 1);
+    mma_abt<T, DP, NT>(s, Rows{sQ.at + wr * P, sQ.part}, kv(st, 0), lane);
+    const int j0 = tile * BN;
+    const bool whole = !mb && j0 + BN <= len && (!a.causal || j0 + BN <= min(qi[0], qi[1]) + a.q_off + 1);
     float mx[2] = {m[0], m[1]};
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -341,7 +440,7 @@ __global__ void __launch_bounds__(kT) attn_mma_fwd_kernel(const __grid_constant_
       for (int x = 0; x < 4; ++x) o[d][x] *= f[x >> 1];
     m[0] = mx[0];
     m[1] = mx[1];
-    mma_pb<T, DP, NT>(o, s, sV + st * kBN * P, lane);
+    mma_pb<T, DP, NT>(o, s, kv(st, 1), lane);
     __syncthreads();
   }
 #pragma unroll
@@ -392,7 +491,7 @@ constexpr int kCluster = 8;
 // Three stages of 128 16-bit values leave room for two blocks to an SM.
 template <typename T, int DP> constexpr int few_stages() { return DP * sizeof(T) > 256 ? 2 : DP * sizeof(T) > 192 ? 3 : 4; }
 template <typename T, int DP> constexpr size_t few_smem() {
-  return std::max((size_t)4 * few_stages<T, DP>() * 2 * 16 * pitch<T, DP>() + (size_t)16 * pitch<T, DP>(),
+  return std::max((size_t)4 * few_stages<T, DP>() * 2 * 16 * raw_pitch<T, DP>() + (size_t)16 * raw_pitch<T, DP>(),
                   (size_t)(5 * 16 * (DP + 4) + 5 * 32) * 4);
 }
 
@@ -414,7 +513,7 @@ __device__ __forceinline__ void cluster_sync() {
 template <typename T, int DP, bool CLUSTER>
 __global__ void __launch_bounds__(kT) attn_mma_few_kernel(const __grid_constant__ AttnArgs a, int vec_q, int vec_kv) {
   extern __shared__ __align__(16) uint8_t smem[];
-  constexpr int P = pitch<T, DP>(), S = few_stages<T, DP>();
+  constexpr int P = raw_pitch<T, DP>(), S = few_stages<T, DP>();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int G = a.Hq / a.Hkv, rows = G * a.Lq;  // <= 16
   const int b = blockIdx.x / a.Hkv, kh = blockIdx.x % a.Hkv;
@@ -478,9 +577,19 @@ __global__ void __launch_bounds__(kT) attn_mma_few_kernel(const __grid_constant_
     }
     cp_commit();
   };
-  stage_rows<T, DP>(sQ, 16, a.D, vec_q, tid, [&](int r) -> const T* {
-    return r < rows ? qb + (int64_t)(r % a.Lq) * a.qs[1] + (int64_t)(kh * G + r / a.Lq) * a.qs[2] : nullptr;
-  });
+  const auto row_of = [&](int r) { return qb + (int64_t)(r % a.Lq) * a.qs[1] + (int64_t)(kh * G + r / a.Lq) * a.qs[2]; };
+  if (vec_q) {
+    for (int e = tid; e < 16 * CH; e += kT) {
+      const int r = e / CH, c = e % CH;
+      const bool on = r < rows && c * E < a.D;
+      cp16(sQ + r * P + c * 16, on ? row_of(r) + c * E : qb, on ? 16u : 0u);
+    }
+  } else {
+    for (int e = tid; e < 16 * DP; e += kT) {
+      const int r = e / DP, c = e % DP;
+      *(reinterpret_cast<T*>(smem + r * P) + c) = r < rows && c < a.D ? row_of(r)[c] : from_f<T>(0.f);
+    }
+  }
   cp_commit();
 #pragma unroll
   for (int x = 0; x < S - 1; ++x) load(x);
@@ -515,7 +624,7 @@ __global__ void __launch_bounds__(kT) attn_mma_few_kernel(const __grid_constant_
 #pragma unroll
       for (int z = 0; z < 4; ++z) s[c][z] = 0.f;
     if constexpr (sizeof(T) == 2) fq.abt(s, sK, lane);
-    else mma_abt<T, DP, 2>(s, sQ, sK, lane);
+    else tf32_abt<DP>(s, sQ, sK, lane);
     const int j0 = (s0 + warp + 4 * x) * 16;
     const bool whole = !mb && j0 + 16 <= len && (!a.causal || j0 + 16 <= min(qi[0], qi[1]) + a.q_off + 1);
     float mx[2] = {-INFINITY, -INFINITY};
@@ -560,7 +669,8 @@ __global__ void __launch_bounds__(kT) attn_mma_few_kernel(const __grid_constant_
         s[c][z] = exp2_approx(s[c][z] - base[z >> 1]);
         l[z >> 1] += s[c][z];
       }
-    mma_pb<T, DP, 2>(o, s, sV, lane);
+    if constexpr (sizeof(T) == 2) mma_pb<T, DP, 2>(o, s, Rows{sV, 0}, lane);
+    else tf32_pb<DP>(o, s, sV, lane);
     __syncwarp();  // the ring's place is read before it is written again
   }
 #pragma unroll
@@ -702,25 +812,51 @@ __global__ void attn_delta_kernel(const __grid_constant__ AttnArgs a, long long 
   if (lane == 0) a.delta[row] = s;
 }
 
+// The second half's accumulators added to the first's, through shared memory
+// that nobody reads any more; false for the second half, which is done.
+template <int DP>
+__device__ __forceinline__ bool add_halves(float (&acc)[DP / 8][4], float* mem, int warp, int half, int lane) {
+  __syncthreads();
+  float* at = mem + (warp * 32 + lane) * (DP / 2 + 1);
+  if (half)
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) at[d * 4 + x] = acc[d][x];
+  __syncthreads();
+  if (half) return false;
+#pragma unroll
+  for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) acc[d][x] += at[d * 4 + x];
+  return true;
+}
+
 // dQ = scale dS K for 64 queries of one query head, with the sums of dS along
 // the diagonals of every tile when the table's gradient is wanted: thread u
 // adds the entries (y, x) with x - y = u - 63, in the order of the rows; the
 // upper half of a tile's diagonals goes on in the next tile.
-template <typename T, int DP, int BN, bool DELTA>
-__global__ void __launch_bounds__(kT) attn_mma_dq_kernel(const __grid_constant__ AttnArgs a, int vec_q, int vec_kv,
+//
+// KS = 2 (fp32, whose blocks are few and long): eight warps, two to 16 rows, each
+// half of a tile's keys; their sums are added at the end.
+template <typename T, int DP, int BN, int KS, bool DELTA>
+__global__ void __launch_bounds__(kT * KS) attn_mma_dq_kernel(const __grid_constant__ AttnArgs a, int vec_q, int vec_kv,
                                                          int vec_do) {
   extern __shared__ __align__(16) uint8_t smem[];
-  constexpr int P = pitch<T, DP>();
-  constexpr int NT = BN / 8;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  constexpr int P = pitch<DP>(), TH = kT * KS;
+  constexpr int NT = BN / 8 / KS;
+  constexpr int ST = sizeof(T) == 4 ? 1 : 2;
+  const int tid = threadIdx.x, warp = (tid >> 5) & 3, key0 = (tid >> 7) * NT * 8, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int G = a.Hq / a.Hkv;
   const unsigned ntile = (unsigned)((a.Lq + kBM - 1) / kBM);
   const int b = blockIdx.x / ntile / a.Hq, h = blockIdx.x / ntile % a.Hq, kh = h / G;
   const long long i0 = (long long)(blockIdx.x % ntile) * kBM;
   const uint32_t sm = ptx::smem_u32(smem);
-  const uint32_t sQ = sm, sO = sQ + kBM * P, sK = sO + kBM * P, sV = sK + 2 * BN * P;
+  constexpr uint32_t TM = tile_bytes<T, DP>(kBM), TB = tile_bytes<T, DP>(BN);
+  const Rows sQ = {sm, kBM * P}, sO = {sm + TM, kBM * P};
+  const auto kv = [&](int st, int v) { return Rows{sm + 2 * TM + (2 * st + v) * TB, BN * P}; };
   constexpr int SL = BN + 1;
-  float* sD = reinterpret_cast<float*>(smem + 2 * kBM * P + 4 * BN * P);  // dS tile [64][BN + 1], carry behind
+  float* sD = reinterpret_cast<float*>(smem + 2 * TM + 2 * ST * TB);  // dS tile [64][BN + 1], carry behind
   float* carry = sD + kBM * SL;
   const int len = kv_len(a, b);
   long long kend = len;
@@ -731,20 +867,20 @@ __global__ void __launch_bounds__(kT) attn_mma_dq_kernel(const __grid_constant__
   const T* kb = static_cast<const T*>(a.k) + (int64_t)b * a.ks[0] + (int64_t)kh * a.ks[2];
   const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.vs[0] + (int64_t)kh * a.vs[2];
   const uint8_t* mb = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
-  stage_rows<T, DP>(sQ, kBM, a.D, vec_q, tid,
+  stage_rows<T, DP, TH>(sQ, kBM, a.D, vec_q, tid,
                     [&](int r) -> const T* { return i0 + r < a.Lq ? qb + (i0 + r) * a.qs[1] : nullptr; });
-  stage_rows<T, DP>(sO, kBM, a.D, vec_do, tid,
+  stage_rows<T, DP, TH>(sO, kBM, a.D, vec_do, tid,
                     [&](int r) -> const T* { return i0 + r < a.Lq ? ob + (i0 + r) * a.dos[1] : nullptr; });
   auto load = [&](int tile, int st) {
     const int j0 = tile * BN;
     auto alive = [&](int r) { return j0 + r < len && (!mb || mb[(int64_t)(j0 + r) * a.mask_k]); };
-    stage_rows<T, DP>(sK + st * BN * P, BN, a.D, vec_kv, tid,
+    stage_rows<T, DP, TH>(kv(st, 0), BN, a.D, vec_kv, tid,
                       [&](int r) -> const T* { return alive(r) ? kb + (int64_t)(j0 + r) * a.ks[1] : nullptr; });
-    stage_rows<T, DP>(sV + st * BN * P, BN, a.D, vec_kv, tid,
+    stage_rows<T, DP, TH>(kv(st, 1), BN, a.D, vec_kv, tid,
                       [&](int r) -> const T* { return alive(r) ? vb + (int64_t)(j0 + r) * a.vs[1] : nullptr; });
     cp_commit();
   };
-  if (tiles > 0) load(0, 0);
+  if (ST == 2 && tiles > 0) load(0, 0);
   long long qi[2];
   float lse2[2], delta[2];
   const float* bias[2];
@@ -767,8 +903,10 @@ __global__ void __launch_bounds__(kT) attn_mma_dq_kernel(const __grid_constant__
   float* dws = a.dws && !DELTA ? a.dws + (long long)blockIdx.x * a.dws_ld : nullptr;
   if (dws && tid < kBM) carry[tid] = 0.f;
   for (int tile = 0; tile < tiles; ++tile) {
-    const int st = tile & 1;
-    if (tile + 1 < tiles) {
+    const int st = ST == 2 ? tile & 1 : 0;
+    if (ST == 1) {
+      load(tile, 0);
+    } else if (tile + 1 < tiles) {
       load(tile + 1, st ^ 1);
       cp_wait<1>();
     } else {
@@ -780,34 +918,35 @@ __global__ void __launch_bounds__(kT) attn_mma_dq_kernel(const __grid_constant__
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int x = 0; x < 4; ++x) s[n][x] = dp[n][x] = 0.f;
-    mma_abt<T, DP, NT>(s, sQ + warp * 16 * P, sK + st * BN * P, lane);
-    mma_abt<T, DP, NT>(dp, sO + warp * 16 * P, sV + st * BN * P, lane);
+    const Rows k = {kv(st, 0).at + key0 * P, BN * P}, v = {kv(st, 1).at + key0 * P, BN * P};
+    mma_abt<T, DP, NT>(s, Rows{sQ.at + warp * 16 * P, sQ.part}, k, lane);
+    mma_abt<T, DP, NT>(dp, Rows{sO.at + warp * 16 * P, sO.part}, v, lane);
     const int j0 = tile * BN;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const int j = j0 + n * 8 + 2 * t + (x & 1), y = x >> 1;
-        float v = s[n][x] * sc;
-        if (a.diag && j < a.Lk) v += __ldg(bias[y] + j);
+        const int j = j0 + key0 + n * 8 + 2 * t + (x & 1), y = x >> 1;
+        float z = s[n][x] * sc;
+        if (a.diag && j < a.Lk) z += __ldg(bias[y] + j);
         const bool on = j < len && (!mb || mb[(int64_t)j * a.mask_k]) && (!a.causal || j <= qi[y] + a.q_off);
-        const float p = on ? exp2_approx(v - lse2[y]) : 0.f;
+        const float p = on ? exp2_approx(z - lse2[y]) : 0.f;
         s[n][x] = p != 0.f ? p * (dp[n][x] - (DELTA ? 0.f : delta[y])) : 0.f;
         if (DELTA) delta[y] += s[n][x];
-        if (dws) sD[(warp * 16 + g + 8 * y) * SL + n * 8 + 2 * t + (x & 1)] = s[n][x];
+        if (dws) sD[(warp * 16 + g + 8 * y) * SL + key0 + n * 8 + 2 * t + (x & 1)] = s[n][x];
       }
-    if (!DELTA) mma_pb<T, DP, NT>(acc, s, sK + st * BN * P, lane);
+    if (!DELTA) mma_pb<T, DP, NT>(acc, s, k, lane);
     __syncthreads();
     if (dws) {  // diagonals u = x - y + 63 of this tile, 0 <= u < 63 + BN
       const int u = tid;
-      float v = u < kBM - 1 ? carry[u] : 0.f;
+      float z = u < kBM - 1 ? carry[u] : 0.f;
       if (u < kBM - 1 + BN) {
         const int d = u - (kBM - 1);
-        for (int y = max(0, -d); y < min(kBM, BN - d); ++y) v += sD[y * SL + y + d];
-        if (u < BN) dws[(long long)tile * BN + u] = v;
+        for (int y = max(0, -d); y < min(kBM, BN - d); ++y) z += sD[y * SL + y + d];
+        if (u < BN) dws[(long long)tile * BN + u] = z;
       }
       __syncthreads();
-      if (u >= BN && u < kBM - 1 + BN) carry[u - BN] = v;
+      if (u >= BN && u < kBM - 1 + BN) carry[u - BN] = z;
       __syncthreads();
     }
   }
@@ -823,7 +962,10 @@ __global__ void __launch_bounds__(kT) attn_mma_dq_kernel(const __grid_constant__
   }
   if (dws) {  // the last diagonals, and zeros where no tile was
     const long long at = (long long)tiles * BN;
-    for (long long x = at + tid; x < a.dws_ld; x += kT) dws[x] = x - at < kBM - 1 ? carry[x - at] : 0.f;
+    for (long long x = at + tid; x < a.dws_ld; x += TH) dws[x] = x - at < kBM - 1 ? carry[x - at] : 0.f;
+  }
+  if constexpr (KS == 2) {
+    if (!add_halves<DP>(acc, reinterpret_cast<float*>(smem), warp, tid >> 7, lane)) return;
   }
 #pragma unroll
   for (int y = 0; y < 2; ++y) {
@@ -840,20 +982,24 @@ __global__ void __launch_bounds__(kT) attn_mma_dq_kernel(const __grid_constant__
 
 // dK = scale sum dS^T Q and dV = sum P^T dO for 64 keys of one KV head, over
 // every query of every head of its group, BQ rows at a time.
-template <typename T, int DP, int BQ>
-__global__ void __launch_bounds__(kT) attn_mma_dkv_kernel(const __grid_constant__ AttnArgs a, int vec_q, int vec_kv,
+// KS as above, over the rows.
+template <typename T, int DP, int BQ, int KS>
+__global__ void __launch_bounds__(kT * KS) attn_mma_dkv_kernel(const __grid_constant__ AttnArgs a, int vec_q, int vec_kv,
                                                           int vec_do) {
   extern __shared__ __align__(16) uint8_t smem[];
-  constexpr int P = pitch<T, DP>();
-  constexpr int NT = BQ / 8;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  constexpr int P = pitch<DP>(), TH = kT * KS;
+  constexpr int NT = BQ / 8 / KS;
+  constexpr int ST = sizeof(T) == 4 ? 1 : 2;
+  const int tid = threadIdx.x, warp = (tid >> 5) & 3, row0 = (tid >> 7) * NT * 8, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int G = a.Hq / a.Hkv;
   const unsigned ntile = (unsigned)((a.Lk + kBN - 1) / kBN);
   const int b = blockIdx.x / ntile / a.Hkv, kh = blockIdx.x / ntile % a.Hkv;
   const int j0 = (int)(blockIdx.x % ntile) * kBN;
   const uint32_t sm = ptx::smem_u32(smem);
-  const uint32_t sK = sm, sV = sK + kBN * P, sQ = sV + kBN * P, sO = sQ + 2 * BQ * P;
-  float* stat = reinterpret_cast<float*>(smem + 2 * kBN * P + 4 * BQ * P);  // [2][2][BQ]: lse2, delta
+  constexpr uint32_t TM = tile_bytes<T, DP>(kBN), TB = tile_bytes<T, DP>(BQ);
+  const Rows sK = {sm, kBN * P}, sV = {sm + TM, kBN * P};
+  const auto qo = [&](int st, int o) { return Rows{sm + 2 * TM + (2 * st + o) * TB, BQ * P}; };
+  float* stat = reinterpret_cast<float*>(smem + 2 * TM + 2 * ST * TB);  // [stages][2][BQ]: lse2, delta
   const int len = kv_len(a, b);
   const T* qb = static_cast<const T*>(a.q) + (int64_t)b * a.qs[0];
   const T* ob = static_cast<const T*>(a.dout) + (int64_t)b * a.dos[0];
@@ -861,9 +1007,9 @@ __global__ void __launch_bounds__(kT) attn_mma_dkv_kernel(const __grid_constant_
   const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.vs[0] + (int64_t)kh * a.vs[2];
   const uint8_t* mb = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
   auto alive = [&](int j) { return j < len && (!mb || mb[(int64_t)j * a.mask_k]); };
-  stage_rows<T, DP>(sK, kBN, a.D, vec_kv, tid,
+  stage_rows<T, DP, TH>(sK, kBN, a.D, vec_kv, tid,
                     [&](int r) -> const T* { return alive(j0 + r) ? kb + (int64_t)(j0 + r) * a.ks[1] : nullptr; });
-  stage_rows<T, DP>(sV, kBN, a.D, vec_kv, tid,
+  stage_rows<T, DP, TH>(sV, kBN, a.D, vec_kv, tid,
                     [&](int r) -> const T* { return alive(j0 + r) ? vb + (int64_t)(j0 + r) * a.vs[1] : nullptr; });
   // rows of one head at a time, so a tile never holds two heads; with a causal
   // mask only queries with i + q_off >= j0 meet these keys
@@ -874,10 +1020,10 @@ __global__ void __launch_bounds__(kT) attn_mma_dkv_kernel(const __grid_constant_
   auto load = [&](long long tile, int st) {
     const int h = kh * G + (int)(tile / per);
     const long long i0 = ifirst + (tile % per) * BQ;
-    stage_rows<T, DP>(sQ + st * BQ * P, BQ, a.D, vec_q, tid, [&](int r) -> const T* {
+    stage_rows<T, DP, TH>(qo(st, 0), BQ, a.D, vec_q, tid, [&](int r) -> const T* {
       return i0 + r < a.Lq ? qb + (i0 + r) * a.qs[1] + (int64_t)h * a.qs[2] : nullptr;
     });
-    stage_rows<T, DP>(sO + st * BQ * P, BQ, a.D, vec_do, tid, [&](int r) -> const T* {
+    stage_rows<T, DP, TH>(qo(st, 1), BQ, a.D, vec_do, tid, [&](int r) -> const T* {
       return i0 + r < a.Lq ? ob + (i0 + r) * a.dos[1] + (int64_t)h * a.dos[2] : nullptr;
     });
     if (tid < BQ) {
@@ -889,7 +1035,7 @@ __global__ void __launch_bounds__(kT) attn_mma_dkv_kernel(const __grid_constant_
     }
     cp_commit();
   };
-  if (tiles > 0) load(0, 0);
+  if (ST == 2 && tiles > 0) load(0, 0);
   int key[2];
   bool on[2];
 #pragma unroll
@@ -904,8 +1050,10 @@ __global__ void __launch_bounds__(kT) attn_mma_dkv_kernel(const __grid_constant_
 #pragma unroll
     for (int x = 0; x < 4; ++x) dk[d][x] = dv[d][x] = 0.f;
   for (long long tile = 0; tile < tiles; ++tile) {
-    const int st = (int)(tile & 1);
-    if (tile + 1 < tiles) {
+    const int st = ST == 2 ? (int)(tile & 1) : 0;
+    if (ST == 1) {
+      load(tile, 0);
+    } else if (tile + 1 < tiles) {
       load(tile + 1, st ^ 1);
       cp_wait<1>();
     } else {
@@ -920,29 +1068,34 @@ __global__ void __launch_bounds__(kT) attn_mma_dkv_kernel(const __grid_constant_
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int x = 0; x < 4; ++x) s[n][x] = dp[n][x] = 0.f;
-    mma_abt<T, DP, NT>(s, sK + warp * 16 * P, sQ + st * BQ * P, lane);
+    const Rows q = {qo(st, 0).at + row0 * P, BQ * P}, o = {qo(st, 1).at + row0 * P, BQ * P};
+    mma_abt<T, DP, NT>(s, Rows{sK.at + warp * 16 * P, sK.part}, q, lane);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const int c = n * 8 + 2 * t + (x & 1), y = x >> 1;
+        const int c = row0 + n * 8 + 2 * t + (x & 1), y = x >> 1;
         const long long i = i0 + c;
         float v = s[n][x] * sc;
         if (bias && i < a.Lq && key[y] < a.Lk) v += __ldg(bias + key[y] - i);
         const bool live = on[y] && (!a.causal || key[y] <= i + a.q_off);
         s[n][x] = live ? exp2_approx(v - stat[st * 2 * BQ + c]) : 0.f;
       }
-    mma_pb<T, DP, NT>(dv, s, sO + st * BQ * P, lane);
-    mma_abt<T, DP, NT>(dp, sV + warp * 16 * P, sO + st * BQ * P, lane);
+    mma_pb<T, DP, NT>(dv, s, o, lane);
+    mma_abt<T, DP, NT>(dp, Rows{sV.at + warp * 16 * P, sV.part}, o, lane);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const float de = stat[(st * 2 + 1) * BQ + n * 8 + 2 * t + (x & 1)];
+        const float de = stat[(st * 2 + 1) * BQ + row0 + n * 8 + 2 * t + (x & 1)];
         s[n][x] = s[n][x] != 0.f ? s[n][x] * (dp[n][x] - de) : 0.f;
       }
-    mma_pb<T, DP, NT>(dk, s, sQ + st * BQ * P, lane);
+    mma_pb<T, DP, NT>(dk, s, q, lane);
     __syncthreads();
+  }
+  if constexpr (KS == 2) {
+    const bool on1 = add_halves<DP>(dk, reinterpret_cast<float*>(smem), warp, tid >> 7, lane);
+    if (!add_halves<DP>(dv, reinterpret_cast<float*>(smem), warp, tid >> 7, lane) || !on1) return;
   }
 #pragma unroll
   for (int y = 0; y < 2; ++y) {
@@ -1010,10 +1163,11 @@ void fwd_dp(const AttnArgs& a, cudaStream_t st) {
   } else {
     const int vq = aligned16(a, a.q, a.qs), vkv = aligned16(a, a.k, a.ks) && aligned16(a, a.v, a.vs);
     const long long rows = (long long)(a.Hq / a.Hkv) * a.Lq;
-    const size_t smem = (size_t)(kBM + 4 * kBN) * pitch<T, DP>();
-    const dim3 grid((unsigned)((rows + kBM - 1) / kBM * a.B * a.Hkv), a.nsplit);
+    constexpr size_t smem = tile_bytes<T, DP>(kFwdRows<T>) + 2 * kFwdStages<T> * tile_bytes<T, DP>(kFwdKeys<T>);
+    constexpr int BM = kFwdRows<T>;
+    const dim3 grid((unsigned)((rows + BM - 1) / BM * a.B * a.Hkv), a.nsplit);
     allow_smem<attn_mma_fwd_kernel<T, DP>>(smem);
-    attn_mma_fwd_kernel<T, DP><<<grid, kT, smem, st>>>(a, vq, vkv);
+    attn_mma_fwd_kernel<T, DP><<<grid, 2 * BM, smem, st>>>(a, vq, vkv);
     note_launch();
     RVC_CUDA_TRY(cudaGetLastError());
   }
@@ -1029,31 +1183,32 @@ template <typename T, int DP>
 void bwd_dp(const AttnArgs& a, cudaStream_t st) {
   const int vq = aligned16(a, a.q, a.qs), vkv = aligned16(a, a.k, a.ks) && aligned16(a, a.v, a.vs),
             vdo = aligned16(a, a.dout, a.dos);
-  constexpr int P = pitch<T, DP>();
-  constexpr int BN = sizeof(T) == 4 && DP > 64 ? 32 : 64;  // fp32 rows of 96 / 128: half the tile, to fit shared memory
+  // fp32: tiles of 32 rows in one stage, eight warps to a block
+  constexpr int BN = sizeof(T) == 4 ? 32 : 64, KS = sizeof(T) == 4 ? 2 : 1, ST = sizeof(T) == 4 ? 1 : 2;
+  constexpr size_t tiles = 2 * tile_bytes<T, DP>(kBM) + 2 * ST * tile_bytes<T, DP>(BN);
+  constexpr size_t halves = KS == 2 ? (size_t)128 * (DP / 2 + 1) * 4 : 0;
   const long long n = (long long)a.B * a.Hq * a.Lq;
   if (n > 0) {
-    const size_t smem = (size_t)(2 * kBM + 4 * BN) * P + (a.dws ? (size_t)(kBM * (BN + 1) + kBM) * 4 : 0);
+    const size_t smem = std::max(halves, tiles + (a.dws ? (size_t)(kBM * (BN + 1) + kBM) * 4 : 0));
+    const unsigned grid = (unsigned)((a.Lq + kBM - 1ll) / kBM * a.B * a.Hq);
     if constexpr (sizeof(T) == 4) {
       attn_delta_kernel<<<(unsigned)((n + 7) / 8), 256, 0, st>>>(a, n);
     } else {
-      allow_smem<attn_mma_dq_kernel<T, DP, BN, true>>(smem);
-      attn_mma_dq_kernel<T, DP, BN, true>
-          <<<(unsigned)((a.Lq + kBM - 1ll) / kBM * a.B * a.Hq), kT, smem, st>>>(a, vq, vkv, vdo);
+      allow_smem<attn_mma_dq_kernel<T, DP, BN, KS, true>>(smem);
+      attn_mma_dq_kernel<T, DP, BN, KS, true><<<grid, kT * KS, smem, st>>>(a, vq, vkv, vdo);
     }
     note_launch();
     RVC_CUDA_TRY(cudaGetLastError());
-    allow_smem<attn_mma_dq_kernel<T, DP, BN, false>>(smem);
-    attn_mma_dq_kernel<T, DP, BN, false>
-        <<<(unsigned)((a.Lq + kBM - 1ll) / kBM * a.B * a.Hq), kT, smem, st>>>(a, vq, vkv, vdo);
+    allow_smem<attn_mma_dq_kernel<T, DP, BN, KS, false>>(smem);
+    attn_mma_dq_kernel<T, DP, BN, KS, false><<<grid, kT * KS, smem, st>>>(a, vq, vkv, vdo);
     note_launch();
     RVC_CUDA_TRY(cudaGetLastError());
   }
   if (a.Lk > 0) {
-    const size_t smem = (size_t)(2 * kBN + 4 * BN) * P + 4 * BN * 4;
-    allow_smem<attn_mma_dkv_kernel<T, DP, BN>>(smem);
-    attn_mma_dkv_kernel<T, DP, BN>
-        <<<(unsigned)((a.Lk + kBN - 1ll) / kBN * a.B * a.Hkv), kT, smem, st>>>(a, vq, vkv, vdo);
+    constexpr size_t smem = std::max(halves, tiles + (size_t)2 * ST * BN * 4);
+    allow_smem<attn_mma_dkv_kernel<T, DP, BN, KS>>(smem);
+    attn_mma_dkv_kernel<T, DP, BN, KS>
+        <<<(unsigned)((a.Lk + kBN - 1ll) / kBN * a.B * a.Hkv), kT * KS, smem, st>>>(a, vq, vkv, vdo);
     note_launch();
     RVC_CUDA_TRY(cudaGetLastError());
   }
@@ -1096,7 +1251,8 @@ int attn_mma_splits(const AttnArgs& a, int sms, bool* workspace) {
     while (p < n && p < kCluster) p *= 2;
     return p;
   }
-  const long long blocks = (rows + kBM - 1) / kBM * a.B * a.Hkv;
+  const int BM = a.type == kF32 ? kFwdRows<float> : kBM;
+  const long long blocks = (rows + BM - 1) / BM * a.B * a.Hkv;
   const int tiles = (a.Lk + kBN - 1) / kBN;
   const long long want = (2ll * sms + blocks - 1) / blocks;
   const int n = (int)std::max(1ll, std::min({want, (long long)(tiles / 2), 64ll}));
