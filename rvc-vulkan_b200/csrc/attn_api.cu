@@ -93,7 +93,7 @@ __global__ void bucket_sums_kernel(const double* __restrict__ sums, const double
 }
 
 struct Layout {
-  int64_t diag = -1, po = -1, pml = -1, delta = -1, lse2 = -1, dws = -1, sums = -1, far = -1, bytes = 0;
+  int64_t diag = -1, po = -1, pml = -1, delta = -1, lse2 = -1, dws = -1, sums = -1, far = -1, split = -1, bytes = 0;
   int nsplit = 1, BM = 64, nt = 0;
   int64_t diag_ld = 0, diag0 = 0, dws_ld = 0, row_ld = 0;
   bool tc = false;
@@ -117,6 +117,7 @@ Layout plan(const AttnArgs& a, bool bias, bool backward, int sms, bool tc) {
   if (!backward) {
     bool parts = false;
     if (!tc) l.nsplit = attn_mma_splits(a, sms, &parts);
+    else if (a.type == kF32) l.split = take(attn_tc_f32_workspace(a));
     if (parts) {
       l.po = take(4 * rows * a.D * l.nsplit);
       l.pml = take(8 * rows * l.nsplit);
@@ -138,7 +139,7 @@ Layout plan(const AttnArgs& a, bool bias, bool backward, int sms, bool tc) {
   return l;
 }
 
-bool use_tc(const AttnArgs& a, bool backward) { return backward ? attn_tc_bwd_fits(a) : attn_tc_fits(a); }
+bool use_tc(const AttnArgs& a, bool backward) { return backward ? attn_tc_bwd_fits(a) : attn_tc_fits(a) || attn_tc_f32_fits(a); }
 
 template <typename P>
 P* at(void* ws, int64_t off) {
@@ -205,7 +206,9 @@ void attn_forward(AttnArgs a, const void* table, const BucketRule* rule, void* w
     a.far_both = rule->both;
     attn_expand_bias(a, table, *rule, const_cast<float*>(a.diag), st);
   }
-  if (l.tc)
+  if (l.tc && a.type == kF32)
+    attn_tc_f32_forward(a, at<char>(ws, l.split), sms, st);
+  else if (l.tc)
     attn_tc_forward(a, st);
   else
     attn_mma_forward(a, st);

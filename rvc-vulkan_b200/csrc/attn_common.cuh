@@ -136,6 +136,11 @@ int attn_mma_splits(const AttnArgs& a, int sms, bool* workspace);
 // kernels of attn_tc.cu (16-bit types, rows aligned to 16 bytes, many queries)
 bool attn_tc_fits(const AttnArgs& a);
 void attn_tc_forward(const AttnArgs& a, cudaStream_t st);
+// kernels of attn_tc_f32.cu (fp32, heads of up to 64 values, many queries)
+bool attn_tc_f32_fits(const AttnArgs& a);
+int64_t attn_tc_f32_workspace(const AttnArgs& a);
+void attn_tc_f32_forward(const AttnArgs& a, void* ws, int sms, cudaStream_t st);
+// kernels of attn_tc_bwd.cu (as attn_tc.cu)
 bool attn_tc_bwd_fits(const AttnArgs& a);
 int attn_tc_bwd_arrays(const AttnArgs& a);  // arrays of diagonal sums to a tile of keys
 void attn_tc_backward(const AttnArgs& a, cudaStream_t st);
