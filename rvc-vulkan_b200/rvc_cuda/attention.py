@@ -41,6 +41,7 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # torch's own short way to the current stream's handle, a microsecond less than the public one
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda i: torch.cuda.current_stream(i).cuda_stream)
+_POSITION_BITS = {torch.int32: 32, torch.int64: 64}
 MAX_HEAD_DIM = 128
 MAX_BUCKETS = 1024
 
@@ -137,7 +138,7 @@ def _scratch(fn, ctx, desc, n, like, *how):
     need = C.c_int64(0)
     check(fn(ctx, desc, n, *how, need))
     nbytes = need.value
-    return (torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None), nbytes
+    return (like.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None), nbytes
 
 
 def _ptr(x):
@@ -145,6 +146,16 @@ def _ptr(x):
 
 
 def _qkv(q, k, v):
+    try:  # the ordinary call in few steps; what is not ordinary is looked at one by one below
+        B, Lq, Hq, D = q.shape
+        Bk, Lk, Hkv, Dk = k.shape
+        t, i = q.dtype, q.get_device()
+        if (Bk == B and Dk == D and v.shape == k.shape and k.dtype is t and v.dtype is t and t in _TYPES
+                and k.get_device() == i and v.get_device() == i and 1 <= D <= MAX_HEAD_DIM and Hkv and Hq
+                and Hq % Hkv == 0 and q.stride(3) == 1 and k.stride(3) == 1 and v.stride(3) == 1):
+            return q, k, v, B, Lq, Lk, Hq, Hkv, D
+    except (AttributeError, ValueError):
+        pass
     q = _tensor(q, "q", 4)
     k, v = _tensor(k, "k", 4, q), _tensor(v, "v", 4, q)
     B, Lq, Hq, D = q.shape
@@ -218,19 +229,25 @@ def attention(q, k, v, *, kv_lens=None, key_mask=None, scale: Optional[float] = 
     (the parts of a packed projection are taken where they lie).
     """
     q, k, v, B, Lq, Lk, Hq, Hkv, D = _qkv(q, k, v)
-    lens, bits = _lens(kv_lens, B, q)
-    mask, mb, mk = _mask(key_mask, B, Lk, q)
-    table, nb, both, borders, nborders = _table(bias, Hq, q)
+    lens = mask = table = borders = None
+    bits = mb = mk = nb = both = nborders = 0
+    if kv_lens is not None:
+        lens, bits = _lens(kv_lens, B, q)
+    if key_mask is not None:
+        mask, mb, mk = _mask(key_mask, B, Lk, q)
+    if bias is not None:
+        table, nb, both, borders, nborders = _table(bias, Hq, q)
     ctx, stream = _where(q)
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     desc = _pack29(_TYPES[q.dtype], B, Hq, Hkv, Lq, Lk, D, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1],
                    vs[2], bits, mb, mk, bool(causal), q_offset, nb, both, 0, 0, 0, 0, 0, 0)
+    scale = _scale(scale, D)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device)
+    lse = q.new_empty((B, Hq, Lq), dtype=torch.float32)
     ws, nbytes = _scratch(lib.rvc_cuda_attention_workspace, ctx, desc, 29, q, 0)
-    check(lib.rvc_cuda_attention_device(ctx, stream, desc, 29, _scale(scale, D), q.data_ptr(), k.data_ptr(),
-                                        v.data_ptr(), _ptr(lens), _ptr(mask), _ptr(table), borders, nborders,
-                                        out.data_ptr(), lse.data_ptr(), _ptr(ws), nbytes))
+    check(lib.rvc_cuda_attention_device(ctx, stream, desc, 29, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                        _ptr(lens), _ptr(mask), _ptr(table), borders, nborders, out.data_ptr(),
+                                        lse.data_ptr(), _ptr(ws), nbytes))
     return out, lse
 
 
@@ -261,7 +278,7 @@ def attention_backward(dout, q, k, v, out, lse, *, kv_lens=None, key_mask=None, 
     desc = _pack29(_TYPES[q.dtype], B, Hq, Hkv, Lq, Lk, D, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], bits, mb,
                    mk, bool(causal), q_offset, nb, both, *dout.stride()[:3], *out.stride()[:3])
     dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
-    dtable = torch.empty((nb, Hq), dtype=q.dtype, device=q.device) if nb else None
+    dtable = q.new_empty((nb, Hq)) if nb else None
     ws, nbytes = _scratch(lib.rvc_cuda_attention_workspace, ctx, desc, 29, q, 1)
     check(lib.rvc_cuda_attention_backward_device(
         ctx, stream, desc, 29, _scale(scale, D), dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
@@ -283,7 +300,7 @@ def relative_bias(bias: BucketBias, Lq: int, Lk: int, *, q_offset: int = 0):
     if Lq < 0 or Lk < 0:
         raise ValueError(f"relative_bias: lengths {Lq} and {Lk}")
     ctx, stream = _where(t)
-    out = torch.empty((H, Lq, Lk), dtype=t.dtype, device=t.device)
+    out = t.new_empty((H, Lq, Lk))
     desc = _pack11(_TYPES[t.dtype], 1, H, Lq, Lk, q_offset, bias.num_buckets, bias.bidirectional, 0, 0, 0)
     check(lib.rvc_cuda_relative_bias_device(ctx, stream, desc, 11, t.data_ptr(), bias._borders, bias._nborders,
                                             out.data_ptr()))
@@ -307,7 +324,7 @@ def relative_bias_backward(bias: BucketBias, dbias, *, q_offset: int = 0):
         raise ValueError(f"relative_bias_backward: {H} heads, the table has {bias.table.shape[1]}")
     ctx, stream = _where(d)
     desc = _pack11(_TYPES[d.dtype], B, H, Lq, Lk, q_offset, bias.num_buckets, bias.bidirectional, *d.stride()[:3])
-    dtable = torch.empty((bias.num_buckets, H), dtype=d.dtype, device=d.device)
+    dtable = d.new_empty((bias.num_buckets, H))
     ws, nbytes = _scratch(lib.rvc_cuda_relative_bias_workspace, ctx, desc, 11, d)
     check(lib.rvc_cuda_relative_bias_backward_device(ctx, stream, desc, 11, d.data_ptr(), bias._borders,
                                                      bias._nborders, dtable.data_ptr(), _ptr(ws), nbytes))
@@ -330,6 +347,24 @@ def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0, devic
 
 
 def _rope(q, k, q_weight, k_weight, cos, sin, positions, interleaved, name):
+    try:  # the ordinary call in few steps; what is not ordinary is looked at one by one below
+        B, L, Hq, D = q.shape
+        Bk, Lk, Hk, Dk = k.shape
+        P, half = cos.shape
+        t, tw, i = q.dtype, q_weight.dtype, q.get_device()
+        if (Bk == B and Lk == L and Dk == D and k.dtype is t and t in _TYPES and 2 <= D <= 256 and D % 2 == 0
+                and (tw is torch.float32 or tw is t) and k_weight.dtype is tw and q_weight.shape == (D,)
+                and k_weight.shape == (D,) and sin.shape == cos.shape and 2 * half <= D and q_weight.is_contiguous()
+                and k_weight.is_contiguous() and cos.is_contiguous() and sin.is_contiguous()
+                and cos.dtype is torch.float32 and sin.dtype is torch.float32 and q.stride(3) == 1 and k.stride(3) == 1
+                and k.get_device() == q_weight.get_device() == k_weight.get_device() == cos.get_device()
+                == sin.get_device() == positions.get_device() == i and positions.shape == (B, L)
+                and positions.dtype in _POSITION_BITS and B * L):
+            return q, k, q_weight, k_weight, cos, sin, positions, (
+                _TYPES[t], _TYPES[tw], B, L, Hq, Hk, D, 2 * half, P, bool(interleaved),
+                _POSITION_BITS[positions.dtype], *positions.stride(), *q.stride()[:3], *k.stride()[:3])
+    except (AttributeError, ValueError):
+        pass
     q = _tensor(q, "q", 4)
     k = _tensor(k, "k", 4, q)
     B, L, Hq, D = q.shape
@@ -359,12 +394,9 @@ def _rope(q, k, q_weight, k_weight, cos, sin, positions, interleaved, name):
             pl = positions.stride(0)
         else:
             raise ValueError(f"{name}: positions [{B}, {L}] or [{L}] expected, got {tuple(positions.shape)}")
-        if positions.dtype is torch.int64:
-            bits = 64
-        elif positions.dtype is torch.int32:
-            bits = 32
-        else:
+        if positions.dtype not in _POSITION_BITS:
             raise ValueError(f"{name}: positions are int32 or int64, got {positions.dtype}")
+        bits = _POSITION_BITS[positions.dtype]
     elif L > cos.shape[0] and cos.shape[1]:
         raise ValueError(f"{name}: the tables hold {cos.shape[0]} positions, fewer than the {L} rows")
     if B * L == 0:
