@@ -117,7 +117,8 @@ Layout plan(const AttnArgs& a, bool bias, bool backward, int sms, bool tc) {
   if (!backward) {
     bool parts = false;
     if (!tc) l.nsplit = attn_mma_splits(a, sms, &parts);
-    else if (a.type == kF32) l.split = take(attn_tc_f32_workspace(a));
+    else parts = (l.nsplit = attn_tc_splits(a, sms)) > 1;
+    if (tc && a.type == kF32) l.split = take(attn_tc_f32_workspace(a));
     if (parts) {
       l.po = take(4 * rows * a.D * l.nsplit);
       l.pml = take(8 * rows * l.nsplit);

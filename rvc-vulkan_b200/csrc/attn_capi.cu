@@ -79,7 +79,7 @@ AttnArgs attn_args(const int64_t* d, int32_t n, const char* who) {
   a.causal = d[19] != 0;
   RVC_CHECK_ARG(d[20] >= -2 * kMaxLen && d[20] <= 2 * kMaxLen, w + ": q_offset out of range");
   a.q_off = d[20];
-  RVC_CHECK_ARG(d[21] >= 0, w + ": negative number of buckets");
+  RVC_CHECK_ARG(d[21] >= 0 && (d[21] == 0 || d[2] <= 65535), w + ": buckets or heads of the bias out of range");
   return a;
 }
 

@@ -131,10 +131,13 @@ void attn_expand_bias(const AttnArgs& a, const void* table, const BucketRule& ru
 // kernels of attn_mma.cu (every type, stride and size)
 void attn_mma_forward(const AttnArgs& a, cudaStream_t st);
 void attn_mma_backward(const AttnArgs& a, cudaStream_t st);
+// joins the splits of the rows in a.po, a.pml (nothing to do without them)
+void attn_join(const AttnArgs& a, cudaStream_t st);
 int attn_mma_splits(const AttnArgs& a, int sms, bool* workspace);
 
 // kernels of attn_tc.cu (16-bit types, rows aligned to 16 bytes, many queries)
 bool attn_tc_fits(const AttnArgs& a);
+int attn_tc_splits(const AttnArgs& a, int sms);  // of attn_tc_f32.cu as well
 void attn_tc_forward(const AttnArgs& a, cudaStream_t st);
 // kernels of attn_tc_f32.cu (fp32, heads of up to 64 values, many queries)
 bool attn_tc_f32_fits(const AttnArgs& a);

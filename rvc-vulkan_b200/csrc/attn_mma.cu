@@ -1171,12 +1171,7 @@ void fwd_dp(const AttnArgs& a, cudaStream_t st) {
     note_launch();
     RVC_CUDA_TRY(cudaGetLastError());
   }
-  if (a.po) {
-    const long long n = (long long)a.B * a.Hq * a.Lq;
-    attn_join_kernel<T><<<(unsigned)((n + 7) / 8), 256, 0, st>>>(a, n);
-    note_launch();
-    RVC_CUDA_TRY(cudaGetLastError());
-  }
+  attn_join(a, st);
 }
 
 template <typename T, int DP>
@@ -1258,6 +1253,17 @@ int attn_mma_splits(const AttnArgs& a, int sms, bool* workspace) {
   const int n = (int)std::max(1ll, std::min({want, (long long)(tiles / 2), 64ll}));
   *workspace = n > 1;
   return n;
+}
+
+void attn_join(const AttnArgs& a, cudaStream_t st) {
+  if (!a.po) return;
+  const long long n = (long long)a.B * a.Hq * a.Lq;
+  const unsigned grid = (unsigned)((n + 7) / 8);
+  if (a.type == kF32) attn_join_kernel<float><<<grid, 256, 0, st>>>(a, n);
+  else if (a.type == kBf16) attn_join_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a, n);
+  else attn_join_kernel<__half><<<grid, 256, 0, st>>>(a, n);
+  note_launch();
+  RVC_CUDA_TRY(cudaGetLastError());
 }
 
 void attn_mma_forward(const AttnArgs& a, cudaStream_t st) {

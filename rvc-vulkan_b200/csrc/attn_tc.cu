@@ -115,7 +115,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   const int len = kv_len(a, b);
   long long kend = len;
   if (a.causal) kend = max(0ll, min(kend, (long long)min(a.Lq, q0 + 256) + a.q_off));
-  const int tiles = (int)((kend + 127) / 128);
+  // the key tiles of this split: from key k0 on
+  const int all = (int)((kend + 127) / 128), t0 = (int)((long long)all * blockIdx.y / a.nsplit);
+  const int tiles = (int)((long long)all * (blockIdx.y + 1) / a.nsplit) - t0, k0 = t0 * 128;
 
   if (threadIdx.x == 0) {
     ptx::mbar_init(Q_FULL, 1);
@@ -165,10 +167,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           }
           ptx::mbar_expect_tx(K_FULL + 8 * st, NS * kSlab + (a.diag ? 384 * 4 : 0));
           for (int s = 0; s < NS; ++s)
-            ptx::tma_load_4d(sK + (st * NS + s) * kSlab, &maps.k, 64 * s, kh, t * 128, b, K_FULL + 8 * st);
+            ptx::tma_load_4d(sK + (st * NS + s) * kSlab, &maps.k, 64 * s, kh, k0 + t * 128, b, K_FULL + 8 * st);
           nk = t + 1;
           if (a.diag)
-            ptx::bulk_g2s(base + oB + st * 384 * 4, a.diag + h * a.diag_ld + (t * 128 - q0 - 256 + a.diag0), 384 * 4,
+            ptx::bulk_g2s(base + oB + st * 384 * 4, a.diag + h * a.diag_ld + (k0 + t * 128 - q0 - 256 + a.diag0), 384 * 4,
                           K_FULL + 8 * st);
           if (!bar_wait(V_EMPTY + 8 * st, ph)) {
             ok = false;
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           }
           ptx::mbar_expect_tx(V_FULL + 8 * st, NS * kSlab);
           for (int s = 0; s < NS; ++s)
-            ptx::tma_load_4d(sV + (st * NS + s) * kSlab, &maps.v, 64 * s, kh, t * 128, b, V_FULL + 8 * st);
+            ptx::tma_load_4d(sV + (st * NS + s) * kSlab, &maps.v, 64 * s, kh, k0 + t * 128, b, V_FULL + 8 * st);
           nv = t + 1;
         }
         if (!ok) atomicExch(a.err, 41);
@@ -261,9 +263,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         bytes[x] = j < len ? mb[(int64_t)j * a.mask_k] : 0;
       }
     };
-    if (mb) fetch(0);
+    if (mb) fetch(k0);
     for (int t = 0; t < tiles && ok; ++t) {
-      const int st = t % R, j0 = t * 128;
+      const int st = t % R, j0 = k0 + t * 128;
       uint32_t alive[4] = {~0u, ~0u, ~0u, ~0u};  // the mask's bytes came with the last tile
       if (mb) {
 #pragma unroll
@@ -406,8 +408,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     if (!ok) {
       if (lane == 0) atomicExch(a.err, 43);
     } else {
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const bool part = a.nsplit > 1;  // the row as it stands, for attn_join_kernel
+      const float inv = part ? 1.f : l > 0.f ? 1.f / l : 0.f;
       T* dst = static_cast<T*>(a.out) + (((long long)b * a.Lq + i) * a.Hq + h) * a.D;
+      const long long row_at = ((long long)b * a.Hq + h) * a.Lq + i;
+      const long long pr = (long long)blockIdx.y * a.B * a.Hq * a.Lq + row_at;
 #pragma unroll 1
       for (int x = 0; x < 64 * NS; x += 16) {
         if (x >= a.D) break;
@@ -418,7 +423,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 #pragma unroll
           for (int c = 0; c < 16; ++c) o[c] = 0.f;
         }
-        if (i < a.Lq) {
+        if (i < a.Lq && part) {
+#pragma unroll
+          for (int c = 0; c < 16; c += 4)
+            if (x + c < a.D)
+              *reinterpret_cast<float4*>(a.po + pr * a.D + x + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+        } else if (i < a.Lq) {
 #pragma unroll
           for (int c = 0; c < 16; c += 8)
             if (x + c < a.D)  // D is a multiple of 8
@@ -427,7 +437,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                              pack2<T>(o[c + 4] * inv, o[c + 5] * inv), pack2<T>(o[c + 6] * inv, o[c + 7] * inv));
         }
       }
-      if (i < a.Lq) a.lse[((long long)b * a.Hq + h) * a.Lq + i] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+      if (i < a.Lq && part) {
+        a.pml[2 * pr] = m;
+        a.pml[2 * pr + 1] = l;
+      } else if (i < a.Lq) {
+        a.lse[row_at] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+      }
     }
   }
   ptx::tc_fence_before();
@@ -451,7 +466,7 @@ void fwd(const AttnArgs& a, cudaStream_t st) {
     if (dev < 64) done.fetch_or(1ull << dev);
   }
   const unsigned grid = (unsigned)((a.Lq + 255ll) / 256 * a.B * a.Hq);
-  attn_tc_fwd_kernel<T, NS, FULL><<<grid, kFwdThreads, fwd_smem<NS>(), st>>>(a, maps);
+  attn_tc_fwd_kernel<T, NS, FULL><<<dim3(grid, a.nsplit), kFwdThreads, fwd_smem<NS>(), st>>>(a, maps);
   note_launch();
   RVC_CUDA_TRY(cudaGetLastError());
 }
@@ -477,6 +492,16 @@ bool attn_tc_fits(const AttnArgs& a) {
 void attn_tc_forward(const AttnArgs& a, cudaStream_t st) {
   if (a.type == kBf16) fwd_t<__nv_bfloat16>(a, st);
   else fwd_t<__half>(a, st);
+  attn_join(a, st);
+}
+
+// Splits of the keys where the query tiles leave half of the SMs or more without
+// work: as many as there are idle SMs for, eight tiles of 128 keys each at least
+// (the parts of a row are written and read once more, 4 D bytes each).
+int attn_tc_splits(const AttnArgs& a, int sms) {
+  const long long rows = a.type == kF32 ? 128 : 256;
+  const long long blocks = (a.Lq + rows - 1) / rows * a.B * a.Hq;
+  return (int)std::max(1ll, std::min({sms / std::max(1ll, blocks), a.Lk / 1024ll, 64ll}));
 }
 
 }  // namespace rvc

@@ -94,7 +94,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int len = kv_len(a, b);
   long long kend = len;
   if (a.causal) kend = max(0ll, min(kend, (long long)min(a.Lq, q0 + 128) + a.q_off));
-  const int tiles = (int)((kend + 63) / 64);
+  // the key tiles of this split: from key k0 on
+  const int all = (int)((kend + 63) / 64), t0 = (int)((long long)all * blockIdx.y / a.nsplit);
+  const int tiles = (int)((long long)all * (blockIdx.y + 1) / a.nsplit) - t0, k0 = t0 * 64;
 
   if (threadIdx.x == 0) {
     ptx::mbar_init(Q_FULL, 1);
@@ -138,16 +140,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           ptx::mbar_expect_tx(K_FULL + 8 * st, 3 * kTile + (a.diag ? 768 : 0));
           for (int i = 0; i < 3; ++i)
-            ptx::tma_load_4d(sK + (st * 3 + i) * kTile, &maps.k, 0, kh, t * 64, i * a.B + b, K_FULL + 8 * st);
+            ptx::tma_load_4d(sK + (st * 3 + i) * kTile, &maps.k, 0, kh, k0 + t * 64, i * a.B + b, K_FULL + 8 * st);
           if (a.diag)
-            ptx::bulk_g2s(base + oB + st * 768, a.diag + h * a.diag_ld + (t * 64 - q0 - 128 + a.diag0), 768,
+            ptx::bulk_g2s(base + oB + st * 768, a.diag + h * a.diag_ld + (k0 + t * 64 - q0 - 128 + a.diag0), 768,
                           K_FULL + 8 * st);
           nk = t + 1;
           ok = bar_wait(V_EMPTY + 8 * st, ph);
           if (!ok) break;
           ptx::mbar_expect_tx(V_FULL + 8 * st, 3 * kTile);
           for (int i = 0; i < 3; ++i)
-            ptx::tma_load_4d(sV + (st * 3 + i) * kTile, &maps.v, 0, kh, t * 64, i * a.B + b, V_FULL + 8 * st);
+            ptx::tma_load_4d(sV + (st * 3 + i) * kTile, &maps.v, 0, kh, k0 + t * 64, i * a.B + b, V_FULL + 8 * st);
           nv = t + 1;
         }
         if (!ok) atomicExch(a.err, 61);
@@ -237,10 +239,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           o[16 * x + c] = mul2(add2(o[16 * x + c], f32x2(__uint_as_float(u[2 * c]), __uint_as_float(u[2 * c + 1]))), f2);
       }
     };
-    if (mb) fetch(64 * w);
+    if (mb) fetch(k0 + 64 * w);
     int last = -1;  // this group's last tile
     for (int t = w; t < tiles; t += 2) {
-      const int st = t % R, j0 = t * 64;
+      const int st = t % R, j0 = k0 + t * 64;
       const uint32_t turn = (t >> 1) & 1;
       uint32_t alive[2] = {~0u, ~0u};
       if (mb) {
@@ -357,8 +359,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (w == 0 && i < a.Lq) {
       const float m1 = part[64 * 128], M = fmaxf(m, m1), off = M == -INFINITY ? 0.f : M;
       const float f0 = exp2_approx(m - off), f1 = exp2_approx(m1 - off);
-      const float L = f0 * l + f1 * part[65 * 128], inv = L > 0.f ? 1.f / L : 0.f;
-      float* dst = static_cast<float*>(a.out) + (((long long)b * a.Lq + i) * a.Hq + h) * a.D;
+      const float L = f0 * l + f1 * part[65 * 128], inv = a.nsplit > 1 ? 1.f : L > 0.f ? 1.f / L : 0.f;
+      const long long row_at = ((long long)b * a.Hq + h) * a.Lq + i;
+      const long long pr = (long long)blockIdx.y * a.B * a.Hq * a.Lq + row_at;
+      float* dst = a.nsplit > 1 ? a.po + pr * a.D  // the row as it stands, for attn_join_kernel
+                                : static_cast<float*>(a.out) + (((long long)b * a.Lq + i) * a.Hq + h) * a.D;
 #pragma unroll
       for (int c = 0; c < 64; c += 4)
         if (c < a.D) {
@@ -369,7 +374,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < 4; ++k) u[k] = (f0 * u[k] + f1 * part[(c + k) * 128]) * inv;
           *reinterpret_cast<float4*>(dst + c) = make_float4(u[0], u[1], u[2], u[3]);
         }
-      a.lse[((long long)b * a.Hq + h) * a.Lq + i] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+      if (a.nsplit > 1) {
+        a.pml[2 * pr] = M;
+        a.pml[2 * pr + 1] = L;
+      } else {
+        a.lse[row_at] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+      }
     }
   }
   ptx::tc_fence_before();
@@ -421,9 +431,10 @@ void attn_tc_f32_forward(const AttnArgs& a, void* ws, int sms, cudaStream_t st) 
     RVC_CUDA_TRY(cudaFuncSetAttribute(attn_tc_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
     if (dev < 64) done.fetch_or(1ull << dev);
   }
-  attn_tc_f32_kernel<<<(unsigned)((a.Lq + 127ll) / 128 * a.B * a.Hq), kThreads, kSmem, st>>>(a, maps);
+  attn_tc_f32_kernel<<<dim3((unsigned)((a.Lq + 127ll) / 128 * a.B * a.Hq), a.nsplit), kThreads, kSmem, st>>>(a, maps);
   note_launch();
   RVC_CUDA_TRY(cudaGetLastError());
+  attn_join(a, st);
 }
 
 }  // namespace rvc

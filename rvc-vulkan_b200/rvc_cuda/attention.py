@@ -12,8 +12,12 @@
 The functions take CUDA tensors (``torch.float32``, ``bfloat16`` or
 ``float16``), run on the tensors' device and its current stream without
 synchronising, and return new contiguous tensors; scratch memory comes from
-torch's allocator, so a call can be captured into a CUDA graph.  Nothing is
-kept between calls.  ``rvc_cuda.ops`` has the forms for numpy arrays.  The
+torch's allocator, so a call can be captured into a CUDA graph (after a first
+call on the device, which opens the library's context there).  Nothing is kept
+between calls, and there is no autograd: the ``*_backward`` functions are called
+with what the forward ones returned.  A wait inside a kernel that gives up
+(after two seconds) is reported by the next ``sync`` of the device's context,
+``rvc_cuda._lib.get_context(i).sync()``.  ``rvc_cuda.ops`` has the forms for numpy arrays.  The
 device code and its C entry points (``include/rvc_cuda.h``) have no counterpart
 in the reference, whose attention (``runtime/models/vits.py:993-1014``,
 ``runtime/models/hubert.py:1315-1400``) has one length, no padding and no
@@ -25,6 +29,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import operator
 import struct
 from typing import Optional
 
@@ -202,6 +207,16 @@ def _table(bias, H: int, like):
     return t.contiguous(), bias.num_buckets, int(bias.bidirectional), bias._borders, bias._nborders
 
 
+def _offset(q_offset) -> int:
+    try:
+        n = operator.index(q_offset)
+    except TypeError:
+        raise ValueError(f"q_offset: a whole number is expected, got {q_offset!r}") from None
+    if not -(1 << 31) <= n <= 1 << 31:
+        raise ValueError(f"q_offset {n} out of range")
+    return n
+
+
 def _scale(scale, D: int) -> float:
     s = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not math.isfinite(s):
@@ -240,7 +255,7 @@ def attention(q, k, v, *, kv_lens=None, key_mask=None, scale: Optional[float] = 
     ctx, stream = _where(q)
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     desc = _pack29(_TYPES[q.dtype], B, Hq, Hkv, Lq, Lk, D, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1],
-                   vs[2], bits, mb, mk, bool(causal), q_offset, nb, both, 0, 0, 0, 0, 0, 0)
+                   vs[2], bits, mb, mk, bool(causal), _offset(q_offset), nb, both, 0, 0, 0, 0, 0, 0)
     scale = _scale(scale, D)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((B, Hq, Lq), dtype=torch.float32)
@@ -276,7 +291,7 @@ def attention_backward(dout, q, k, v, out, lse, *, kv_lens=None, key_mask=None, 
     table, nb, both, borders, nborders = _table(bias, Hq, q)
     ctx, stream = _where(q)
     desc = _pack29(_TYPES[q.dtype], B, Hq, Hkv, Lq, Lk, D, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], bits, mb,
-                   mk, bool(causal), q_offset, nb, both, *dout.stride()[:3], *out.stride()[:3])
+                   mk, bool(causal), _offset(q_offset), nb, both, *dout.stride()[:3], *out.stride()[:3])
     dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
     dtable = q.new_empty((nb, Hq)) if nb else None
     ws, nbytes = _scratch(lib.rvc_cuda_attention_workspace, ctx, desc, 29, q, 1)
@@ -301,7 +316,7 @@ def relative_bias(bias: BucketBias, Lq: int, Lk: int, *, q_offset: int = 0):
         raise ValueError(f"relative_bias: lengths {Lq} and {Lk}")
     ctx, stream = _where(t)
     out = t.new_empty((H, Lq, Lk))
-    desc = _pack11(_TYPES[t.dtype], 1, H, Lq, Lk, q_offset, bias.num_buckets, bias.bidirectional, 0, 0, 0)
+    desc = _pack11(_TYPES[t.dtype], 1, H, Lq, Lk, _offset(q_offset), bias.num_buckets, bias.bidirectional, 0, 0, 0)
     check(lib.rvc_cuda_relative_bias_device(ctx, stream, desc, 11, t.data_ptr(), bias._borders, bias._nborders,
                                             out.data_ptr()))
     return out
@@ -323,7 +338,7 @@ def relative_bias_backward(bias: BucketBias, dbias, *, q_offset: int = 0):
     if H != bias.table.shape[1]:
         raise ValueError(f"relative_bias_backward: {H} heads, the table has {bias.table.shape[1]}")
     ctx, stream = _where(d)
-    desc = _pack11(_TYPES[d.dtype], B, H, Lq, Lk, q_offset, bias.num_buckets, bias.bidirectional, *d.stride()[:3])
+    desc = _pack11(_TYPES[d.dtype], B, H, Lq, Lk, _offset(q_offset), bias.num_buckets, bias.bidirectional, *d.stride()[:3])
     dtable = d.new_empty((bias.num_buckets, H))
     ws, nbytes = _scratch(lib.rvc_cuda_relative_bias_workspace, ctx, desc, 11, d)
     check(lib.rvc_cuda_relative_bias_backward_device(ctx, stream, desc, 11, d.data_ptr(), bias._borders,

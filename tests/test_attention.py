@@ -97,6 +97,9 @@ def test_attention_refusals():
     refused("key_mask", A.attention, q, k, k, key_mask=t(2, 7))
     refused("key_mask", A.attention, q, k, k, key_mask=t(2, 6, dtype=torch.bool))
     refused("BucketBias", A.attention, q, k, k, bias=t(8, 4))
+    refused("q_offset", A._offset, 1.5)
+    refused("q_offset", A._offset, (1 << 31) + 1)
+    refused("q_offset", A._offset, -(1 << 40))
     refused("4 query heads", A.attention, q, k, k, bias=A.BucketBias(t(8, 2)))
     refused("bias table", A.attention, q, k, k, bias=A.BucketBias(t(8, 4, dtype=torch.float16)))
 

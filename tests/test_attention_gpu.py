@@ -194,6 +194,33 @@ def test_masks_and_bias(dtype, mask, Lq):
     c.backward()
 
 
+SPLIT = {
+    "plain": {},
+    "lens": dict(lens=[4100, 0], junk=float("nan")),
+    "keys_bias": dict(keep="random", bias=(32, 400, True), junk=float("inf")),
+    "causal": dict(causal=True, q_offset=700),
+    "causal_nothing": dict(causal=True, q_offset=-100000),
+}
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("mask", SPLIT, ids=str)
+@pytest.mark.parametrize("D", [64, 128])
+def test_keys_split_over_blocks(dtype, mask, D):
+    """Few queries on long states: the keys are shared out to blocks and joined,
+    on every path (few rows, many rows, tensor-core tiles), some shares empty."""
+    for Lq in (2, 40, 130):
+        Case(dtype, 2, 2, 1, D, Lq, 4100, **SPLIT[mask]).forward()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_causal_with_nothing_alive_and_scale_zero(dtype):
+    for kw in (dict(causal=True, q_offset=-100000), dict(scale=0.0), dict(scale=0.0, keep="random", junk=float("nan"))):
+        c = Case(dtype, 2, 4, 2, 64, 270, 200, **kw)
+        c.forward()
+        c.backward()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("D", [64, 96, 128])
 def test_bias_gradient_over_many_tiles(dtype, D):
