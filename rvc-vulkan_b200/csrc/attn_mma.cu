@@ -812,6 +812,12 @@ __global__ void attn_delta_kernel(const __grid_constant__ AttnArgs a, long long 
   if (lane == 0) a.delta[row] = s;
 }
 
+// A query that can meet one key at most has weight 1 there whatever the score:
+// its dS is zero, not what the roundings of P and delta leave of it.
+__device__ __forceinline__ bool lone_row(const AttnArgs& a, int len, long long i) {
+  return (a.causal ? min((long long)len, i + a.q_off + 1) : (long long)len) <= 1;
+}
+
 // The second half's accumulators added to the first's, through shared memory
 // that nobody reads any more; false for the second half, which is done.
 template <int DP>
@@ -891,7 +897,7 @@ __global__ void __launch_bounds__(kT * KS) attn_mma_dq_kernel(const __grid_const
     const float z = a.lse[row];
     const bool live = z != -INFINITY && i0 + warp * 16 + g + 8 * y < a.Lq;
     lse2[y] = live ? z * kLog2e : INFINITY;  // a row that is not there or has no key: P = 0
-    delta[y] = DELTA ? 0.f : a.delta[row];
+    delta[y] = DELTA ? 0.f : lone_row(a, len, qi[y]) ? INFINITY : a.delta[row];
     bias[y] = a.diag ? a.diag + h * a.diag_ld + a.diag0 - qi[y] : nullptr;
   }
   const float sc = a.scale * kLog2e;
@@ -931,7 +937,7 @@ __global__ void __launch_bounds__(kT * KS) attn_mma_dq_kernel(const __grid_const
         if (a.diag && j < a.Lk) z += __ldg(bias[y] + j);
         const bool on = j < len && (!mb || mb[(int64_t)j * a.mask_k]) && (!a.causal || j <= qi[y] + a.q_off);
         const float p = on ? exp2_approx(z - lse2[y]) : 0.f;
-        s[n][x] = p != 0.f ? p * (dp[n][x] - (DELTA ? 0.f : delta[y])) : 0.f;
+        s[n][x] = p != 0.f && (DELTA || delta[y] != INFINITY) ? p * (dp[n][x] - (DELTA ? 0.f : delta[y])) : 0.f;
         if (DELTA) delta[y] += s[n][x];
         if (dws) sD[(warp * 16 + g + 8 * y) * SL + key0 + n * 8 + 2 * t + (x & 1)] = s[n][x];
       }
@@ -1031,7 +1037,7 @@ __global__ void __launch_bounds__(kT * KS) attn_mma_dkv_kernel(const __grid_cons
       const long long row = ((long long)b * a.Hq + h) * a.Lq + i0 + tid;
       const float z = in ? a.lse[row] : -INFINITY;
       stat[(st * 2) * BQ + tid] = z != -INFINITY ? z * kLog2e : INFINITY;
-      stat[(st * 2 + 1) * BQ + tid] = in ? a.delta[row] : 0.f;
+      stat[(st * 2 + 1) * BQ + tid] = !in ? 0.f : lone_row(a, len, i0 + tid) ? INFINITY : a.delta[row];
     }
     cp_commit();
   };
@@ -1088,7 +1094,7 @@ __global__ void __launch_bounds__(kT * KS) attn_mma_dkv_kernel(const __grid_cons
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const float de = stat[(st * 2 + 1) * BQ + row0 + n * 8 + 2 * t + (x & 1)];
-        s[n][x] = s[n][x] != 0.f ? s[n][x] * (dp[n][x] - de) : 0.f;
+        s[n][x] = s[n][x] != 0.f && de != INFINITY ? s[n][x] * (dp[n][x] - de) : 0.f;
       }
     mma_pb<T, DP, NT>(dk, s, q, lane);
     __syncthreads();

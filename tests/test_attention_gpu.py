@@ -230,6 +230,15 @@ def test_bias_gradient_over_many_tiles(dtype, D):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_queries_with_one_key(dtype):
+    """A softmax over one key is 1: no gradient reaches q, k or the table, exactly."""
+    for Lq, Lk, kw in ((1, 1, {}), (70, 1, {}), (5, 40, dict(lens=[1, 1])), (1, 9, dict(causal=True))):
+        c = Case(dtype, 2, 4, 2, 64, Lq, Lk, bias=(8, 6, True), **kw)
+        dq, dk, _, dt = c.backward()
+        assert (dq == 0).all() and (dk == 0).all() and (dt == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 def test_no_keys_and_no_rows(dtype):
     c = Case(dtype, 2, 4, 2, 64, 7, 0, bias=(8, 6, True))
     out, lse = c.forward()
