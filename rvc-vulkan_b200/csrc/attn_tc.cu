@@ -488,10 +488,14 @@ void fwd_t(const AttnArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-// 16-bit operands that TMA can address, and enough queries to fill a tile of
-// 128 rows more than half.
+// 16-bit operands that TMA can address, and queries enough: the general kernel
+// fills its tiles with the rows of a whole group, this one leaves them empty.
+// Measured in us, general / tiles (6831 keys): 12 heads of 64, 20 queries 38 / 32;
+// 8 x 16/4 heads of 128, 20 queries 199 / 111, 6 queries 105 / 111; 4 x 64/8 heads
+// of 64, 32 queries 141 / 198, 48 queries 204 / 198.
 bool attn_tc_fits(const AttnArgs& a) {
-  return a.type != kF32 && a.Lq >= 64 && a.Lk >= 1 && atc::map_ok(a, a.q, a.qs, a.Lq, a.Hq) &&
+  const int least = a.D > 64 || a.Hq / a.Hkv <= 4 ? 20 : 48;
+  return a.type != kF32 && a.Lq >= least && a.Lk >= 1 && atc::map_ok(a, a.q, a.qs, a.Lq, a.Hq) &&
          atc::map_ok(a, a.k, a.ks, a.Lk, a.Hkv) && atc::map_ok(a, a.v, a.vs, a.Lk, a.Hkv) &&
          reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
 }

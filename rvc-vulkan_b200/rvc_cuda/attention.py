@@ -240,7 +240,9 @@ def attention(q, k, v, *, kv_lens=None, key_mask=None, scale: Optional[float] = 
     ``1 / sqrt(D)`` by default; ``bias`` adds ``table[bucket(j - i - q_offset),
     h]``.  Returns ``out [B, Lq, Hq, D]`` in the type of ``q`` and the float32
     log sums ``lse [B, Hq, Lq]`` that the backward pass takes; a query without
-    a live key gives 0 and ``-inf``.  Heads of 1 to 128 values; any strides
+    a live key gives 0 and ``-inf``.  float32 values are worked on as parts of
+    16 bits: an infinite one that is alive comes out as NaN.  Heads of 1 to 128
+    values; any strides
     (the parts of a packed projection are taken where they lie).
     """
     q, k, v, B, Lq, Lk, Hq, Hkv, D = _qkv(q, k, v)
