@@ -127,6 +127,11 @@ Layout plan(const AttnArgs& a, bool bias, bool backward, int sms, bool tc) {
   }
   l.row_ld = tc ? up(a.Lq, 128) : a.Lq;
   l.delta = take(4 * l.row_ld * a.B * a.Hq);
+  if (tc && (l.nsplit = attn_tc_bwd_shares(a, sms)) > 1) {
+    const int64_t n = 4ll * l.nsplit * a.B * a.Lk * a.Hkv * a.D;
+    l.po = take(n);
+    l.pml = take(n);
+  }
   if (tc) l.lse2 = take(4 * l.row_ld * a.B * a.Hq);
   if (bias) {
     l.BM = tc ? 128 : 64;

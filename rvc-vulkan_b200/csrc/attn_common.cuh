@@ -67,6 +67,7 @@ struct AttnArgs {
   int nsplit = 1;
   float* po = nullptr;           // [nsplit][B][Hq][Lq][D]
   float* pml = nullptr;          // [nsplit][B][Hq][Lq][2]
+  // (backward: shares of the query heads of a group, parts of dK and dV [nsplit][B][Lk][Hkv][D])
   // backward
   const void *dout = nullptr, *fout = nullptr;
   int64_t dos[3] = {0, 0, 0}, os[3] = {0, 0, 0};
@@ -145,6 +146,7 @@ int64_t attn_tc_f32_workspace(const AttnArgs& a);
 void attn_tc_f32_forward(const AttnArgs& a, void* ws, int sms, cudaStream_t st);
 // kernels of attn_tc_bwd.cu (as attn_tc.cu)
 bool attn_tc_bwd_fits(const AttnArgs& a);
+int attn_tc_bwd_shares(const AttnArgs& a, int sms);
 int attn_tc_bwd_arrays(const AttnArgs& a);  // arrays of diagonal sums to a tile of keys
 void attn_tc_backward(const AttnArgs& a, cudaStream_t st);
 

@@ -87,14 +87,17 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
   uint32_t* slot = reinterpret_cast<uint32_t*>(gen + oBar + 504);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  const int G = a.Hq / a.Hkv;
+  const int group = a.Hq / a.Hkv;
   const int ny = KV ? (a.Lq + 63) / 64 : 0;  // second: query tiles of a head
   const int ntile = KV ? (a.Lk + 127) / 128 : (a.Lq + 127) / 128;
   const int heads = KV ? a.Hkv : a.Hq;
   // with a causal limit the longest walks come first: late queries, early keys
   const int xt = a.causal && !KV ? ntile - 1 - (int)(blockIdx.x % ntile) : (int)(blockIdx.x % ntile);
   const int bh = blockIdx.x / ntile, b = bh / heads, hx = bh % heads;
-  const int kh = KV ? hx : hx / G;
+  const int kh = KV ? hx : hx / group;
+  // second: the query heads of this share of the group, h0 .. h0 + G - 1
+  const int g0 = KV ? group * (int)blockIdx.y / a.nsplit : 0;
+  const int G = KV ? group * ((int)blockIdx.y + 1) / a.nsplit - g0 : 1, h0 = kh * group + g0;
   const int x0 = xt * 128;
   const int len = kv_len(a, b);
   // tiles that pass by: first: keys [0, kend); second: queries from `first` on, head by head
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
       for (int t = 0; t < tiles; ++t) {
         const int st = t % R;
         const uint32_t ph = ((t / R) & 1) ^ 1;
-        const int hy = KV ? kh * G + t / per : kh;
+        const int hy = KV ? h0 + t / per : kh;
         const int y0 = KV ? (first + t % per) * 64 : t * 64;
         ok = bar_wait(Y1_EMPTY + 8 * st, ph);
         if (!ok) break;
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
       const int y0 = KV ? (first + t % per) * 64 : t * 64;
       const float* e = ext + st * kExt;
       if (KV && a.dws)
-        for (; head < t / per; ++head) end_head(kh * G + head);
+        for (; head < t / per; ++head) end_head(h0 + head);
       uint32_t alive[2] = {~0u, ~0u};  // first: keys of the tile; the mask's bytes came with the last one
       if (!KV && mb) {
         alive[0] = __ballot_sync(0xffffffffu, byte0 != 0);
@@ -465,7 +468,7 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
       if (KV && a.dws) ok = ptx::named_bar_and(1 + w, 128, ok);
       if (!ok) break;
       if (KV && a.dws) {
-        float* dws = a.dws + ((((int64_t)b * a.Hq + kh * G + head) * ntile + xt) * GR + w) * a.dws_ld;
+        float* dws = a.dws + ((((int64_t)b * a.Hq + h0 + head) * ntile + xt) * GR + w) * a.dws_ld;
         // Diagonal u < 191 of the tile: key - query = 127 - u; it is entry y0 + u of
         // the array.  The first kStep are whole with this tile (the group's next is
         // kStep queries on), the others stay open.
@@ -509,7 +512,7 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
       }
     }
     if (KV && a.dws && ok)
-      for (; head < G; ++head) end_head(kh * G + head);
+      for (; head < G; ++head) end_head(h0 + head);
     if (ok && tiles > 0) ok = warp_wait(DONE, 0);
     ptx::tc_fence_after();
     if (!ok) {
@@ -547,6 +550,16 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
           for (int c = 0; c < 16; ++c) u[c] = v[c] = 0.f;
         }
         if (x >= L) continue;
+        if (KV && a.nsplit > 1) {  // this share's part, for kv_join_kernel
+          const int64_t part = (int64_t)blockIdx.y * a.B * a.Lk * a.Hkv * a.D + to + c0;
+#pragma unroll
+          for (int c = 0; c < 16; c += 4)
+            if (c0 + c < a.D) {
+              *reinterpret_cast<float4*>(a.po + part + c) = make_float4(u[c], u[c + 1], u[c + 2], u[c + 3]);
+              *reinterpret_cast<float4*>(a.pml + part + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+            }
+          continue;
+        }
 #pragma unroll
         for (int c = 0; c < 16; ++c) u[c] = a.scale * (KV ? u[c] : u[c] - rr * v[c]);
 #pragma unroll
@@ -567,6 +580,20 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
   if (warp == kIssue) ptx::tmem_dealloc(tmem, 256 * GR);
 }
 
+// dK and dV from the shares of the query heads, added in order.
+template <typename T>
+__global__ void __launch_bounds__(256) kv_join_kernel(const __grid_constant__ AttnArgs a, long long n) {
+  const long long e = blockIdx.x * 256ll + threadIdx.x;
+  if (e >= n) return;
+  float k = 0.f, v = 0.f;
+  for (int s = 0; s < a.nsplit; ++s) {
+    k += a.po[s * n + e];
+    v += a.pml[s * n + e];
+  }
+  static_cast<T*>(a.dk)[e] = from_f<T>(a.scale * k);
+  static_cast<T*>(a.dv)[e] = from_f<T>(v);
+}
+
 template <typename T, int NS, bool KV, bool FULL>
 void launch(const AttnArgs& a, const BwdMaps& maps, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};  // one bit per device
@@ -578,9 +605,15 @@ void launch(const AttnArgs& a, const BwdMaps& maps, cudaStream_t st) {
     if (dev < 64) done.fetch_or(1ull << dev);
   }
   const unsigned grid = KV ? (unsigned)((a.Lk + 127ll) / 128 * a.B * a.Hkv) : (unsigned)((a.Lq + 127ll) / 128 * a.B * a.Hq);
-  attn_tc_bwd_kernel<T, NS, KV, FULL><<<grid, kBwdThreads<NS>, bwd_smem<NS>(), st>>>(a, maps);
+  attn_tc_bwd_kernel<T, NS, KV, FULL><<<dim3(grid, KV ? a.nsplit : 1), kBwdThreads<NS>, bwd_smem<NS>(), st>>>(a, maps);
   note_launch();
   RVC_CUDA_TRY(cudaGetLastError());
+  if (KV && a.nsplit > 1) {
+    const long long n = (long long)a.B * a.Lk * a.Hkv * a.D;
+    kv_join_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a, n);
+    note_launch();
+    RVC_CUDA_TRY(cudaGetLastError());
+  }
 }
 
 template <typename T, int NS, bool FULL>
@@ -607,6 +640,13 @@ void bwd_t(const AttnArgs& a, cudaStream_t st) {
 }
 
 }  // namespace
+
+// Shares of a group's query heads for the second kernel, where its key tiles
+// leave half of the SMs' places or more empty.
+int attn_tc_bwd_shares(const AttnArgs& a, int sms) {
+  const long long blocks = (a.Lk + 127ll) / 128 * a.B * a.Hkv, places = (a.D <= 64 ? 2ll : 1ll) * sms;
+  return (int)std::max(1ll, std::min((long long)(a.Hq / a.Hkv), places / std::max(1ll, blocks)));
+}
 
 int attn_tc_bwd_arrays(const AttnArgs& a) { return a.D <= 64 ? kGroups<1> : kGroups<2>; }
 

@@ -213,6 +213,14 @@ def test_keys_split_over_blocks(dtype, mask, D):
         Case(dtype, 2, 2, 1, D, Lq, 4100, **SPLIT[mask]).forward()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("D", [40, 128])
+def test_shares_of_a_group(dtype, D):
+    """Few key tiles and a large group: its query heads are shared out to blocks."""
+    Case(dtype, 1, 7, 1, D, 150, 200, bias=(32, 60, True), causal=True, q_offset=50).backward()
+    Case(dtype, 3, 24, 2, D, 70, 300, lens=[300, 0, 129], junk=float("nan"), bias=(16, 30, False)).backward()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_causal_with_nothing_alive_and_scale_zero(dtype):
     for kw in (dict(causal=True, q_offset=-100000), dict(scale=0.0), dict(scale=0.0, keep="random", junk=float("nan"))):
