@@ -408,8 +408,10 @@ int32_t rvc_cuda_to_int16(int64_t ctx, const float* x, int64_t n, int16_t* y);
  * bidirectional, dout stride (3), out stride (3)}: 29 values.  1 <= D <= 128,
  * Hq a multiple of Hkv.  Key j of batch entry b is alive when j < kv_lens[b]
  * (clamped to [0, Lk]), key_mask[b, j] != 0 and, when causal, j <= i + q_offset;
- * nothing of a dead key's k or v reaches a result, whatever it holds.  A query
- * without a live key gives out = 0, lse = -inf and zero gradients.
+ * nothing of the k or v of a key that no query meets reaches a result, whatever it
+ * holds (a key that is causally dead for some queries only has to be finite: its
+ * weight there is 0, which meets the value).  A query without a live key gives
+ * out = 0, lse = -inf and zero gradients.
  * table [buckets, Hq] (in `type`) adds table[bucket(j - i - q_offset), h] to the
  * scaled score; borders (host, int32) are the smallest distances of the buckets
  * 1, 2, ... of one direction.  out [B, Lq, Hq, D] contiguous, lse [B, Hq, Lq]

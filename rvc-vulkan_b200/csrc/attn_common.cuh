@@ -51,7 +51,7 @@ struct AttnArgs {
   const void *q = nullptr, *k = nullptr, *v = nullptr;
   // strides in elements: batch, row, head (the head's D values are contiguous)
   int64_t qs[3] = {0, 0, 0}, ks[3] = {0, 0, 0}, vs[3] = {0, 0, 0};
-  const void* lens = nullptr;  // [B] int32 or int64, clamped to [0, Lk]
+  const void* lens = nullptr;  // [B] int32 or int64, clamped to [0, Lk]; read through kv_len
   int lens64 = 0;
   const uint8_t* mask = nullptr;  // [B, Lk] bytes, non-zero = alive
   int64_t mask_b = 0, mask_k = 0;
@@ -81,10 +81,14 @@ struct AttnArgs {
   int* err = nullptr;            // the context's error word, set by a bounded wait that gave up
 };
 
+// Keys of batch entry b that some query of the call may meet.  What lies behind
+// is neither read as it is nor left to a product: a cache that is filled up to
+// the last query's limit may hold anything past it.
 __device__ __forceinline__ int kv_len(const AttnArgs& a, int b) {
-  if (!a.lens) return a.Lk;
-  const long long n = a.lens64 ? static_cast<const long long*>(a.lens)[b] : (long long)static_cast<const int*>(a.lens)[b];
-  return (int)(n < 0 ? 0 : (n > a.Lk ? a.Lk : n));
+  long long n = a.Lk;
+  if (a.lens) n = min(n, a.lens64 ? static_cast<const long long*>(a.lens)[b] : (long long)static_cast<const int*>(a.lens)[b]);
+  if (a.causal) n = min(n, a.Lq + (long long)a.q_off);
+  return (int)max(n, 0ll);
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {

@@ -235,7 +235,10 @@ def attention(q, k, v, *, kv_lens=None, key_mask=None, scale: Optional[float] = 
     those before ``kv_lens [B]`` (int32 or int64, clamped to ``[0, Lk]``), with
     ``key_mask [B, Lk]`` (bool or uint8) set, and, when ``causal``, not past
     ``i + q_offset`` for query ``i`` (``q_offset = Lk - Lq`` aligns the last
-    query with the last key).  Whatever a dead key holds reaches no result.
+    query with the last key).  Whatever a key holds that no query meets reaches
+    no result: padding, masked keys, a cache past the last query's limit.  A key
+    that is past the limit of some queries only must be finite, as its weight of
+    0 there meets the value.
     Query head ``h`` reads key head ``h // (Hq / Hkv)``.  ``scale`` is
     ``1 / sqrt(D)`` by default; ``bias`` adds ``table[bucket(j - i - q_offset),
     h]``.  Returns ``out [B, Lq, Hq, D]`` in the type of ``q`` and the float32
