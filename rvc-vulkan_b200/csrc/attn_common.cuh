@@ -97,6 +97,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// What a row's sum of weights L (held over the maximum M) makes of it.  L is 0
+// only where no key is alive or every score is -inf: out = 0, lse = -inf.  A NaN
+// sum (a live NaN or infinity) is no such row: it goes on into both.
+__device__ __forceinline__ float row_inv(float L) { return L == 0.f ? 0.f : 1.f / L; }
+__device__ __forceinline__ float row_lse(float M, float L) { return L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2; }
+
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }

@@ -471,14 +471,14 @@ __global__ void __launch_bounds__(kFwdRows<T> * 2, sizeof(T) == 4 && DP <= 64 ? 
         a.pml[2 * pr + 1] = l[y];
       }
     } else {
-      const float inv = l[y] > 0.f ? 1.f / l[y] : 0.f;
+      const float inv = row_inv(l[y]);
       T* dst = static_cast<T*>(a.out) + (((long long)b * a.Lq + i) * a.Hq + h) * a.D;
 #pragma unroll
       for (int d = 0; d < DP / 8; ++d)
 #pragma unroll
         for (int z = 0; z < 2; ++z)
           if (d * 8 + 2 * t + z < a.D) dst[d * 8 + 2 * t + z] = from_f<T>(o[d][2 * y + z] * inv);
-      if (t == 0) a.lse[row] = l[y] > 0.f ? (m[y] + log2f(l[y])) * kLn2 : -INFINITY;
+      if (t == 0) a.lse[row] = row_lse(m[y], l[y]);
     }
   }
 }
@@ -762,8 +762,8 @@ __global__ void __launch_bounds__(kT) attn_mma_few_kernel(const __grid_constant_
       M = bml[2 * r], L = bml[2 * r + 1], v = mine[r * LD + d];
     }
     const int i = r % a.Lq, h = kh * G + r / a.Lq;
-    static_cast<T*>(a.out)[(((long long)b * a.Lq + i) * a.Hq + h) * a.D + d] = from_f<T>(L > 0.f ? v / L : 0.f);
-    if (d == 0) a.lse[((long long)b * a.Hq + h) * a.Lq + i] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+    static_cast<T*>(a.out)[(((long long)b * a.Lq + i) * a.Hq + h) * a.D + d] = from_f<T>(L == 0.f ? 0.f : v / L);
+    if (d == 0) a.lse[((long long)b * a.Hq + h) * a.Lq + i] = row_lse(M, L);
   }
   if (CLUSTER) cluster_sync();  // no block leaves while another reads its memory
 }
@@ -782,20 +782,21 @@ __global__ void attn_join_kernel(const __grid_constant__ AttnArgs a, long long r
   for (int s = 0; s < a.nsplit; ++s) {
     const long long pr = s * rows + row;
     const float ms = a.pml[2 * pr];
-    if (ms == -INFINITY) continue;
+    const float ls = a.pml[2 * pr + 1];
+    if (ls == 0.f) continue;  // no weight; a NaN sum has a maximum of -inf too where every score is NaN
     const float f = exp2_approx(ms - M);
-    L = fmaf(f, a.pml[2 * pr + 1], L);
+    L = fmaf(f, ls, L);
 #pragma unroll
     for (int x = 0; x < 4; ++x)
       if (lane + 32 * x < a.D) o[x] = fmaf(f, a.po[pr * a.D + lane + 32 * x], o[x]);
   }
-  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const float inv = row_inv(L);
   const long long i = row % a.Lq, bh = row / a.Lq, b = bh / a.Hq, h = bh % a.Hq;
   T* dst = static_cast<T*>(a.out) + ((b * a.Lq + i) * a.Hq + h) * a.D;
 #pragma unroll
   for (int x = 0; x < 4; ++x)
     if (lane + 32 * x < a.D) dst[lane + 32 * x] = from_f<T>(o[x] * inv);
-  if (lane == 0) a.lse[row] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+  if (lane == 0) a.lse[row] = row_lse(M, L);
 }
 
 // --------------------------------------------------------------- backward

@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       if (lane == 0) atomicExch(a.err, 43);
     } else {
       const bool part = a.nsplit > 1;  // the row as it stands, for attn_join_kernel
-      const float inv = part ? 1.f : l > 0.f ? 1.f / l : 0.f;
+      const float inv = part ? 1.f : row_inv(l);
       T* dst = static_cast<T*>(a.out) + (((long long)b * a.Lq + i) * a.Hq + h) * a.D;
       const long long row_at = ((long long)b * a.Hq + h) * a.Lq + i;
       const long long pr = (long long)blockIdx.y * a.B * a.Hq * a.Lq + row_at;
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         a.pml[2 * pr] = m;
         a.pml[2 * pr + 1] = l;
       } else if (i < a.Lq) {
-        a.lse[row_at] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        a.lse[row_at] = row_lse(m, l);
       }
     }
   }

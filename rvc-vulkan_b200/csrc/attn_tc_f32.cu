@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (w == 0 && i < a.Lq) {
       const float m1 = part[64 * 128], M = fmaxf(m, m1), off = M == -INFINITY ? 0.f : M;
       const float f0 = exp2_approx(m - off), f1 = exp2_approx(m1 - off);
-      const float L = f0 * l + f1 * part[65 * 128], inv = a.nsplit > 1 ? 1.f : L > 0.f ? 1.f / L : 0.f;
+      const float L = f0 * l + f1 * part[65 * 128], inv = a.nsplit > 1 ? 1.f : row_inv(L);
       const long long row_at = ((long long)b * a.Hq + h) * a.Lq + i;
       const long long pr = (long long)blockIdx.y * a.B * a.Hq * a.Lq + row_at;
       float* dst = a.nsplit > 1 ? a.po + pr * a.D  // the row as it stands, for attn_join_kernel
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         a.pml[2 * pr] = M;
         a.pml[2 * pr + 1] = L;
       } else {
-        a.lse[row_at] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+        a.lse[row_at] = row_lse(M, L);
       }
     }
   }
