@@ -84,6 +84,10 @@ using namespace atc;
 
 constexpr int kFwdThreads = 384;  // three warpgroups: two of softmax, one of loader and issuer
 constexpr float kGrow = 8.f;  // log2 of the growth of a maximum that is taken without rescaling
+// Largest bias that a whole tile may keep beside its products, x mul + (add - m):
+// up to here add and m are exact to 2^-12, beyond (and for -inf, which masks) the
+// bias is added pair by pair, so that a row's maximum holds it as its scores do.
+constexpr float kFlatMost = 4096.f;
 
 struct FwdMaps {
   CUtensorMap q, k, v;
@@ -315,9 +319,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       for (int x = 0; x < 4; ++x) ptx::tmem_wait_ld(s[x]);
       // exponents are s x + c - m; without a bias by pair the products stay as they are
       float mul = 1.f, add = 0.f;
-      const bool plain = flat && sc > 0.f;
+      bool plain = flat && sc > 0.f;
       if (a.diag) {
         const float* bb = bias_s + st * 384 + 256 - 128 * w - row;
+        plain = plain && fabsf(bb[0]) <= kFlatMost;
         if (plain) {
           add = bb[0];
         } else {

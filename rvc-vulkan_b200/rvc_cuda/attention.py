@@ -241,7 +241,8 @@ def attention(q, k, v, *, kv_lens=None, key_mask=None, scale: Optional[float] = 
     0 there meets the value.
     Query head ``h`` reads key head ``h // (Hq / Hkv)``.  ``scale`` is
     ``1 / sqrt(D)`` by default; ``bias`` adds ``table[bucket(j - i - q_offset),
-    h]``.  Returns ``out [B, Lq, Hq, D]`` in the type of ``q`` and the float32
+    h]`` (an entry of ``-inf``, or the type's lowest in float32 and bfloat16,
+    masks its pairs).  Returns ``out [B, Lq, Hq, D]`` in the type of ``q`` and the float32
     log sums ``lse [B, Hq, Lq]`` that the backward pass takes; a query without
     a live key gives 0 and ``-inf``.  float32 values are worked on as parts of
     16 bits: an infinite one that is alive comes out as NaN.  Heads of 1 to 128

@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import attention as OA
 from tests.test_attention_gpu import Case, f8
 
 pytestmark = pytest.mark.gpu
@@ -73,3 +74,42 @@ def test_live_values_that_are_not_finite_are_seen(dtype, size, bad):
         col = np.zeros((B, Lq, Hq, D), bool)
         col[B - 1, :, h * g:(h + 1) * g, D - 1] = True
         assert not np.isfinite(f8(out)[col]).any() and np.isfinite(f8(out)[~col]).all() and np.isfinite(f8(lse)).all(), "value"
+
+
+# ------------------------------------------------- table entries that mask
+
+
+def with_table(c, rows, value):
+    """``c`` with rows of its table set, and what the oracle says of it: an entry
+    whose scaled form leaves float32 (-inf, the lowest bfloat16 and float32)
+    masks the pairs of its bucket."""
+    t = c.kw["bias"].table
+    t[rows] = value
+    tab = f8(t)
+    tab = np.where(tab * np.log2(np.e) < np.finfo(np.float32).min, -np.inf, tab)
+    c.tab = tab.T[:, c.where]
+    rep = lambda x: np.repeat(x, c.g, 2)  # noqa: E731
+    c.out, c.lse, c.p = OA.attention(c.q8, c.k8, c.v8, c.scale, c.live, c.tab)
+    s = OA.scores(c.q8, c.k8, c.scale, c.live, c.tab)
+    mag = np.einsum("bihd,bjhd->bhij", np.abs(c.q8), rep(np.abs(c.k8))) * abs(c.scale)
+    c.es = np.where(np.isfinite(s), 2.0 ** -20 * mag + 2.0 ** -21 * np.abs(np.where(np.isfinite(s), s, 0)), 0.0)
+    c.ep = 2 * c.es.max(-1, keepdims=True, initial=0.0) + 2.0 ** -20
+    c.pv = np.einsum("bhij,bjhd->bihd", c.p * (c.ep + c.w), rep(np.abs(c.v8)))
+    return c
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("value", ["-inf", "lowest"])
+@pytest.mark.parametrize("size", [(2, 4, 2, 64, 3, 900), (1, 2, 2, 40, 150, 700), (1, 2, 1, 128, 300, 900),
+                                  (1, 2, 2, 64, 70, 4100), (1, 2, 1, 96, 80, 260)], ids=str)
+def test_a_masked_bucket(dtype, value, size):
+    """A window: the far buckets are masked.  Queries meet far tiles first, some
+    meet nothing else; scores are large enough to overflow fp16 weights that
+    forget the bias."""
+    Lk = size[5]
+    for both, off, rows in ((True, Lk // 2, [3, 7]), (True, 5000, [3, 7]), (True, -5000, [7]), (False, Lk // 2, [7]),
+                            (True, 40, slice(None))):
+        c = Case(dtype, *size, bias=(8, 6, both), q_offset=off, scale=3.0 / np.sqrt(size[3]))
+        c = with_table(c, rows, float("-inf") if value == "-inf" else torch.finfo(c.t).min)
+        c.forward()
+        c.backward()
