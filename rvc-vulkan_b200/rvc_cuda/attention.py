@@ -195,6 +195,12 @@ def _mask(key_mask, B: int, Lk: int, like):
     return key_mask, key_mask.stride(0), key_mask.stride(1)
 
 
+def _rows(bias, t):
+    """The object's table ``t`` (which may have been replaced) has the rows that its borders lead to."""
+    if t.shape[0] != bias.num_buckets:
+        raise ValueError(f"bias: table {tuple(t.shape)}, its rows must be the {bias.num_buckets} buckets")
+
+
 def _table(bias, H: int, like):
     """The table as the kernels read it (contiguous), its size and borders."""
     if bias is None:
@@ -202,7 +208,8 @@ def _table(bias, H: int, like):
     if not isinstance(bias, BucketBias):
         raise ValueError("bias: a BucketBias is expected")
     t = _tensor(bias.table, "bias table", 2, like)
-    if t.shape != (bias.num_buckets, H):
+    _rows(bias, t)
+    if t.shape[1] != H:
         raise ValueError(f"bias: table {tuple(t.shape)}, expected [{bias.num_buckets}, {H}] for {H} query heads")
     return t.contiguous(), bias.num_buckets, int(bias.bidirectional), bias._borders, bias._nborders
 
@@ -317,6 +324,7 @@ def relative_bias(bias: BucketBias, Lq: int, Lk: int, *, q_offset: int = 0):
     if not isinstance(bias, BucketBias):
         raise ValueError("relative_bias: a BucketBias is expected")
     t = _tensor(bias.table, "bias table", 2).contiguous()
+    _rows(bias, t)
     Lq, Lk, H = int(Lq), int(Lk), t.shape[1]
     if Lq < 0 or Lk < 0:
         raise ValueError(f"relative_bias: lengths {Lq} and {Lk}")
@@ -341,6 +349,7 @@ def relative_bias_backward(bias: BucketBias, dbias, *, q_offset: int = 0):
     if d.dtype not in _TYPES:
         raise ValueError(f"dbias: float32, bfloat16 or float16 expected, got {d.dtype}")
     B, H, Lq, Lk = d.shape
+    _rows(bias, _tensor(bias.table, "bias table", 2))
     if H != bias.table.shape[1]:
         raise ValueError(f"relative_bias_backward: {H} heads, the table has {bias.table.shape[1]}")
     ctx, stream = _where(d)

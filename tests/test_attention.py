@@ -157,3 +157,15 @@ def test_rope_table_keeps_far_positions():
     # one rounding to fp32 of values up to 1
     assert np.abs(cos[69999].numpy() - np.cos(a)).max() <= 2.0 ** -24
     assert np.abs(sin[69999].numpy() - np.sin(a)).max() <= 2.0 ** -24
+
+
+def test_a_table_that_was_replaced():
+    """The object's table may be swapped, for one of as many rows only."""
+    b = A.BucketBias(t(32, 4))
+    for rows in (31, 8, 33, 0):
+        b.table = t(rows, 4)
+        refused("32 buckets", A.relative_bias, b, 3, 3)
+        refused("32 buckets", A.relative_bias_backward, b, t(4, 5, 6))
+        refused("32 buckets", A.attention, t(2, 5, 4, 16), t(2, 7, 2, 16), t(2, 7, 2, 16), bias=b)
+    b.table = t(32, 4)
+    refused("CUDA", A.relative_bias, b, 3, 3)
