@@ -15,7 +15,9 @@ synchronising, and return new contiguous tensors; scratch memory comes from
 torch's allocator, so a call can be captured into a CUDA graph (after a first
 call on the device, which opens the library's context there).  Nothing is kept
 between calls, and there is no autograd: the ``*_backward`` functions are called
-with what the forward ones returned.  A wait inside a kernel that gives up
+with what the forward ones returned, and an input that requires grad is refused
+while grad mode is on (call under ``torch.no_grad()`` or inside an
+``autograd.Function``, where it is off).  A wait inside a kernel that gives up
 (after two seconds) is reported by the next ``sync`` of the device's context,
 ``rvc_cuda._lib.get_context(i).sync()``.  ``rvc_cuda.ops`` has the forms for numpy arrays.  The
 device code and its C entry points (``include/rvc_cuda.h``) have no counterpart
@@ -146,6 +148,15 @@ def _scratch(fn, ctx, desc, n, like, *how):
     return (like.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None), nbytes
 
 
+def _no_graph(name: str, *tensors):
+    """Results have no graph behind them: a gradient that autograd was asked for would be lost without a word."""
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x is not None and x.requires_grad:
+                raise ValueError(f"{name}: an input requires grad, and this function records no graph: call it under "
+                                 "torch.no_grad() and use the *_backward functions")
+
+
 def _ptr(x):
     return x.data_ptr() if x is not None else None
 
@@ -265,6 +276,7 @@ def attention(q, k, v, *, kv_lens=None, key_mask=None, scale: Optional[float] = 
         mask, mb, mk = _mask(key_mask, B, Lk, q)
     if bias is not None:
         table, nb, both, borders, nborders = _table(bias, Hq, q)
+    _no_graph("attention", q, k, v, table)
     ctx, stream = _where(q)
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     desc = _pack29(_TYPES[q.dtype], B, Hq, Hkv, Lq, Lk, D, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1],
@@ -302,6 +314,7 @@ def attention_backward(dout, q, k, v, out, lse, *, kv_lens=None, key_mask=None, 
     lens, bits = _lens(kv_lens, B, q)
     mask, mb, mk = _mask(key_mask, B, Lk, q)
     table, nb, both, borders, nborders = _table(bias, Hq, q)
+    _no_graph("attention_backward", dout, q, k, v, out, lse, table)
     ctx, stream = _where(q)
     desc = _pack29(_TYPES[q.dtype], B, Hq, Hkv, Lq, Lk, D, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], bits, mb,
                    mk, bool(causal), _offset(q_offset), nb, both, *dout.stride()[:3], *out.stride()[:3])
@@ -328,6 +341,7 @@ def relative_bias(bias: BucketBias, Lq: int, Lk: int, *, q_offset: int = 0):
     Lq, Lk, H = int(Lq), int(Lk), t.shape[1]
     if Lq < 0 or Lk < 0:
         raise ValueError(f"relative_bias: lengths {Lq} and {Lk}")
+    _no_graph("relative_bias", t)
     ctx, stream = _where(t)
     out = t.new_empty((H, Lq, Lk))
     desc = _pack11(_TYPES[t.dtype], 1, H, Lq, Lk, _offset(q_offset), bias.num_buckets, bias.bidirectional, 0, 0, 0)
@@ -352,6 +366,7 @@ def relative_bias_backward(bias: BucketBias, dbias, *, q_offset: int = 0):
     _rows(bias, _tensor(bias.table, "bias table", 2))
     if H != bias.table.shape[1]:
         raise ValueError(f"relative_bias_backward: {H} heads, the table has {bias.table.shape[1]}")
+    _no_graph("relative_bias_backward", d)
     ctx, stream = _where(d)
     desc = _pack11(_TYPES[d.dtype], B, H, Lq, Lk, _offset(q_offset), bias.num_buckets, bias.bidirectional, *d.stride()[:3])
     dtable = d.new_empty((bias.num_buckets, H))
@@ -451,6 +466,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps: flo
     """
     q, k, wq, wk, cos, sin, pos, head = _rope(q, k, q_weight, k_weight, cos, sin, positions, interleaved,
                                               "qk_norm_rope")
+    _no_graph("qk_norm_rope", q, k, wq, wk, cos, sin)
     ctx, stream = _where(q)
     desc = _pack25(*head, 0, 0, 0, 0, 0, 0)
     qo, ko = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k))
@@ -471,6 +487,7 @@ def qk_norm_rope_backward(dqo, dko, q, k, q_weight, k_weight, cos, sin, *, posit
     if gq.shape != q.shape or gk.shape != k.shape:
         raise ValueError(f"qk_norm_rope_backward: dqo {tuple(gq.shape)}, dko {tuple(gk.shape)} for q {tuple(q.shape)}, "
                          f"k {tuple(k.shape)}")
+    _no_graph("qk_norm_rope_backward", gq, gk, q, k, wq, wk, cos, sin)
     ctx, stream = _where(q)
     desc = _pack25(*head, *gq.stride()[:3], *gk.stride()[:3])
     dq, dk = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k))

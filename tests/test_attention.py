@@ -169,3 +169,28 @@ def test_a_table_that_was_replaced():
         refused("32 buckets", A.attention, t(2, 5, 4, 16), t(2, 7, 2, 16), t(2, 7, 2, 16), bias=b)
     b.table = t(32, 4)
     refused("CUDA", A.relative_bias, b, 3, 3)
+
+
+def test_no_gradient_is_lost_silently():
+    """An input that requires grad is refused while grad mode is on; without it the call goes on (to the device)."""
+    q, k, w, c, lse = t(2, 5, 4, 16), t(2, 5, 4, 16), t(16), t(9, 8), t(2, 4, 5)
+    b, d = A.BucketBias(t(8, 4)), t(4, 5, 5)
+    calls = [
+        ([q, k, k + 0], lambda q, k, v: A.attention(q, k, v)),
+        ([b.table], lambda x: A.attention(q, k, k, bias=A.BucketBias(x))),
+        ([q, q + 0, k, k + 0, q + 0, lse], lambda do, q, k, v, o, z: A.attention_backward(do, q, k, v, o, z)),
+        ([b.table], lambda x: A.attention_backward(q, q, k, k, q, lse, bias=A.BucketBias(x))),
+        ([b.table], lambda x: A.relative_bias(A.BucketBias(x), 3, 3)),
+        ([d], lambda x: A.relative_bias_backward(b, x)),
+        ([q, k, w, w + 0, c, c + 0], lambda *x: A.qk_norm_rope(*x)),
+        ([q, k, w, w + 0, c, c + 0], lambda *x: A.qk_norm_rope(*x, positions=t(2, 5, dtype=torch.int64))),
+        ([q, k, q + 0, k + 0, w, w + 0, c, c + 0], lambda *x: A.qk_norm_rope_backward(*x)),
+    ]
+    for args, fn in calls:
+        for n in range(len(args)):
+            x = [a.detach().requires_grad_(i == n) for i, a in enumerate(args)]
+            refused("requires grad", fn, *x)
+            with torch.no_grad():
+                refused("CUDA", fn, *x)
+    x = torch.nn.Parameter(t(2, 5, 4, 16, 2))[..., 0]  # a view that has to be copied is part of a graph too
+    refused("requires grad", A.attention, x, k, k)
