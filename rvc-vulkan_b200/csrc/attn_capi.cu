@@ -6,6 +6,8 @@
 #include "context.cuh"
 #include "norm_rope.cuh"
 
+#include <cmath>
+
 using namespace rvc;
 
 // Defined beside the registry of capi.cu.
@@ -83,6 +85,12 @@ AttnArgs attn_args(const int64_t* d, int32_t n, const char* who) {
   return a;
 }
 
+// Kernels hold the scale, and the scale times log2 e, in 32 bits.
+float scale_arg(const char* who, double scale) {
+  RVC_CHECK_ARG(std::abs(scale) <= 0x1p127, std::string(who) + ": the scale is not finite in float32");
+  return (float)scale;
+}
+
 void check_ws(const char* who, const void* ws, int64_t have, int64_t need) {
   RVC_CHECK_ARG(need == 0 || (ws && reinterpret_cast<uintptr_t>(ws) % 16 == 0),
                 std::string(who) + ": the workspace is null or not aligned to 16 bytes");
@@ -128,7 +136,7 @@ int32_t rvc_cuda_attention_device(int64_t ctx, void* stream, const int64_t* desc
     RVC_CHECK_ARG((desc[16] != 0) == (kv_lens != nullptr), "attention: kv_lens and their width do not agree");
     RVC_CHECK_ARG((desc[21] != 0) == (table != nullptr), "attention: table and bucket count do not agree");
     a.q = q, a.k = k, a.v = v, a.lens = kv_lens, a.mask = key_mask;
-    a.out = out, a.lse = lse, a.scale = (float)scale, a.err = c->d_err;
+    a.out = out, a.lse = lse, a.scale = scale_arg(who, scale), a.err = c->d_err;
     BucketRule rule;
     if (desc[21]) rule = bucket_rule(desc[21], desc[22], borders, nborders, who);
     check_ws(who, ws, ws_bytes, attn_workspace(a, desc[21] > 0, false, c->num_sms()));
@@ -172,7 +180,7 @@ int32_t rvc_cuda_attention_backward_device(int64_t ctx, void* stream, const int6
       return;
     }
     a.q = q, a.k = k, a.v = v, a.lens = kv_lens, a.mask = key_mask;
-    a.dout = dout, a.fout = out, a.lse = const_cast<float*>(lse), a.scale = (float)scale;
+    a.dout = dout, a.fout = out, a.lse = const_cast<float*>(lse), a.scale = scale_arg(who, scale);
     a.dq = dq, a.dk = dk, a.dv = dv, a.err = c->d_err;
     check_ws(who, ws, ws_bytes, attn_workspace(a, desc[21] > 0, true, c->num_sms()));
     attn_backward(a, table, desc[21] ? &rule : nullptr, dtable, ws, c->num_sms(), st);

@@ -51,6 +51,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 _POSITION_BITS = {torch.int32: 32, torch.int64: 64}
 MAX_HEAD_DIM = 128
 MAX_BUCKETS = 1024
+MAX_SCALE = 2.0 ** 127  # times log2 e it is still a float32
 
 _pack29 = struct.Struct("=29q").pack
 _pack25 = struct.Struct("=25q").pack
@@ -237,8 +238,8 @@ def _offset(q_offset) -> int:
 
 def _scale(scale, D: int) -> float:
     s = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not math.isfinite(s):
-        raise ValueError(f"attention: scale {s} is not finite")
+    if not abs(s) <= MAX_SCALE:
+        raise ValueError(f"attention: scale {s} is not finite in float32")
     return s
 
 

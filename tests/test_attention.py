@@ -194,3 +194,9 @@ def test_no_gradient_is_lost_silently():
                 refused("CUDA", fn, *x)
     x = torch.nn.Parameter(t(2, 5, 4, 16, 2))[..., 0]  # a view that has to be copied is part of a graph too
     refused("requires grad", A.attention, x, k, k)
+
+
+def test_a_scale_that_float32_cannot_hold():
+    for s in (float("inf"), float("-inf"), float("nan"), 1e39, -1e39, 2.0 ** 127 * (1 + 2.0 ** -50)):
+        refused("scale", A._scale, s, 64)
+    assert A._scale(2.0 ** 127, 64) == 2.0 ** 127 and A._scale(None, 64) == 0.125

@@ -12,7 +12,7 @@ from tests.test_attention_gpu import Case, f8
 
 pytestmark = pytest.mark.gpu
 
-from rvc_cuda import attention as A  # noqa: E402
+from rvc_cuda import _lib, attention as A  # noqa: E402
 
 # B, Hq, Hkv, D, Lq, Lk: few rows (one launch, a cluster, the workspace), the general kernels with one and
 # several splits, the tiles of 16 bits, those of fp32
@@ -113,3 +113,21 @@ def test_a_masked_bucket(dtype, value, size):
         c = with_table(c, rows, float("-inf") if value == "-inf" else torch.finfo(c.t).min)
         c.forward()
         c.backward()
+
+
+def test_the_entry_points_refuse_a_scale_that_float32_cannot_hold():
+    c = Case("bf16", 1, 1, 1, 64, 1, 40)
+    desc = (A.C.c_int64 * 29)(1, 1, 1, 1, 1, 40, 64, *c.q.stride()[:3], *c.k.stride()[:3], *c.v.stride()[:3], 0, 0, 0, 0, 0,
+                              0, 0, *c.do.stride()[:3], *c.q.stride()[:3])
+    ctx, lse = _lib.get_context().handle, torch.zeros(1, device="cuda")
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    o = [torch.empty_like(x) for x in (c.q, c.q, c.k, c.v)]
+    p = [x.data_ptr() for x in (c.do, c.q, c.k, c.v, *o, lse, ws)]
+    n0 = _lib.launch_count()
+    for s in (1e39, float("inf"), float("nan")):
+        assert _lib.lib.rvc_cuda_attention_device(ctx, None, desc, 29, s, *p[1:4], None, None, None, None, 0, p[4], p[8], p[9],
+                                                  1 << 20) == _lib.RVC_E_ARG
+        assert _lib.lib.rvc_cuda_attention_backward_device(ctx, None, desc, 29, s, *p[:5], p[8], None, None, None, None, 0,
+                                                           *p[5:8], None, p[9], 1 << 20) == _lib.RVC_E_ARG
+        assert "scale" in _lib.last_error()
+    assert _lib.launch_count() == n0
