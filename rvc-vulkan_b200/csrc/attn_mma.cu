@@ -819,7 +819,11 @@ __global__ void attn_delta_kernel(const __grid_constant__ AttnArgs a, long long 
 }
 
 // A query that can meet one key at most has weight 1 there whatever the score:
-// its dS is zero, not what the roundings of P and delta leave of it.
+// its dS is zero, not what the roundings of P and delta leave of it.  Its delta
+// is this NaN, whose bits no sum gives (an infinite delta is a result, which has
+// to go on into the gradients).
+constexpr uint32_t kLone = 0x7fc01ead;
+__device__ __forceinline__ bool is_lone(float delta) { return __float_as_uint(delta) == kLone; }
 __device__ __forceinline__ bool lone_row(const AttnArgs& a, int len, long long i) {
   return (a.causal ? min((long long)len, i + a.q_off + 1) : (long long)len) <= 1;
 }
@@ -903,7 +907,7 @@ __global__ void __launch_bounds__(kT * KS) attn_mma_dq_kernel(const __grid_const
     const float z = a.lse[row];
     const bool live = z != -INFINITY && i0 + warp * 16 + g + 8 * y < a.Lq;
     lse2[y] = live ? z * kLog2e : INFINITY;  // a row that is not there or has no key: P = 0
-    delta[y] = DELTA ? 0.f : lone_row(a, len, qi[y]) ? INFINITY : a.delta[row];
+    delta[y] = DELTA ? 0.f : lone_row(a, len, qi[y]) ? __uint_as_float(kLone) : a.delta[row];
     bias[y] = a.diag ? a.diag + h * a.diag_ld + a.diag0 - qi[y] : nullptr;
   }
   const float sc = a.scale * kLog2e;
@@ -943,7 +947,7 @@ __global__ void __launch_bounds__(kT * KS) attn_mma_dq_kernel(const __grid_const
         if (a.diag && j < a.Lk) z += __ldg(bias[y] + j);
         const bool on = j < len && (!mb || mb[(int64_t)j * a.mask_k]) && (!a.causal || j <= qi[y] + a.q_off);
         const float p = on ? exp2_approx(z - lse2[y]) : 0.f;
-        s[n][x] = p != 0.f && (DELTA || delta[y] != INFINITY) ? p * (dp[n][x] - (DELTA ? 0.f : delta[y])) : 0.f;
+        s[n][x] = p != 0.f && (DELTA || !is_lone(delta[y])) ? p * (dp[n][x] - (DELTA ? 0.f : delta[y])) : 0.f;
         if (DELTA) delta[y] += s[n][x];
         if (dws) sD[(warp * 16 + g + 8 * y) * SL + key0 + n * 8 + 2 * t + (x & 1)] = s[n][x];
       }
@@ -1043,7 +1047,7 @@ __global__ void __launch_bounds__(kT * KS) attn_mma_dkv_kernel(const __grid_cons
       const long long row = ((long long)b * a.Hq + h) * a.Lq + i0 + tid;
       const float z = in ? a.lse[row] : -INFINITY;
       stat[(st * 2) * BQ + tid] = z != -INFINITY ? z * kLog2e : INFINITY;
-      stat[(st * 2 + 1) * BQ + tid] = !in ? 0.f : lone_row(a, len, i0 + tid) ? INFINITY : a.delta[row];
+      stat[(st * 2 + 1) * BQ + tid] = !in ? 0.f : lone_row(a, len, i0 + tid) ? __uint_as_float(kLone) : a.delta[row];
     }
     cp_commit();
   };
@@ -1100,7 +1104,7 @@ __global__ void __launch_bounds__(kT * KS) attn_mma_dkv_kernel(const __grid_cons
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const float de = stat[(st * 2 + 1) * BQ + row0 + n * 8 + 2 * t + (x & 1)];
-        s[n][x] = s[n][x] != 0.f && de != INFINITY ? s[n][x] * (dp[n][x] - de) : 0.f;
+        s[n][x] = s[n][x] != 0.f && !is_lone(de) ? s[n][x] * (dp[n][x] - de) : 0.f;
       }
     mma_pb<T, DP, NT>(dk, s, q, lane);
     __syncthreads();

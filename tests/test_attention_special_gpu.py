@@ -131,3 +131,23 @@ def test_the_entry_points_refuse_a_scale_that_float32_cannot_hold():
                                                            *p[5:8], None, p[9], 1 << 20) == _lib.RVC_E_ARG
         assert "scale" in _lib.last_error()
     assert _lib.launch_count() == n0
+
+
+# ----------------------------------------------------------- infinite gradients
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("size", [(1, 2, 1, 64, 1, 40), (2, 2, 2, 33, 5, 70), (1, 2, 1, 64, 80, 300), (1, 1, 1, 128, 9, 400)],
+                         ids=str)
+def test_an_infinite_gradient_is_seen(dtype, size):
+    """A loss scale that overflowed: dq and dk must not look as if nothing was."""
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        c = Case(dtype, *size)
+        i, h, g = size[4] // 2, 0, size[1] // size[2]
+        v, do = c.v.abs() + 0.1, c.do.clone()
+        do[0, i, h, 1] = bad
+        out, lse = A.attention(c.q, c.k, v)
+        dq, dk, dv = A.attention_backward(do, c.q, c.k, v, out, lse)
+        assert not torch.isfinite(dq[0, i, h]).any() and torch.isfinite(dq[0, i, g:]).all()
+        assert not torch.isfinite(dk[0, :, 0]).any() and not torch.isfinite(dv[0, :, 0, 1]).any()
+        assert torch.isfinite(dk[1:]).all() and torch.isfinite(dv[1:]).all() and torch.isfinite(dq[1:]).all()
