@@ -91,6 +91,40 @@ __device__ __forceinline__ int kv_len(const AttnArgs& a, int b) {
   return (int)max(n, 0ll);
 }
 
+// The second key that is alive by the mask's bytes, `len` when there is none.
+// Called by whole warps; all but nearly empty masks end the search with the first
+// 256 keys.  (Not inlined: inside the gradients' kernels it cost the fp32 ones
+// registers and 3 % of their time.)
+static __device__ __noinline__ int second_key(const uint8_t* mb, int64_t stride, int len) {
+  const int lane = threadIdx.x & 31;
+  int seen = 0, second = len;
+  for (int j0 = 0; j0 < len && seen < 2; j0 += 256) {
+    uint8_t byte[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int j = j0 + 32 * x + lane;
+      byte[x] = j < len ? mb[(int64_t)j * stride] : 0;
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const uint32_t word = __ballot_sync(0xffffffffu, byte[x] != 0), rest = seen ? word : word & (word - 1);
+      if (seen < 2 && rest) second = j0 + 32 * x + __ffs(rest) - 1;
+      seen += __popc(word);
+    }
+  }
+  return second;
+}
+
+// Queries before this one can meet one key of batch entry b at most, by length,
+// mask and causal limit (entries of the bias that mask a pair are not looked at).
+// Such a query's weight is 1 whatever the score: its dS is zero, not what the
+// roundings of P and delta leave of it.  Called by whole warps.
+__device__ __forceinline__ int lone_queries(const AttnArgs& a, int b, int len) {
+  const int second = a.mask ? second_key(a.mask + (int64_t)b * a.mask_b, a.mask_k, len) : 1;
+  if (len <= second) return a.Lq;
+  return a.causal ? (int)max(0ll, min((long long)a.Lq, second - (long long)a.q_off)) : 0;
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

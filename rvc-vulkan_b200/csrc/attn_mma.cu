@@ -818,15 +818,11 @@ __global__ void attn_delta_kernel(const __grid_constant__ AttnArgs a, long long 
   if (lane == 0) a.delta[row] = s;
 }
 
-// A query that can meet one key at most has weight 1 there whatever the score:
-// its dS is zero, not what the roundings of P and delta leave of it.  Its delta
-// is this NaN, whose bits no sum gives (an infinite delta is a result, which has
-// to go on into the gradients).
+// The delta of a query with one key at most (lone_queries) is this NaN, whose bits
+// no sum gives (an infinite delta is a result, which has to go on into the
+// gradients).
 constexpr uint32_t kLone = 0x7fc01ead;
 __device__ __forceinline__ bool is_lone(float delta) { return __float_as_uint(delta) == kLone; }
-__device__ __forceinline__ bool lone_row(const AttnArgs& a, int len, long long i) {
-  return (a.causal ? min((long long)len, i + a.q_off + 1) : (long long)len) <= 1;
-}
 
 // The second half's accumulators added to the first's, through shared memory
 // that nobody reads any more; false for the second half, which is done.
@@ -897,6 +893,7 @@ __global__ void __launch_bounds__(kT * KS) attn_mma_dq_kernel(const __grid_const
     cp_commit();
   };
   if (ST == 2 && tiles > 0) load(0, 0);
+  const int lone = DELTA ? 0 : lone_queries(a, b, len);
   long long qi[2];
   float lse2[2], delta[2];
   const float* bias[2];
@@ -907,7 +904,7 @@ __global__ void __launch_bounds__(kT * KS) attn_mma_dq_kernel(const __grid_const
     const float z = a.lse[row];
     const bool live = z != -INFINITY && i0 + warp * 16 + g + 8 * y < a.Lq;
     lse2[y] = live ? z * kLog2e : INFINITY;  // a row that is not there or has no key: P = 0
-    delta[y] = DELTA ? 0.f : lone_row(a, len, qi[y]) ? __uint_as_float(kLone) : a.delta[row];
+    delta[y] = DELTA ? 0.f : qi[y] < lone ? __uint_as_float(kLone) : a.delta[row];
     bias[y] = a.diag ? a.diag + h * a.diag_ld + a.diag0 - qi[y] : nullptr;
   }
   const float sc = a.scale * kLog2e;
@@ -1033,6 +1030,7 @@ __global__ void __launch_bounds__(kT * KS) attn_mma_dkv_kernel(const __grid_cons
   if (a.causal) ifirst = max(0ll, (long long)j0 - a.q_off) / BQ * BQ;
   const int per = j0 < len && ifirst < a.Lq ? (int)((a.Lq - ifirst + BQ - 1) / BQ) : 0;
   const long long tiles = (long long)per * G;
+  const int lone = tiles > 0 ? lone_queries(a, b, len) : 0;
   auto load = [&](long long tile, int st) {
     const int h = kh * G + (int)(tile / per);
     const long long i0 = ifirst + (tile % per) * BQ;
@@ -1047,7 +1045,7 @@ __global__ void __launch_bounds__(kT * KS) attn_mma_dkv_kernel(const __grid_cons
       const long long row = ((long long)b * a.Hq + h) * a.Lq + i0 + tid;
       const float z = in ? a.lse[row] : -INFINITY;
       stat[(st * 2) * BQ + tid] = z != -INFINITY ? z * kLog2e : INFINITY;
-      stat[(st * 2 + 1) * BQ + tid] = !in ? 0.f : lone_row(a, len, i0 + tid) ? __uint_as_float(kLone) : a.delta[row];
+      stat[(st * 2 + 1) * BQ + tid] = !in ? 0.f : i0 + tid < lone ? __uint_as_float(kLone) : a.delta[row];
     }
     cp_commit();
   };

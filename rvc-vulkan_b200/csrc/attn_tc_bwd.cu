@@ -316,6 +316,7 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
       byte1 = y0 + 32 + lane < len ? mb[(int64_t)(y0 + 32 + lane) * a.mask_k] : 0;
     };
     if (!KV && mb) fetch(64 * w);
+    const int lone = tiles > 0 ? lone_queries(a, b, len) : 0;  // queries whose dS is zero: the first ones
     for (int t = w; t < tiles; t += GR) {
       const int st = t % R;
       const uint32_t turn = (t / GR) & 1;
@@ -413,6 +414,11 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(P_READY + 8 * w);
 
+        if (KV ? lone > y0 : x < lone) {
+          const int n = KV ? lone - y0 : 64;
+          alive[0] &= ~low_bits(n), alive[1] &= ~low_bits(n - 32);
+          cut = true;
+        }
         if (!(ok = warp_wait(DP_FULL + 8 * w, turn))) break;
         ptx::tc_fence_after();
         uint64_t sum = f32x2(0.f, 0.f);

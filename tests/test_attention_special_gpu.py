@@ -151,3 +151,31 @@ def test_an_infinite_gradient_is_seen(dtype, size):
         assert not torch.isfinite(dq[0, i, h]).any() and torch.isfinite(dq[0, i, g:]).all()
         assert not torch.isfinite(dk[0, :, 0]).any() and not torch.isfinite(dv[0, :, 0, 1]).any()
         assert torch.isfinite(dk[1:]).all() and torch.isfinite(dv[1:]).all() and torch.isfinite(dq[1:]).all()
+
+
+# --------------------------------------------------- queries that meet one key
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("size", [(2, 4, 2, 64, 70, 300), (2, 2, 1, 128, 150, 400), (2, 3, 3, 40, 9, 700),
+                                  (2, 2, 2, 64, 300, 300), (2, 2, 1, 64, 5, 40)], ids=str)
+def test_queries_with_one_live_key(dtype, size):
+    """A softmax over one key is 1, whether the length, the mask or the causal
+    limit leaves it: exactly no gradient reaches q, the key or the table from there."""
+    B, Lq, Lk = size[0], size[4], size[5]
+    one = np.zeros((B, Lk), bool)
+    one[0, 0] = one[1, Lk - 1] = True
+    two = one.copy()
+    two[:, Lk // 2] = True
+    none = one.copy()
+    none[1] = False
+    one, two, none = one.tolist(), two.tolist(), none.tolist()
+    for kw in (dict(lens=[1, 1]), dict(keep=one), dict(keep=none), dict(causal=True), dict(keep=two, causal=True, q_offset=3),
+               dict(keep=two, lens=[Lk, Lk // 2 + 1]), dict(causal=True, q_offset=1 - Lq), dict(lens=[1, Lk], causal=True)):
+        c = Case(dtype, *size, bias=(8, 6, True), **kw)
+        dq, dk, _, dt = c.backward()
+        lone = torch.from_numpy(c.live.sum(-1) <= 1).cuda()
+        assert (dq[lone] == 0).all(), kw
+        for b in range(B):
+            assert not lone[b].all() or (dk[b] == 0).all(), kw
+        assert not lone.all() or (dt == 0).all(), kw
