@@ -374,10 +374,11 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
         if (KV) {
           // causal: queries c with y0 + c + q_off < key are out
           const long long lo = a.causal ? x - a.q_off - y0 : 0;
-          cut = dead || lo > 0;
+          const int rest = a.Lq - y0;  // rows past the last query are out too: they may meet any entry of the table
+          cut = dead || lo > 0 || rest < 64;
           if (cut) {
             const int n = dead ? 64 : (int)min(64ll, lo);
-            alive[0] = ~low_bits(n), alive[1] = ~low_bits(n - 32);
+            alive[0] = ~low_bits(n) & low_bits(rest), alive[1] = ~low_bits(n - 32) & low_bits(rest - 32);
           }
         } else {
           const long long lim = (a.causal ? min((long long)len, x + a.q_off + 1) : (long long)len) - y0;

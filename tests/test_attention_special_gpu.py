@@ -179,3 +179,24 @@ def test_queries_with_one_live_key(dtype, size):
         for b in range(B):
             assert not lone[b].all() or (dk[b] == 0).all(), kw
         assert not lone.all() or (dt == 0).all(), kw
+
+
+# ------------------------------------------------- table rows that no pair uses
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("size", [(1, 2, 2, 64, 70, 300), (2, 4, 2, 128, 129, 260), (1, 2, 1, 40, 5, 270), (1, 2, 1, 64, 3, 50)],
+                         ids=str)
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_entries_that_no_pair_uses_reach_nothing(dtype, size, value):
+    """Buckets past the call's distances may hold anything: rows and keys that pad
+    a tile lie at such distances."""
+    for both, off in ((True, 0), (True, size[5] - size[4]), (False, size[5]), (True, 2 * size[5])):
+        c = Case(dtype, *size, bias=(64, 8000, both), q_offset=off, lens=[size[5]] + [size[5] - 7] * (size[0] - 1))
+        used = np.unique(c.where[c.live.any(0)])
+        rest = torch.ones(64, dtype=torch.bool, device="cuda")
+        rest[torch.from_numpy(used).cuda()] = False
+        c.kw["bias"].table[rest] = value
+        c.forward()
+        got = c.backward()
+        assert all(torch.isfinite(x).all() for x in got)
