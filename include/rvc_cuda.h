@@ -413,11 +413,12 @@ int32_t rvc_cuda_to_int16(int64_t ctx, const float* x, int64_t n, int16_t* y);
  * weight there is 0, which meets the value).  A query without a live key gives
  * out = 0, lse = -inf and zero gradients.
  * table [buckets, Hq] (in `type`) adds table[bucket(j - i - q_offset), h] to the
- * scaled score; an entry below -2.36e38 (-inf, the lowest float32 or bfloat16)
- * masks its pairs, as scores are held times log2 e in float32, and a query whose
- * pairs are all masked has no live key.  borders (host, int32) are the smallest
- * distances of the buckets 1, 2, ... of one direction.  out [B, Lq, Hq, D] contiguous, lse [B, Hq, Lq]
- * float32 (natural logarithm). */
+ * scaled score; an entry below -65536 (-inf, -1e9, the lowest float32 or bfloat16)
+ * masks its pairs, and a query whose pairs are all masked has no live key.  Other
+ * entries and scores are meant to stay below 1e5 in size: gradients take their
+ * weights from the float32 log sums.  borders (host, int32) are the smallest
+ * distances of the buckets 1, 2, ... of one direction.  out [B, Lq, Hq, D]
+ * contiguous, lse [B, Hq, Lq] float32 (natural logarithm). */
 int32_t rvc_cuda_attention_workspace(int64_t ctx, const int64_t* desc, int32_t ndesc, int32_t backward,
                                      int64_t* bytes);
 int32_t rvc_cuda_attention_device(int64_t ctx, void* stream, const int64_t* desc, int32_t ndesc, double scale,

@@ -12,13 +12,23 @@ namespace {
 constexpr int64_t kAlign = 256;
 int64_t up(int64_t n, int64_t g = kAlign) { return (n + g - 1) / g * g; }
 
+// Entries below this mask their pairs, as -inf does.  Further down a score keeps
+// nothing of its product in 32 bits, and the log sum of a row that meets only
+// such entries, which the backward pass takes the weights from, is off by more
+// than the weights themselves: at -1e9 by factors of 2^64.  The lowest float16
+// (-65504) is still a number; its log sums are good to 2^-8.
+constexpr float kMasked = -65536.f;
+
 template <typename T>
 __global__ void expand_bias_kernel(const T* __restrict__ table, int H, long long ld, long long d0, float mul,
                                    const __grid_constant__ BucketRule rule, float* __restrict__ diag) {
   const long long x = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (x >= ld) return;
   const int b = bucket_of(rule, x - d0);
-  for (int h = 0; h < H; ++h) diag[h * ld + x] = to_f(table[(long long)b * H + h]) * mul;
+  for (int h = 0; h < H; ++h) {
+    const float t = to_f(table[(long long)b * H + h]);
+    diag[h * ld + x] = t < kMasked ? -INFINITY : t * mul;
+  }
 }
 
 // sums[h][x] = sum over batch entries and tiles of the diagonal j - i = x - (Lq - 1).

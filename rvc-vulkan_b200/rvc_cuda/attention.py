@@ -260,8 +260,9 @@ def attention(q, k, v, *, kv_lens=None, key_mask=None, scale: Optional[float] = 
     0 there meets the value.
     Query head ``h`` reads key head ``h // (Hq / Hkv)``.  ``scale`` is
     ``1 / sqrt(D)`` by default; ``bias`` adds ``table[bucket(j - i - q_offset),
-    h]`` (an entry of ``-inf``, or the type's lowest in float32 and bfloat16,
-    masks its pairs).  Returns ``out [B, Lq, Hq, D]`` in the type of ``q`` and the float32
+    h]`` (an entry below -65536 masks its pairs: ``-inf``, ``-1e9``, the lowest
+    float32 and bfloat16).  Other entries and scores are meant to stay below 1e5
+    in size, as gradients take their weights from the float32 log sums.  Returns ``out [B, Lq, Hq, D]`` in the type of ``q`` and the float32
     log sums ``lse [B, Hq, Lq]`` that the backward pass takes; a query without
     a live key gives 0 and ``-inf``.  float32 values are worked on as parts of
     16 bits: an infinite one that is alive comes out as NaN.  Heads of 1 to 128

@@ -200,3 +200,23 @@ def test_entries_that_no_pair_uses_reach_nothing(dtype, size, value):
         c.forward()
         got = c.backward()
         assert all(torch.isfinite(x).all() for x in got)
+
+
+# ------------------------------------------------- table entries far below zero
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("value", [-70000.0, -1e9, -1e30])
+@pytest.mark.parametrize("size", [(2, 4, 2, 64, 3, 900), (1, 2, 2, 40, 150, 700), (1, 2, 1, 128, 300, 900), (1, 2, 2, 64, 70, 4100)],
+                         ids=str)
+def test_entries_far_below_zero_mask(dtype, value, size):
+    """Queries whose every pair has such an entry have no live key; the gradients
+    of the others are what they are without those pairs."""
+    Lk = size[5]
+    for both, off, rows in ((True, Lk // 2, [3, 7]), (True, 5000, [3, 7]), (True, -5000, [7]), (False, Lk // 2, [7]),
+                            (True, 40, slice(None))):
+        c = Case(dtype, *size, bias=(8, 6, both), q_offset=off)
+        c = with_table(c, rows, float("-inf"))
+        c.kw["bias"].table[rows] = value
+        c.forward()
+        c.backward()
