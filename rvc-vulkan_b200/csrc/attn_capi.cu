@@ -104,6 +104,10 @@ void check_ptr(const char* who, const char* name, const void* p, int64_t size) {
   RVC_CHECK_ARG(reinterpret_cast<uintptr_t>(p) % size == 0, std::string(who) + ": misaligned " + name);
 }
 
+void check_opt(const char* who, const char* name, const void* p, int64_t size) {
+  if (p && size) check_ptr(who, name, p, size);
+}
+
 void zero(void* p, int64_t bytes, cudaStream_t st) {
   if (bytes > 0) RVC_CUDA_TRY(cudaMemsetAsync(p, 0, bytes, st));
 }
@@ -135,6 +139,8 @@ int32_t rvc_cuda_attention_device(int64_t ctx, void* stream, const int64_t* desc
     check_ptr(who, "lse", lse, 4);
     RVC_CHECK_ARG((desc[16] != 0) == (kv_lens != nullptr), "attention: kv_lens and their width do not agree");
     RVC_CHECK_ARG((desc[21] != 0) == (table != nullptr), "attention: table and bucket count do not agree");
+    check_opt(who, "kv_lens", kv_lens, desc[16] / 8);
+    check_opt(who, "table", table, es);
     a.q = q, a.k = k, a.v = v, a.lens = kv_lens, a.mask = key_mask;
     a.out = out, a.lse = lse, a.scale = scale_arg(who, scale), a.err = c->d_err;
     BucketRule rule;
@@ -157,6 +163,8 @@ int32_t rvc_cuda_attention_backward_device(int64_t ctx, void* stream, const int6
     RVC_CHECK_ARG((desc[16] != 0) == (kv_lens != nullptr) || a.B == 0,
                   "attention_backward: kv_lens and their width do not agree");
     RVC_CHECK_ARG((desc[21] != 0) == (table != nullptr), "attention_backward: table and bucket count do not agree");
+    check_opt(who, "kv_lens", kv_lens, desc[16] / 8);
+    check_opt(who, "table", table, es);
     if (rows > 0) {
       check_ptr(who, "dout", dout, es), check_ptr(who, "q", q, es), check_ptr(who, "out", out, es);
       check_ptr(who, "lse", lse, 4);
@@ -267,6 +275,7 @@ static void rope_tables(RopeArgs& a, const int64_t* d, const float* cos, const f
                         const char* who) {
   if (a.R > 0 && a.P > 0) check_ptr(who, "cos", cos, 4), check_ptr(who, "sin", sin, 4);
   RVC_CHECK_ARG((d[10] != 0) == (pos != nullptr), std::string(who) + ": positions and their width do not agree");
+  check_opt(who, "positions", pos, d[10] / 8);
   RVC_CHECK_ARG(pos || a.R == 0 || a.L <= a.P, std::string(who) + ": the tables hold " + std::to_string(a.P) +
                                                    " positions, fewer than the rows");
   a.cos = cos, a.sin = sin, a.pos = pos;

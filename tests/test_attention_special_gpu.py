@@ -220,3 +220,39 @@ def test_entries_far_below_zero_mask(dtype, value, size):
         c.kw["bias"].table[rows] = value
         c.forward()
         c.backward()
+
+
+# ----------------------------------------------------- pointers of the C calls
+
+
+def test_the_entry_points_refuse_misaligned_lengths_tables_and_positions():
+    """A value that lies across its size would fault the device: refused before any launch."""
+    c = Case("fp32", 2, 2, 2, 64, 3, 40, lens=[40, 3], bias=(8, 6, True))
+    ctx, n0 = _lib.get_context().handle, _lib.launch_count()
+    bias, borders, nb = c.kw["bias"], c.kw["bias"]._borders, c.kw["bias"]._nborders
+    room = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    at = room.data_ptr()
+    o = [torch.empty_like(x) for x in (c.q, c.q, c.k, c.v)]
+    p = [x.data_ptr() for x in (c.do, c.q, c.k, c.v, *o)]
+    lse = torch.zeros(2, 2, 3, device="cuda").data_ptr()
+    for bits, lens, table, word in ((32, at + 2, at, "kv_lens"), (64, at + 4, at, "kv_lens"), (32, at, at + 2, "table")):
+        desc = (A.C.c_int64 * 29)(0, 2, 2, 2, 3, 40, 64, *c.q.stride()[:3], *c.k.stride()[:3], *c.v.stride()[:3], bits, 0, 0,
+                                  0, 0, 8, 1, *c.do.stride()[:3], *c.q.stride()[:3])
+        assert _lib.lib.rvc_cuda_attention_device(ctx, None, desc, 29, 0.125, *p[1:4], lens, None, table, borders, nb, p[4],
+                                                  lse, at, 1 << 20) == _lib.RVC_E_ARG
+        assert word in _lib.last_error() and "misaligned" in _lib.last_error()
+        assert _lib.lib.rvc_cuda_attention_backward_device(ctx, None, desc, 29, 0.125, *p[:4], p[4], lse, lens, None, table,
+                                                           borders, nb, *p[5:8], bias.table.data_ptr(), at, 1 << 20) == _lib.RVC_E_ARG
+        assert word in _lib.last_error() and "misaligned" in _lib.last_error()
+    cos, sin = (x.data_ptr() for x in A.rope_table(9, 64, device="cuda"))
+    w = torch.ones(64, device="cuda").data_ptr()
+    for bits, pos in ((32, at + 2), (64, at + 4)):
+        desc = (A.C.c_int64 * 25)(0, 0, 2, 3, 2, 2, 64, 64, 9, 0, bits, 3, 1, *c.q.stride()[:3], *c.q.stride()[:3],
+                                  *c.q.stride()[:3], *c.q.stride()[:3])
+        assert _lib.lib.rvc_cuda_qk_norm_rope_device(ctx, None, desc, 25, 1e-6, p[1], p[1], w, w, cos, sin, pos, p[4],
+                                                     p[5]) == _lib.RVC_E_ARG
+        assert "misaligned positions" in _lib.last_error()
+        assert _lib.lib.rvc_cuda_qk_norm_rope_backward_device(ctx, None, desc, 25, 1e-6, p[0], p[0], p[1], p[1], w, w, cos,
+                                                              sin, pos, p[4], p[5], w, w, at, 1 << 20) == _lib.RVC_E_ARG
+        assert "misaligned positions" in _lib.last_error()
+    assert _lib.launch_count() == n0
