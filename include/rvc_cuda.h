@@ -396,10 +396,12 @@ int32_t rvc_cuda_to_int16(int64_t ctx, const float* x, int64_t n, int16_t* y);
  * runtime/models/vits.py:993-1014 and runtime/models/hubert.py:1315-1400).
  * All pointers but `desc` and `borders` are DEVICE pointers; the calls are
  * asynchronous on `stream` (a cudaStream_t of the context's device, NULL = its
- * default stream) and touch no memory of the context: scratch is the caller's
- * `ws` (16-byte aligned, at least the bytes that the matching *_workspace call
- * gives), so calls on several streams, and captured graphs, run side by side as
- * long as each has its own.  Types: 0 = float32, 1 = bfloat16, 2 = float16.
+ * default stream) and of the context's memory touch the error word only: scratch
+ * is the caller's `ws` (16-byte aligned, at least the bytes that the matching
+ * *_workspace call gives), so calls on several streams, and captured graphs, run
+ * side by side as long as each has its own.  A wait inside a kernel that gives up
+ * (after two seconds) leaves NaN in the results that waited and sets the error
+ * word, which the context's next rvc_cuda_sync reports.  Types: 0 = float32, 1 = bfloat16, 2 = float16.
  * Strides count elements; the D values of a head are contiguous.
  *
  * desc of attention: {type, B, Hq, Hkv, Lq, Lk, D, q stride (batch, row, head),

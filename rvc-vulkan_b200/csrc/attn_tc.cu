@@ -18,8 +18,8 @@
 // A tile's dead keys get s = -inf; their rows of V are zeroed in shared memory
 // first, so that nothing a padded buffer holds reaches a product.
 //
-// Every wait is bounded; one that gives up sets the context's error word and
-// lets the block wind down.
+// Every wait is bounded; one that gives up sets the context's error word, lets the
+// block wind down and leaves NaN in the rows that are not finished.
 //
 // Measured: 2 x 16/4 heads x 2048 x 16384 x 128, bf16: 485 to 551 us, 1.0 to 1.13
 // PFLOP/s of 1.70; the same pipeline with the softmax taken out takes 433, so the
@@ -417,11 +417,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       ok = warp_wait(O_DONE + 8 * w, (tiles - 1) & 1);
       ptx::tc_fence_after();
     }
-    if (!ok) {
-      if (lane == 0) atomicExch(a.err, 43);
-    } else {
+    if (!ok && lane == 0) atomicExch(a.err, 43);
+    {
       const bool part = a.nsplit > 1;  // the row as it stands, for attn_join_kernel
-      const float inv = part ? 1.f : row_inv(l);
+      const float inv = part || !ok ? 1.f : row_inv(l);
       T* dst = static_cast<T*>(a.out) + (((long long)b * a.Lq + i) * a.Hq + h) * a.D;
       const long long row_at = ((long long)b * a.Hq + h) * a.Lq + i;
       const long long pr = (long long)blockIdx.y * a.B * a.Hq * a.Lq + row_at;
@@ -429,11 +428,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       for (int x = 0; x < 64 * NS; x += 16) {
         if (x >= a.D) break;
         float o[16];
-        if (tiles > 0) {
+        if (ok && tiles > 0) {
           ptx::tmem_ld16(o_col + x, o);
         } else {
 #pragma unroll
-          for (int c = 0; c < 16; ++c) o[c] = 0.f;
+          for (int c = 0; c < 16; ++c) o[c] = ok ? 0.f : no_result();
         }
         if (i < a.Lq && part) {
 #pragma unroll
@@ -451,9 +450,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       }
       if (i < a.Lq && part) {
         a.pml[2 * pr] = m;
-        a.pml[2 * pr + 1] = l;
+        a.pml[2 * pr + 1] = ok ? l : no_result();
       } else if (i < a.Lq) {
-        a.lse[row_at] = row_lse(m, l);
+        a.lse[row_at] = ok ? row_lse(m, l) : no_result();
       }
     }
   }

@@ -12,6 +12,8 @@ namespace rvc {
 namespace atc {
 
 constexpr uint64_t kWaitNs = 2000000000ull;
+// What stands in results whose waits gave up.
+__device__ __forceinline__ float no_result() { return __uint_as_float(0x7fffffffu); }
 
 // A tile is [128 rows][64 values of 16 bits] per slab, 128 bytes to a row,
 // 16-byte chunks permuted by the row (TMA's 128-byte swizzle), slabs 16 KB apart.

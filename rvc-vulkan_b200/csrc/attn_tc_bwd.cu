@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
                  Y2_EMPTY = Y1_EMPTY + 8 * R, S_FULL = Y2_EMPTY + 8 * R /* [2 groups] each from here */,
                  DP_FULL = S_FULL + 16, P_READY = S_FULL + 32, DS_READY = S_FULL + 48, DONE = S_FULL + 64;
   uint32_t* slot = reinterpret_cast<uint32_t*>(gen + oBar + 504);
+  volatile uint32_t* undone = slot + 1;  // products that were not issued, set before DONE
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   const int group = a.Hq / a.Hkv;
@@ -127,7 +128,8 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
       ptx::mbar_init(P_READY + 8 * w, 4);
       ptx::mbar_init(DS_READY + 8 * w, 4);
     }
-    ptx::mbar_init(DONE, 1);
+    ptx::mbar_init(DONE, 2);
+    *undone = 0;
     ptx::fence_mbar_init();
   }
   if (warp == kIssue) {
@@ -245,8 +247,12 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
         }
         if (t + 1 < tiles) issue_dp(t + 1);
       }
-      if (!ok) atomicExch(a.err, 52);
+      if (!ok) {
+        atomicExch(a.err, 52);
+        *undone = 1;
+      }
       ptx::mma_commit(DONE);
+      ptx::mbar_arrive(DONE);
       bar_wait(DONE, 0);  // every product done before tensor memory is freed
     }
     __syncwarp();
@@ -520,10 +526,16 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
     }
     if (KV && a.dws && ok)
       for (; head < G; ++head) end_head(h0 + head);
-    if (ok && tiles > 0) ok = warp_wait(DONE, 0);
+    if (ok && tiles > 0) ok = warp_wait(DONE, 0) && *undone == 0;
     ptx::tc_fence_after();
-    if (!ok) {
+    if (KV && a.dws) ok = ptx::named_bar_and(1 + w, 128, ok);
+    if (!ok) {  // a wait gave up: NaN in what this block was to write
       if (lane == 0) atomicExch(a.err, 53);
+      if (KV && a.dws)
+        for (int hy = h0; hy < h0 + G; ++hy) {
+          float* dws = a.dws + ((((int64_t)b * a.Hq + hy) * ntile + xt) * GR + w) * a.dws_ld;
+          for (int64_t z = row; z < a.dws_ld; z += 128) dws[z] = no_result();
+        }
     }
     float rr = 0.f;
     if (!KV) {
@@ -536,11 +548,11 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
       }
       if (w == 0) {
         const int64_t to = ((int64_t)b * a.Hq + hx) * Lp + x;
-        a.lse2[to] = nl;
+        a.lse2[to] = ok ? nl : no_result();
         a.delta[to] = nl == -INFINITY ? 0.f : nt - rr;
       }
     }
-    if (ok) {
+    {
       const int L = KV ? a.Lk : a.Lq;
       const int64_t to = (((int64_t)b * L + x) * heads + hx) * a.D;
       T* d1 = static_cast<T*>(KV ? a.dk : a.dq) + to;
@@ -549,12 +561,12 @@ __global__ void __launch_bounds__(kBwdThreads<NS>, NS == 1 ? 2 : 1)
       for (int c0 = 64 * NS / GR * w; c0 < 64 * NS / GR * (w + 1); c0 += 16) {  // each group its share of the values
         if (c0 >= a.D) break;
         float u[16], v[16];
-        if (tiles > 0) {
+        if (ok && tiles > 0) {
           ptx::tmem_ld16(tA1 + lanes + c0, u);
           ptx::tmem_ld16(tA2 + lanes + c0, v);
         } else {
 #pragma unroll
-          for (int c = 0; c < 16; ++c) u[c] = v[c] = 0.f;
+          for (int c = 0; c < 16; ++c) u[c] = v[c] = ok ? 0.f : no_result();
         }
         if (x >= L) continue;
         if (KV && a.nsplit > 1) {  // this share's part, for kv_join_kernel

@@ -357,9 +357,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       part[65 * 128] = l;
     }
     ptx::named_bar(1, 256);
-    if (!ok) {
-      if (lane == 0) atomicExch(a.err, 63);
-    } else if (w == 0 && i < a.Lq) {
+    if (!ok && lane == 0) atomicExch(a.err, 63);
+    if (w == 0 && i < a.Lq) {
       const float m1 = part[64 * 128], M = fmaxf(m, m1), off = M == -INFINITY ? 0.f : M;
       const float f0 = exp2_approx(m - off), f1 = exp2_approx(m1 - off);
       const float L = f0 * l + f1 * part[65 * 128], inv = a.nsplit > 1 ? 1.f : row_inv(L);
@@ -374,14 +373,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           split2(o[c / 2], u[0], u[1]);
           split2(o[c / 2 + 1], u[2], u[3]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) u[k] = (f0 * u[k] + f1 * part[(c + k) * 128]) * inv;
+          for (int k = 0; k < 4; ++k) u[k] = ok ? (f0 * u[k] + f1 * part[(c + k) * 128]) * inv : no_result();
           *reinterpret_cast<float4*>(dst + c) = make_float4(u[0], u[1], u[2], u[3]);
         }
       if (a.nsplit > 1) {
         a.pml[2 * pr] = M;
-        a.pml[2 * pr + 1] = L;
+        a.pml[2 * pr + 1] = ok ? L : no_result();
       } else {
-        a.lse[row_at] = row_lse(M, L);
+        a.lse[row_at] = ok ? row_lse(M, L) : no_result();
       }
     }
   }

@@ -18,9 +18,9 @@ between calls, and there is no autograd: the ``*_backward`` functions are called
 with what the forward ones returned, and an input that requires grad is refused
 while grad mode is on (call under ``torch.no_grad()`` or inside an
 ``autograd.Function``, where it is off).  A wait inside a kernel that gives up
-(after two seconds) is reported by the next ``sync`` of the device's context,
-``rvc_cuda._lib.get_context(i).sync()``.  ``rvc_cuda.ops`` has the forms for numpy arrays.  The
-device code and its C entry points (``include/rvc_cuda.h``) have no counterpart
+(after two seconds) leaves NaN in the results that waited and is reported by the
+next ``sync`` of the device's context, ``rvc_cuda._lib.get_context(i).sync()``.
+``rvc_cuda.ops`` has the forms for numpy arrays.  The device code and its C entry points (``include/rvc_cuda.h``) have no counterpart
 in the reference, whose attention (``runtime/models/vits.py:993-1014``,
 ``runtime/models/hubert.py:1315-1400``) has one length, no padding and no
 gradient.  A shape, type or argument that is not served raises ``ValueError``.
