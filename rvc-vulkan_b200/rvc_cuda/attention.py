@@ -236,6 +236,16 @@ def _offset(q_offset) -> int:
     return n
 
 
+def _length(n) -> int:
+    try:
+        i = operator.index(n)
+    except TypeError:
+        i = -1
+    if i < 0:
+        raise ValueError(f"relative_bias: lengths are whole numbers from 0 on, got {n!r}")
+    return i
+
+
 def _scale(scale, D: int) -> float:
     s = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not abs(s) <= MAX_SCALE:
@@ -340,9 +350,7 @@ def relative_bias(bias: BucketBias, Lq: int, Lk: int, *, q_offset: int = 0):
         raise ValueError("relative_bias: a BucketBias is expected")
     t = _tensor(bias.table, "bias table", 2).contiguous()
     _rows(bias, t)
-    Lq, Lk, H = int(Lq), int(Lk), t.shape[1]
-    if Lq < 0 or Lk < 0:
-        raise ValueError(f"relative_bias: lengths {Lq} and {Lk}")
+    Lq, Lk, H = _length(Lq), _length(Lk), t.shape[1]
     _no_graph("relative_bias", t)
     ctx, stream = _where(t)
     out = t.new_empty((H, Lq, Lk))

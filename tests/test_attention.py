@@ -200,3 +200,11 @@ def test_a_scale_that_float32_cannot_hold():
     for s in (float("inf"), float("-inf"), float("nan"), 1e39, -1e39, 2.0 ** 127 * (1 + 2.0 ** -50)):
         refused("scale", A._scale, s, 64)
     assert A._scale(2.0 ** 127, 64) == 2.0 ** 127 and A._scale(None, 64) == 0.125
+
+
+def test_lengths_that_are_no_whole_numbers():
+    b = A.BucketBias(t(32, 4))
+    for n in (2.5, 3.0, "3", None, -1):
+        refused("lengths", A.relative_bias, b, n, 3)
+        refused("lengths", A.relative_bias, b, 3, n)
+    refused("CUDA", A.relative_bias, b, np.int64(3), 3)
