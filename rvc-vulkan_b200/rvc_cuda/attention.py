@@ -20,8 +20,9 @@ while grad mode is on (call under ``torch.no_grad()`` or inside an
 ``autograd.Function``, where it is off).  A wait inside a kernel that gives up
 (after two seconds) leaves NaN in the results that waited and is reported by the
 next ``sync`` of the device's context, ``rvc_cuda._lib.get_context(i).sync()``.
-``rvc_cuda.ops`` has the forms for numpy arrays.  The device code and its C entry points (``include/rvc_cuda.h``) have no counterpart
-in the reference, whose attention (``runtime/models/vits.py:993-1014``,
+``rvc_cuda.ops`` has the forms for numpy arrays.  The device code and its C entry
+points (``include/rvc_cuda.h``) have no counterpart in the reference, whose
+attention (``runtime/models/vits.py:993-1014``,
 ``runtime/models/hubert.py:1315-1400``) has one length, no padding and no
 gradient.  A shape, type or argument that is not served raises ``ValueError``.
 """
@@ -29,16 +30,14 @@ gradient.  A shape, type or argument that is not served raises ``ValueError``.
 from __future__ import annotations
 
 import ctypes as C
-import functools
-import math
-import operator
-import struct
 from typing import Optional
 
 import numpy as np
 import torch
 
 from . import _lib
+from ._attn_args import (MAX_BUCKETS, MAX_HEAD_DIM, MAX_SCALE, BucketBias, _length, _offset,  # noqa: F401
+                         _pack11, _pack25, _pack29, _scale, bucket_borders)
 from ._lib import check, lib
 
 __all__ = ["BucketBias", "attention", "attention_backward", "relative_bias", "relative_bias_backward",
@@ -49,69 +48,6 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda i: torch.cuda.current_stream(i).cuda_stream)
 _POSITION_BITS = {torch.int32: 32, torch.int64: 64}
-MAX_HEAD_DIM = 128
-MAX_BUCKETS = 1024
-MAX_SCALE = 2.0 ** 127  # times log2 e it is still a float32
-
-_pack29 = struct.Struct("=29q").pack
-_pack25 = struct.Struct("=25q").pack
-_pack11 = struct.Struct("=11q").pack
-
-
-@functools.lru_cache(maxsize=64)
-def bucket_borders(num_buckets: int, max_distance: int, bidirectional: bool = True) -> tuple:
-    """Smallest distances of the buckets 1, 2, ... of one direction.
-
-    With ``n`` buckets to a direction and ``e = n // 2``, distances below ``e``
-    have a bucket each; bucket ``e + k`` begins where ``(r / e)^(n - e)``
-    reaches ``(max_distance / e)^k``, decided on whole numbers so that no
-    rounding of a logarithm moves a border.
-    """
-    n = num_buckets // 2 if bidirectional else num_buckets
-    e = n // 2
-    borders = list(range(1, e + 1))
-    lo = e
-    for k in range(1, n - e):
-        want = max_distance ** k * e ** (n - e)
-        hi = max_distance
-        while lo < hi:  # smallest r with r^(n-e) e^k >= want
-            mid = (lo + hi) // 2
-            if mid ** (n - e) * e ** k >= want:
-                hi = mid
-            else:
-                lo = mid + 1
-        borders.append(lo)
-    return tuple(borders)
-
-
-class BucketBias:
-    """A learned bias of relative position: ``table [num_buckets, heads]``.
-
-    The bias of query ``i`` and key ``j`` is ``table[bucket(j - i), head]``.
-    ``bidirectional``: the first half of the rows holds distances of keys at or
-    behind the query, the second half those of keys ahead; otherwise every key
-    ahead counts as distance 0.  Distances of ``max_distance`` and more share
-    the last bucket.  The object holds the table itself (an optimiser may
-    change it in place between calls) and the borders of the buckets.
-    """
-
-    def __init__(self, table, max_distance: int = 128, bidirectional: bool = True):
-        if table.ndim != 2:
-            raise ValueError(f"BucketBias: table [num_buckets, heads] expected, got shape {tuple(table.shape)}")
-        n, max_distance = int(table.shape[0]), int(max_distance)
-        if bidirectional and n % 2:
-            raise ValueError(f"BucketBias: {n} buckets cannot be shared by two directions")
-        half = n // 2 if bidirectional else n
-        if half < 2 or n > MAX_BUCKETS:
-            raise ValueError(f"BucketBias: {n} buckets; 2 to {MAX_BUCKETS // (1 + bool(bidirectional))} to a direction "
-                             "are supported")
-        if not half // 2 < max_distance < 1 << 30:
-            raise ValueError(f"BucketBias: max_distance {max_distance} must exceed the {half // 2} single distances")
-        self.table = table
-        self.num_buckets, self.max_distance, self.bidirectional = n, max_distance, bool(bidirectional)
-        b = bucket_borders(n, max_distance, self.bidirectional)
-        self._borders = (C.c_int32 * max(1, len(b)))(*b)
-        self._nborders = len(b)
 
 
 # ------------------------------------------------------------------ plumbing
@@ -224,33 +160,6 @@ def _table(bias, H: int, like):
     if t.shape[1] != H:
         raise ValueError(f"bias: table {tuple(t.shape)}, expected [{bias.num_buckets}, {H}] for {H} query heads")
     return t.contiguous(), bias.num_buckets, int(bias.bidirectional), bias._borders, bias._nborders
-
-
-def _offset(q_offset) -> int:
-    try:
-        n = operator.index(q_offset)
-    except TypeError:
-        raise ValueError(f"q_offset: a whole number is expected, got {q_offset!r}") from None
-    if not -(1 << 31) <= n <= 1 << 31:
-        raise ValueError(f"q_offset {n} out of range")
-    return n
-
-
-def _length(n) -> int:
-    try:
-        i = operator.index(n)
-    except TypeError:
-        i = -1
-    if i < 0:
-        raise ValueError(f"relative_bias: lengths are whole numbers from 0 on, got {n!r}")
-    return i
-
-
-def _scale(scale, D: int) -> float:
-    s = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not abs(s) <= MAX_SCALE:
-        raise ValueError(f"attention: scale {s} is not finite in float32")
-    return s
 
 
 # ----------------------------------------------------------------- attention

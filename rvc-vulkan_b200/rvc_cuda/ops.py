@@ -9,14 +9,17 @@ does not take raise ``ValueError``, which the reference's ``nn`` callers catch
 to pick their own path (``runtime/nn.py:286-289``, ``:382-387``, ``:590-593``).
 
 ``buf_*`` arguments (the Vulkan engine's resident-buffer handles) are accepted
-and ignored.
+and ignored.  Nothing here needs torch.
 """
 
 from __future__ import annotations
 
+import ctypes as C
+
 import numpy as np
 
 from . import _lib
+from ._attn_args import MAX_HEAD_DIM, BucketBias, _length, _offset, _pack11, _pack25, _pack29, _scale
 from ._lib import check, fptr, iptr, lib
 
 __all__ = [
@@ -307,86 +310,235 @@ def im2col_1d(x, kernel_size, stride=1, padding=0, dilation=1):
 
 # ------------------------------------------------------- attention operators
 # Host forms of rvc_cuda.attention: float32 numpy arrays in and out, on the
-# default context's device.
+# default context's device and stream.  They need no torch.
 
 
-def _on_device(fn, arrays, **kw):
-    """``fn`` of ``rvc_cuda.attention`` on device copies of ``arrays``."""
-    import torch  # noqa: PLC0415
+class _Scratch:
+    """Device memory of one call: inputs, results and workspace from the context's
+    pool, given back when the call ends (the pool is reused in stream order)."""
 
-    dev = torch.device("cuda", _lib.get_context().device)
+    def __init__(self):
+        self.ctx = _lib.get_context()
+        self.handle, self.stream = self.ctx.handle, self.ctx.stream()
+        self.held = []
 
-    def up(a, dtype):
-        return torch.from_numpy(np.ascontiguousarray(a, dtype=dtype)).to(dev)
+    def __enter__(self):
+        return self
 
-    for n in ("kv_lens", "positions"):
-        if kw.get(n) is not None:
-            if not np.issubdtype(np.asarray(kw[n]).dtype, np.integer):
-                raise ValueError(f"{n}: integers are expected")
-            kw[n] = up(kw[n], np.int64)
-    if kw.get("key_mask") is not None:
-        kw["key_mask"] = up(kw["key_mask"], np.bool_)
-    if kw.get("bias") is not None:
-        kw["bias"] = _device_bias(kw["bias"], dev)
-    r = fn(*[up(a, np.float32) for a in arrays], **kw)
-    return tuple(x.cpu().numpy() for x in r) if isinstance(r, tuple) else r.cpu().numpy()
+    def __exit__(self, *exc):
+        for p in self.held:
+            self.ctx.free(p)
+
+    def new(self, nbytes: int) -> int:
+        p = self.ctx.alloc(max(16, nbytes))
+        self.held.append(p)
+        return p
+
+    def up(self, a):
+        """Device copy of an array (None stays None)."""
+        if a is None:
+            return None
+        p = self.new(a.nbytes)
+        if a.nbytes:
+            self.ctx.h2d(p, a)
+        return p
+
+    def out(self, *shapes):
+        return [self.new(4 * int(np.prod(s))) for s in shapes]
+
+    def workspace(self, fn, desc, n, *how):
+        need = C.c_int64(0)
+        check(fn(self.handle, desc, n, *how, need))
+        return (self.new(need.value) if need.value else None), need.value
+
+    def down(self, p: int, shape) -> np.ndarray:
+        a = np.empty(shape, np.float32)
+        if a.nbytes:
+            self.ctx.d2h(a, p)
+        return a
 
 
-def _device_bias(bias, dev):
-    import torch  # noqa: PLC0415
+def _dims(a, name: str, ndim: int) -> np.ndarray:
+    a = _f32(a)
+    if a.ndim != ndim:
+        raise ValueError(f"{name}: {ndim} dimensions expected, got shape {a.shape}")
+    return a
 
-    from . import attention as A  # noqa: PLC0415
 
-    if not isinstance(bias, A.BucketBias):
+def _whole(a, name: str) -> np.ndarray:
+    a = np.asarray(a)
+    if not np.issubdtype(a.dtype, np.integer):
+        raise ValueError(f"{name}: integers are expected")
+    return np.ascontiguousarray(a, dtype=np.int64)
+
+
+def _rows(a) -> tuple:
+    """Strides (batch, row, head) of a contiguous [B, L, H, D]."""
+    _, L, H, D = a.shape
+    return L * H * D, H * D, D
+
+
+def _host_bias(bias):
+    if not isinstance(bias, BucketBias):
         raise ValueError("bias: an rvc_cuda.attention.BucketBias is expected")
-    t = torch.from_numpy(_f32(bias.table)).to(dev)
-    return A.BucketBias(t, bias.max_distance, bias.bidirectional)
+    t = _dims(bias.table, "bias table", 2)
+    if t.shape[0] != bias.num_buckets:
+        raise ValueError(f"bias: table {t.shape}, its rows must be the {bias.num_buckets} buckets")
+    return t
+
+
+def _host_attention(q, k, v, kv_lens, key_mask, scale, causal, q_offset, bias, rest=()):
+    """(q, k, v, lens, mask, table, descriptor, scale, borders and their count); ``rest``: dout and out."""
+    q, k, v = _dims(q, "q", 4), _dims(k, "k", 4), _dims(v, "v", 4)
+    B, Lq, Hq, D = q.shape
+    Bk, Lk, Hkv, Dk = k.shape
+    if Bk != B or Dk != D or v.shape != k.shape:
+        raise ValueError(f"attention: q {q.shape}, k {k.shape}, v {v.shape} do not match [B, Lq, Hq, D] and [B, Lk, Hkv, D]")
+    if not 1 <= D <= MAX_HEAD_DIM:
+        raise ValueError(f"attention: head dimension {D}; 1 to {MAX_HEAD_DIM} are supported")
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"attention: {Hq} query heads are no multiple of {Hkv} key heads")
+    lens = mask = table = None
+    if kv_lens is not None:
+        lens = _whole(kv_lens, "kv_lens")
+        if lens.shape != (B,):
+            raise ValueError(f"kv_lens: [{B}] expected, got {lens.shape}")
+    if key_mask is not None:
+        mask = np.ascontiguousarray(key_mask, dtype=np.bool_)
+        if mask.shape != (B, Lk):
+            raise ValueError(f"key_mask: [{B}, {Lk}] expected, got {mask.shape}")
+    if bias is not None:
+        table = _host_bias(bias)
+        if table.shape[1] != Hq:
+            raise ValueError(f"bias: table {table.shape}, expected [{bias.num_buckets}, {Hq}] for {Hq} query heads")
+    desc = _pack29(0, B, Hq, Hkv, Lq, Lk, D, *_rows(q), *_rows(k), *_rows(v), 64 if lens is not None else 0,
+                   Lk if mask is not None else 0, 1 if mask is not None else 0, bool(causal), _offset(q_offset),
+                   bias.num_buckets if bias is not None else 0, bias.bidirectional if bias is not None else 0,
+                   *(_rows(q) * 2 if rest else (0,) * 6))
+    borders, n = (bias._borders, bias._nborders) if bias is not None else (None, 0)
+    return q, k, v, lens, mask, table, desc, _scale(scale, D), borders, n
 
 
 def attention(q, k, v, kv_lens=None, key_mask=None, scale=None, causal=False, q_offset=0, bias=None):
     """``rvc_cuda.attention.attention`` for numpy arrays: ``q [B, Lq, Hq, D]``,
     ``k, v [B, Lk, Hkv, D]`` -> ``(out, lse)``; the table of ``bias`` (a
     ``BucketBias``) is a numpy array too."""
-    from . import attention as A  # noqa: PLC0415
-
-    return _on_device(A.attention, (q, k, v), kv_lens=kv_lens, key_mask=key_mask, scale=scale, causal=causal,
-                      q_offset=q_offset, bias=bias)
+    q, k, v, lens, mask, table, desc, scale, borders, n = _host_attention(q, k, v, kv_lens, key_mask, scale, causal,
+                                                                          q_offset, bias)
+    B, Lq, Hq, _ = q.shape
+    with _Scratch() as d:
+        out, lse = d.out(q.shape, (B, Hq, Lq))
+        ws, nbytes = d.workspace(lib.rvc_cuda_attention_workspace, desc, 29, 0)
+        check(lib.rvc_cuda_attention_device(d.handle, d.stream, desc, 29, scale, d.up(q), d.up(k), d.up(v), d.up(lens),
+                                            d.up(mask), d.up(table), borders, n, out, lse, ws, nbytes))
+        return d.down(out, q.shape), d.down(lse, (B, Hq, Lq))
 
 
 def attention_backward(dout, q, k, v, out, lse, kv_lens=None, key_mask=None, scale=None, causal=False, q_offset=0,
                        bias=None):
     """``rvc_cuda.attention.attention_backward`` for numpy arrays."""
-    from . import attention as A  # noqa: PLC0415
-
-    return _on_device(A.attention_backward, (dout, q, k, v, out, lse), kv_lens=kv_lens, key_mask=key_mask, scale=scale,
-                      causal=causal, q_offset=q_offset, bias=bias)
+    q, k, v, lens, mask, table, desc, scale, borders, n = _host_attention(q, k, v, kv_lens, key_mask, scale, causal,
+                                                                          q_offset, bias, (dout, out))
+    dout, out, lse = _dims(dout, "dout", 4), _dims(out, "out", 4), _dims(lse, "lse", 3)
+    B, Lq, Hq, _ = q.shape
+    if dout.shape != q.shape or out.shape != q.shape:
+        raise ValueError(f"attention_backward: dout {dout.shape} and out {out.shape} must have the shape of q {q.shape}")
+    if lse.shape != (B, Hq, Lq):
+        raise ValueError(f"attention_backward: lse must be [{B}, {Hq}, {Lq}], got {lse.shape}")
+    with _Scratch() as d:
+        shapes = [q.shape, k.shape, v.shape] + ([table.shape] if table is not None else [])
+        grads = d.out(*shapes)
+        ws, nbytes = d.workspace(lib.rvc_cuda_attention_workspace, desc, 29, 1)
+        check(lib.rvc_cuda_attention_backward_device(
+            d.handle, d.stream, desc, 29, scale, d.up(dout), d.up(q), d.up(k), d.up(v), d.up(out), d.up(lse), d.up(lens),
+            d.up(mask), d.up(table), borders, n, *grads[:3], grads[3] if table is not None else None, ws, nbytes))
+        return tuple(d.down(p, s) for p, s in zip(grads, shapes))
 
 
 def relative_bias(bias, Lq, Lk, q_offset=0):
     """``rvc_cuda.attention.relative_bias`` with a numpy table -> ``[heads, Lq, Lk]``."""
-    from . import attention as A  # noqa: PLC0415
-
-    return _on_device(lambda **kw: A.relative_bias(kw["bias"], Lq, Lk, q_offset=q_offset), (), bias=bias)
+    table = _host_bias(bias)
+    shape = (table.shape[1], _length(Lq), _length(Lk))
+    desc = _pack11(0, 1, *shape, _offset(q_offset), bias.num_buckets, bias.bidirectional, 0, 0, 0)
+    with _Scratch() as d:
+        out, = d.out(shape)
+        check(lib.rvc_cuda_relative_bias_device(d.handle, d.stream, desc, 11, d.up(table), bias._borders, bias._nborders,
+                                                out))
+        return d.down(out, shape)
 
 
 def relative_bias_backward(bias, dbias, q_offset=0):
     """``rvc_cuda.attention.relative_bias_backward`` for numpy arrays."""
-    from . import attention as A  # noqa: PLC0415
+    table, dbias = _host_bias(bias), _f32(dbias)
+    dbias = _dims(dbias[None] if dbias.ndim == 3 else dbias, "dbias", 4)
+    B, H, Lq, Lk = dbias.shape
+    if H != table.shape[1]:
+        raise ValueError(f"relative_bias_backward: {H} heads, the table has {table.shape[1]}")
+    desc = _pack11(0, B, H, Lq, Lk, _offset(q_offset), bias.num_buckets, bias.bidirectional, H * Lq * Lk, Lq * Lk, Lk)
+    with _Scratch() as d:
+        out, = d.out(table.shape)
+        ws, nbytes = d.workspace(lib.rvc_cuda_relative_bias_workspace, desc, 11)
+        check(lib.rvc_cuda_relative_bias_backward_device(d.handle, d.stream, desc, 11, d.up(dbias), bias._borders,
+                                                         bias._nborders, out, ws, nbytes))
+        return d.down(out, table.shape)
 
-    return _on_device(lambda d, bias: A.relative_bias_backward(bias, d, q_offset=q_offset), (dbias,), bias=bias)
+
+def _host_rope(q, k, q_weight, k_weight, cos, sin, positions, interleaved, name, grads=()):
+    """The arrays, and the descriptor."""
+    q, k = _dims(q, "q", 4), _dims(k, "k", 4)
+    wq, wk, cos, sin = _dims(q_weight, "q_weight", 1), _dims(k_weight, "k_weight", 1), _dims(cos, "cos", 2), _dims(sin, "sin", 2)
+    B, L, Hq, D = q.shape
+    if k.shape[:2] != (B, L) or k.shape[3] != D:
+        raise ValueError(f"{name}: q {q.shape} and k {k.shape} do not match [B, L, heads, D]")
+    if D < 2 or D > 256 or D % 2:
+        raise ValueError(f"{name}: head dimension {D}; even ones from 2 to 256 are supported")
+    if wq.shape != (D,) or wk.shape != (D,):
+        raise ValueError(f"{name}: weights [{D}] expected, got {wq.shape} and {wk.shape}")
+    if cos.shape != sin.shape or 2 * cos.shape[1] > D:
+        raise ValueError(f"{name}: cos {cos.shape} and sin {sin.shape} do not fit head dimension {D}")
+    bits = pb = pl = 0
+    pos = None
+    if positions is not None:
+        pos = _whole(positions, "positions")
+        if pos.shape == (B, L):
+            pb, pl = L, 1
+        elif pos.shape == (L,):
+            pl = 1
+        else:
+            raise ValueError(f"{name}: positions [{B}, {L}] or [{L}] expected, got {pos.shape}")
+        bits = 64
+    elif L > cos.shape[0] and cos.shape[1]:
+        raise ValueError(f"{name}: the tables hold {cos.shape[0]} positions, fewer than the {L} rows")
+    grads = [_dims(g, n, 4) for g, n in zip(grads, ("dqo", "dko"))]
+    for g, x in zip(grads, (q, k)):
+        if g.shape != x.shape:
+            raise ValueError(f"{name}: a gradient {g.shape} for {x.shape}")
+    desc = _pack25(0, 0, B, L, Hq, k.shape[2], D, 2 * cos.shape[1], cos.shape[0], bool(interleaved), bits, pb, pl,
+                   *_rows(q), *_rows(k), *(_rows(q) + _rows(k) if grads else (0,) * 6))
+    return [*grads, q, k, wq, wk, cos, sin, pos], desc
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, interleaved=False):
     """``rvc_cuda.attention.qk_norm_rope`` for numpy arrays."""
-    from . import attention as A  # noqa: PLC0415
-
-    return _on_device(A.qk_norm_rope, (q, k, q_weight, k_weight, cos, sin), positions=positions, eps=eps,
-                      interleaved=interleaved)
+    arrays, desc = _host_rope(q, k, q_weight, k_weight, cos, sin, positions, interleaved, "qk_norm_rope")
+    shapes = [a.shape for a in arrays[:2]]
+    with _Scratch() as d:
+        out = d.out(*shapes)
+        check(lib.rvc_cuda_qk_norm_rope_device(d.handle, d.stream, desc, 25, float(eps), *map(d.up, arrays), *out))
+        return tuple(d.down(p, s) for p, s in zip(out, shapes))
 
 
 def qk_norm_rope_backward(dqo, dko, q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, interleaved=False):
     """``rvc_cuda.attention.qk_norm_rope_backward`` for numpy arrays."""
-    from . import attention as A  # noqa: PLC0415
-
-    return _on_device(A.qk_norm_rope_backward, (dqo, dko, q, k, q_weight, k_weight, cos, sin), positions=positions,
-                      eps=eps, interleaved=interleaved)
+    arrays, desc = _host_rope(q, k, q_weight, k_weight, cos, sin, positions, interleaved, "qk_norm_rope_backward",
+                              (dqo, dko))
+    shapes = [a.shape for a in arrays[2:6]]
+    with _Scratch() as d:
+        out = d.out(*shapes)
+        ws, nbytes = d.workspace(lib.rvc_cuda_qk_norm_rope_workspace, desc, 25)
+        check(lib.rvc_cuda_qk_norm_rope_backward_device(d.handle, d.stream, desc, 25, float(eps), *map(d.up, arrays), *out,
+                                                        ws, nbytes))
+        r = [d.down(p, s) for p, s in zip(out, shapes)]
+    if arrays[3].shape[2] == 0:  # no keys: nobody writes their weight's gradient
+        r[3][:] = 0
+    return tuple(r)

@@ -208,3 +208,66 @@ def test_lengths_that_are_no_whole_numbers():
         refused("lengths", A.relative_bias, b, n, 3)
         refused("lengths", A.relative_bias, b, 3, n)
     refused("CUDA", A.relative_bias, b, np.int64(3), 3)
+
+
+# ------------------------------------------------------- host forms, no torch
+
+WITHOUT_TORCH = """
+import sys
+sys.path[:0] = {paths!r}
+sys.modules["torch"] = None  # an import of torch raises
+import numpy as np
+from rvc_cuda import ops
+"""
+
+
+def without_torch(body):
+    """Runs ``body`` in an interpreter that cannot import torch."""
+    import subprocess
+    import sys
+
+    from tests.conftest import PKG, ROOT
+
+    r = subprocess.run([sys.executable, "-c", WITHOUT_TORCH.format(paths=[ROOT, PKG]) + body], capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_host_forms_refuse_without_torch():
+    """The operator module and its refusals (before the device is touched) work where there is no torch."""
+    without_torch("""
+def refused(word, fn, *a, **k):
+    try:
+        fn(*a, **k)
+    except ValueError as e:
+        assert word in str(e), (word, str(e))
+    else:
+        raise AssertionError(word)
+
+t = lambda *s: np.zeros(s, np.float32)
+q, k, w, c, b = t(2, 5, 4, 16), t(2, 7, 2, 16), t(16), t(9, 8), ops.BucketBias(t(8, 4))
+refused("dimensions", ops.attention, q[0], k, k)
+refused("do not match", ops.attention, q, k, t(2, 8, 2, 16))
+refused("no multiple", ops.attention, q, t(2, 7, 3, 16), t(2, 7, 3, 16))
+refused("head dimension", ops.attention, t(1, 1, 1, 129), t(1, 1, 1, 129), t(1, 1, 1, 129))
+refused("integers", ops.attention, q, k, k, kv_lens=[1.5, 2.0])
+refused("kv_lens", ops.attention, q, k, k, kv_lens=[1, 2, 3])
+refused("key_mask", ops.attention, q, k, k, key_mask=np.ones((2, 6)))
+refused("BucketBias", ops.attention, q, k, k, bias=t(8, 4))
+refused("4 query heads", ops.attention, q, k, k, bias=ops.BucketBias(t(8, 2)))
+refused("scale", ops.attention, q, k, k, scale=1e39)
+refused("q_offset", ops.attention, q, k, k, q_offset=1.5)
+refused("shape of q", ops.attention_backward, q[:, :4], q, k, k, q, t(2, 4, 5))
+refused("lse", ops.attention_backward, q, q, k, k, q, t(2, 5, 4))
+refused("lengths", ops.relative_bias, b, -1, 3)
+refused("heads", ops.relative_bias_backward, b, t(3, 5, 6))
+refused("dbias", ops.relative_bias_backward, b, t(5, 6))
+b.table = t(7, 4)
+refused("8 buckets", ops.relative_bias, b, 3, 3)
+refused("do not match", ops.qk_norm_rope, q, k, w, w, c, c)
+refused("weights", ops.qk_norm_rope, q, q, t(8), w, c, c)
+refused("fit head", ops.qk_norm_rope, q, q, w, w, t(9, 9), t(9, 9))
+refused("fewer", ops.qk_norm_rope, q, q, w, w, t(4, 8), t(4, 8))
+refused("positions", ops.qk_norm_rope, q, q, w, w, c, c, positions=np.zeros((2, 4), int))
+refused("gradient", ops.qk_norm_rope_backward, q[:, :4], q, q, q, w, w, c, c)
+""")

@@ -256,3 +256,74 @@ def test_the_entry_points_refuse_misaligned_lengths_tables_and_positions():
                                                               sin, pos, p[4], p[5], w, w, at, 1 << 20) == _lib.RVC_E_ARG
         assert "misaligned positions" in _lib.last_error()
     assert _lib.launch_count() == n0
+
+
+# ------------------------------------------------------------------ host forms
+
+
+def test_host_forms_without_torch():
+    """The numpy forms run where torch cannot be imported."""
+    from tests.test_attention import without_torch
+
+    without_torch("""
+from oracle import attention as OA
+rs = np.random.RandomState(0)
+n = lambda *s: rs.standard_normal(s).astype(np.float32)
+q, k, v, do, bias = n(2, 30, 4, 32), n(2, 41, 2, 32), n(2, 41, 2, 32), n(2, 30, 4, 32), ops.BucketBias(n(16, 4), 30, True)
+lens = np.array([41, 20])
+out, lse = ops.attention(q, k, v, kv_lens=lens, bias=bias)
+live = OA.alive(2, 30, 41, lens)
+where = OA.bucket(np.arange(41)[None] - np.arange(30)[:, None], 16, 30, True)
+o, z, _ = OA.attention(q, k, v, 32 ** -0.5, live, bias.table.T[:, where])
+assert np.abs(out - o).max() <= 2.0 ** -15 and np.abs(lse - z).max() <= 2.0 ** -15
+got = ops.attention_backward(do, q, k, v, out, lse, kv_lens=lens, bias=bias)
+want = OA.attention_backward(do, q, k, v, 32 ** -0.5, live, bias.table.T[:, where], where, 16)
+for a, b in zip(got, want):
+    assert np.abs(a - b).max() <= 2.0 ** -13 * max(1.0, np.abs(b).max())
+assert (ops.relative_bias(bias, 30, 41) == bias.table.T[:, where]).all()
+assert ops.relative_bias_backward(bias, n(4, 30, 41)).shape == (16, 4)
+g, ang = n(32), n(41, 16)
+a, b = ops.qk_norm_rope(k, v, g, g, np.cos(ang), np.sin(ang))
+pos = np.broadcast_to(np.arange(41), (2, 41))
+assert np.abs(b - OA.norm_rope(v, g, np.cos(ang), np.sin(ang), pos, 1e-6, False)).max() <= 2.0 ** -17 * 16
+assert len(ops.qk_norm_rope_backward(a, b, k, v, g, g, np.cos(ang), np.sin(ang), positions=np.arange(41))) == 4
+""")
+
+
+def test_host_forms_are_the_tensor_forms():
+    """Same bits as the calls on tensors, empty sizes and every option included."""
+    from rvc_cuda import ops
+
+    rs = np.random.RandomState(1)
+    n = lambda *s: rs.standard_normal(s).astype(np.float32)  # noqa: E731
+    up = lambda x: torch.from_numpy(np.ascontiguousarray(x)).cuda()  # noqa: E731
+
+    def same(a, b):
+        a, b = (x if isinstance(x, tuple) else (x,) for x in (a, b))
+        assert len(a) == len(b)
+        for x, y in zip(a, b):
+            np.testing.assert_array_equal(x, y.cpu().numpy())
+
+    for B, Lq, Lk, Hq, Hkv, D in ((2, 30, 41, 4, 2, 32), (1, 1, 300, 3, 3, 7), (2, 70, 90, 2, 1, 64), (1, 3, 0, 2, 2, 8),
+                                  (0, 3, 5, 2, 2, 8), (1, 0, 5, 2, 1, 8)):
+        q, k, v, do = n(B, Lq, Hq, D), n(B, Lk, Hkv, D), n(B, Lk, Hkv, D), n(B, Lq, Hq, D)
+        tab, lens, keep = n(16, Hq), rs.randint(0, Lk + 2, B), rs.rand(B, Lk) < 0.7
+        for kw in ({}, dict(scale=0.3, causal=True, q_offset=4), dict(kv_lens=lens, key_mask=keep, bias=tab, q_offset=-2)):
+            th = {x: up(y) if isinstance(y, np.ndarray) else y for x, y in kw.items()}
+            if "bias" in kw:
+                kw, th = dict(kw, bias=A.BucketBias(tab, 30, True)), dict(th, bias=A.BucketBias(up(tab), 30, True))
+            r = A.attention(up(q), up(k), up(v), **th)
+            h = ops.attention(q, k, v, **kw)
+            same(h, r)
+            same(ops.attention_backward(do, q, k, v, *h, **kw), A.attention_backward(up(do), up(q), up(k), up(v), *r, **th))
+        b, bt = A.BucketBias(tab, 30, False), A.BucketBias(up(tab), 30, False)
+        same(ops.relative_bias(b, Lq, Lk, 3), A.relative_bias(bt, Lq, Lk, q_offset=3))
+        d = n(B, Hq, Lq, Lk)
+        same(ops.relative_bias_backward(b, d, 3), A.relative_bias_backward(bt, up(d), q_offset=3))
+    for B, L, Hq, Hk, D, R in ((2, 5, 4, 2, 64, 64), (1, 9, 3, 0, 18, 6), (0, 4, 1, 1, 8, 8), (2, 3, 1, 1, 32, 0)):
+        q, k, gq, gk, ang = n(B, L, Hq, D), n(B, L, Hk, D), n(B, L, Hq, D), n(B, L, Hk, D), n(20, R // 2)
+        x = (q, k, n(D), n(D), np.cos(ang), np.sin(ang))
+        for kw in ({}, dict(positions=rs.randint(0, 20, (B, L)), interleaved=True, eps=1e-3), dict(positions=rs.randint(0, 20, L))):
+            th = {a: up(y) if isinstance(y, np.ndarray) else y for a, y in kw.items()}
+            same(ops.qk_norm_rope(*x, **kw), A.qk_norm_rope(*map(up, x), **th))
+            same(ops.qk_norm_rope_backward(gq, gk, *x, **kw), A.qk_norm_rope_backward(up(gq), up(gk), *map(up, x), **th))
