@@ -411,8 +411,8 @@ int32_t rvc_cuda_to_int16(int64_t ctx, const float* x, int64_t n, int16_t* y);
  * Hq a multiple of Hkv.  Key j of batch entry b is alive when j < kv_lens[b]
  * (clamped to [0, Lk]), key_mask[b, j] != 0 and, when causal, j <= i + q_offset;
  * nothing of the k or v of a key that no query meets reaches a result, whatever it
- * holds (a key that is causally dead for some queries only has to be finite: its
- * weight there is 0, which meets the value).  A query without a live key gives
+ * holds (a key that is causally dead for some queries only, or dead by the table
+ * alone, has to be finite: its weight there is 0, which meets the value).  A query without a live key gives
  * out = 0, lse = -inf and zero gradients.
  * table [buckets, Hq] (in `type`) adds table[bucket(j - i - q_offset), h] to the
  * scaled score; an entry below -65536 (-inf, -1e9, the lowest float32 or bfloat16)
@@ -420,7 +420,9 @@ int32_t rvc_cuda_to_int16(int64_t ctx, const float* x, int64_t n, int16_t* y);
  * entries and scores are meant to stay below 1e5 in size: gradients take their
  * weights from the float32 log sums.  borders (host, int32) are the smallest
  * distances of the buckets 1, 2, ... of one direction.  out [B, Lq, Hq, D]
- * contiguous, lse [B, Hq, Lq] float32 (natural logarithm). */
+ * contiguous, lse [B, Hq, Lq] float32 (natural logarithm).  The workspace of the
+ * backward pass grows with Lq Lk where there is a table: up to B Hq Lq Lk / 16
+ * bytes. */
 int32_t rvc_cuda_attention_workspace(int64_t ctx, const int64_t* desc, int32_t ndesc, int32_t backward,
                                      int64_t* bytes);
 int32_t rvc_cuda_attention_device(int64_t ctx, void* stream, const int64_t* desc, int32_t ndesc, double scale,

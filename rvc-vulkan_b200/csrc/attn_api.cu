@@ -102,6 +102,10 @@ __global__ void bucket_sums_kernel(const double* __restrict__ sums, const double
   if (threadIdx.x == 0) dtable[(long long)b * H + h] = from_f<T>((float)red[0]);
 }
 
+// Workspace.  The largest part is the table's gradient: the diagonal sums of every
+// tile of every (batch entry, query head), 4 B Hq (Lk / 128) (Lq + 130) bytes on the
+// 16-bit tiles (twice for heads above 64), 4 B Hq (Lq / 64) (Lk + 64) elsewhere: 8.6
+// GB for 32 heads of 128 at 65536 x 65536.
 struct Layout {
   int64_t diag = -1, po = -1, pml = -1, delta = -1, lse2 = -1, dws = -1, sums = -1, far = -1, split = -1, bytes = 0;
   int nsplit = 1, BM = 64, nt = 0;

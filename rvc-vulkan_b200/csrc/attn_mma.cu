@@ -21,10 +21,11 @@
 // staged as zeros: whatever the caller's buffer holds there, NaN included, never
 // meets a product.
 //
-// Measured: one row, 12 heads, 499 keys of 64, bf16: 6 to 8 us; 32 x 4 key heads of
-// 128, ragged to 8192 keys: 89 us (3.8 TB/s; 580 instructions per 16 keys of a
-// warp); fp32 gradients of 4 x 2 x 1000 x 1000 x 96 with a bias: 410 us (tensor
-// pipe busy a third of the time: eight warps to an SM and their splitting).
+// Measured: one row, 12 heads, 499 keys of 64, bf16: 8.8 us alone and cold (the
+// call is 17 to 18, its host part); 32 x 4 key heads of 128, ragged to 8192 keys:
+// 89 to 95 us (3.6 TB/s; 580 instructions per 16 keys of a warp); fp32 gradients of
+// 4 x 2 x 1000 x 1000 x 96 with a bias: 417 us (tensor pipe busy 23 and 30 % of the
+// two kernels: eight warps to an SM, which load, split and multiply in turn).
 #include "attn_common.cuh"
 #include "context.cuh"
 #include "tc_ptx.cuh"

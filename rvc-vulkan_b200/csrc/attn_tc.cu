@@ -21,10 +21,10 @@
 // Every wait is bounded; one that gives up sets the context's error word, lets the
 // block wind down and leaves NaN in the rows that are not finished.
 //
-// Measured: 2 x 16/4 heads x 2048 x 16384 x 128, bf16: 485 to 551 us, 1.0 to 1.13
-// PFLOP/s of 1.70; the same pipeline with the softmax taken out takes 433, so the
+// Measured: 2 x 16/4 heads x 2048 x 16384 x 128, bf16: 485 to 555 us from box to
+// box, 0.99 to 1.13 PFLOP/s of 1.70; the same pipeline with the softmax taken out takes 433, so the
 // products and their two waves of blocks bound it.  4 x 16 x 2047 x 2047 x 64 with
-// the bias, fp16: 160 us, of which 38 are the look-ups of the bias.  Sixteen
+// the bias, fp16: 159 us, of which 38 are the look-ups of the bias.  Sixteen
 // softmax warps (two to a row) took 895 us for the first, exponentials by
 // polynomial for one pair in eight 588 against 511.
 #include "attn_tc.cuh"
@@ -494,9 +494,17 @@ void fwd_t(const AttnArgs& a, cudaStream_t st) {
 
 // 16-bit operands that TMA can address, and queries enough: the general kernel
 // fills its tiles with the rows of a whole group, this one leaves them empty.
-// Measured in us, general / tiles (6831 keys): 12 heads of 64, 20 queries 38 / 32;
-// 8 x 16/4 heads of 128, 20 queries 199 / 111, 6 queries 105 / 111; 4 x 64/8 heads
-// of 64, 32 queries 141 / 198, 48 queries 204 / 198.
+// Measured in us, general / tiles, at 20, 32 and 48 queries (6831 keys unless said):
+//   heads of 128   8 x 16/4  191 / 107  181 / 107  235 / 107 (6 queries 98 / 107)
+//                  4 x 64/8  233 / 211  308 / 211  450 / 211
+//   12 heads of 64  33 / 26   34 / 27   35 / 27;  8 x 12  102 / 98 at 20 to 64
+//   64, groups of 2 to 4   8 x 16/4  85 / 98  87 / 98  104 / 98;  1 x 16/4  35 / 26
+//       35 / 27  36 / 27;  8 x 8/4  49 / 56  50 / 56  85 / 56;  8 x 16/4 on 499
+//       keys  17 / 13  17 / 13  19 / 13;  on 1499 keys  28 / 27  28 / 27  32 / 27
+//   64, groups of 8   4 x 64/8  103 / 193  136 / 193  198 / 193
+// So for heads of up to 64 in groups of 2 to 4 the general kernel is ahead (12 to 15
+// %) at 20 to 32 queries of large batches on thousands of keys, and the tiles
+// elsewhere (by up to a third): they take the whole range.
 bool attn_tc_fits(const AttnArgs& a) {
   const int least = a.D > 64 || a.Hq / a.Hkv <= 4 ? 20 : 48;
   return a.type != kF32 && a.Lq >= least && a.Lk >= 1 && atc::map_ok(a, a.q, a.qs, a.Lq, a.Hq) &&

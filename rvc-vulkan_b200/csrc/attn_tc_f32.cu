@@ -17,8 +17,9 @@
 //   P = 2^(s - m) in three parts,  O_t = P V in the same order,
 //   o = (o + O_(t-2)) 2^(m_old - m) in registers, rounded as fp32.
 //
-// Measured: 8 x 12 x 499 x 1499 x 64, padded: 210 us, about 35 of them for the parts
-// (the general kernel: 369); error 2e-7 of the output's norm.
+// Measured: 8 x 12 x 499 x 1499 x 64, padded: 202 to 223 us, about 35 of them for
+// the parts (the general kernel: 369; tensor pipe busy 26 %, captured alone); error
+// 2e-7 of the output's norm.
 #include "attn_tc.cuh"
 #include "context.cuh"
 

@@ -5,9 +5,10 @@
 // from a row of Lq + Lk - 1 values, the backward pass reads every pair once
 // into as many sums, and a small kernel adds those up per bucket.
 //
-// Measured: 12 x 499 x 1499 fp32 written in 11 us (36 MB, the host's share of the
-// call is as long); the gradient of 4 x 16 x 4095 x 4095 bf16 (2.1 GB) in 424 to 438
-// us, 364 of them the pass at 5.9 TB/s.
+// Measured: 12 x 499 x 1499 fp32 written in 11 us (36 MB; that is the kernel, alone
+// and cold: each block waits for its look-ups, which search the borders with
+// divergent indices, and then stores four bytes a thread); the gradient of 4 x 16 x
+// 4095 x 4095 bf16 (2.1 GB) in 424 to 439 us, 368 of them the pass (73 % of DRAM).
 #include "attn_common.cuh"
 #include "context.cuh"
 

@@ -175,8 +175,8 @@ def attention(q, k, v, *, kv_lens=None, key_mask=None, scale: Optional[float] = 
     ``i + q_offset`` for query ``i`` (``q_offset = Lk - Lq`` aligns the last
     query with the last key).  Whatever a key holds that no query meets reaches
     no result: padding, masked keys, a cache past the last query's limit.  A key
-    that is past the limit of some queries only must be finite, as its weight of
-    0 there meets the value.
+    that is past the limit of some queries only, or masked by the bias alone, must
+    be finite, as its weight of 0 there meets the value.
     Query head ``h`` reads key head ``h // (Hq / Hkv)``.  ``scale`` is
     ``1 / sqrt(D)`` by default; ``bias`` adds ``table[bucket(j - i - q_offset),
     h]`` (an entry below -65536 masks its pairs: ``-inf``, ``-1e9``, the lowest
@@ -220,8 +220,12 @@ def attention_backward(dout, q, k, v, out, lse, *, kv_lens=None, key_mask=None, 
     Returns ``(dq, dk, dv)``, and ``dtable [num_buckets, Hq]`` behind them when
     a ``bias`` is given, in the types of their inputs; a key head's gradient is
     the sum over the query heads that share it.  Dead keys and queries without
-    a live key get zeros.  Sums run in a fixed order: the same call gives the
-    same bits.
+    a live key get zeros, and so do ``q``, ``k`` and the table from a query that
+    length, mask and causal limit leave one key.  Sums run in a fixed order: the
+    same call gives the same bits.  With a ``bias`` the scratch memory grows with
+    ``Lq Lk``, up to ``B Hq Lq Lk / 16`` bytes.  float16 gradients want a loss
+    scale that keeps ``p (dout v - sum p dout v)``, which is rounded to float16 on
+    the way, between its subnormals and 65504.
     """
     q, k, v, B, Lq, Lk, Hq, Hkv, D = _qkv(q, k, v)
     dout, out = _tensor(dout, "dout", 4, q), _tensor(out, "out", 4, q)
