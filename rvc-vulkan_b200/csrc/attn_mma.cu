@@ -115,8 +115,6 @@ template <typename T, int DP> constexpr int tile_bytes(int rows) { return kParts
 struct Rows {
   uint32_t at, part;
 };
-template <typename T> struct MmaType { using type = T; };
-template <> struct MmaType<float> { using type = __nv_bfloat16; };
 
 // x = hi + mid + lo in bf16 for two values at once, each rounded from what is left.
 __device__ __forceinline__ void split3(float a, float b, uint32_t (&w)[3]) {
