@@ -22,10 +22,10 @@
 // block wind down and leaves NaN in the rows that are not finished.
 //
 // Measured: 2 x 16/4 heads x 2048 x 16384 x 128, bf16: 485 to 555 us from run to
-// run, 0.99 to 1.13 PFLOP/s of 1.70; the same pipeline with the softmax taken out takes 433, so the
-// products and their two waves of blocks bound it.  4 x 16 x 2047 x 2047 x 64 with
-// the bias, fp16: 159 us, of which 38 are the look-ups of the bias.  Sixteen
-// softmax warps (two to a row) took 895 us for the first, exponentials by
+// run, 0.99 to 1.13 PFLOP/s of 1.70; the same pipeline with the softmax taken out
+// takes 433, so the products and their two waves of blocks bound it.  4 x 16 x 2047
+// x 2047 x 64 with the bias, fp16: 159 us, of which 38 are the look-ups of the bias.
+// Sixteen softmax warps (two to a row) took 895 us for the first, exponentials by
 // polynomial for one pair in eight 588 against 511.
 #include "attn_tc.cuh"
 #include "context.cuh"
